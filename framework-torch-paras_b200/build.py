@@ -26,9 +26,10 @@ PKG = os.path.join(HERE, "python", "torch_paras")
 OBJ = os.path.join(HERE, "build")
 
 CUDA_SOURCES = ["runtime.cu", "elementwise.cu", "rmsnorm.cu", "sdpa.cu", "sdpa_simt.cu",
-                "sdpa_tc.cu", "sdpa_decode.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_skinny.cu", "sdpa_bwd.cu", "sdpa_bwd_tc.cu", "sdpa_bwd_general.cu", "sdpa_weights.cu", "selftest.cu"]
+                "sdpa_tc.cu", "sdpa_decode.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_skinny.cu", "sdpa_bwd.cu", "sdpa_bwd_tc.cu", "sdpa_bwd_general.cu", "sdpa_weights.cu", "selftest.cu",
+                "paged_kv.cu", "paged_attn.cu", "add_rmsnorm.cu"]
 EXT_SOURCES = ["core/device_runtime.cpp", "ops/lifecycle_ops.cpp", "ops/attention_ops.cpp",
-               "ops/norm_glu_ops.cpp", "ops/matmul_ops.cpp", "python/module.cpp"]
+               "ops/norm_glu_ops.cpp", "ops/matmul_ops.cpp", "ops/paged_ops.cpp", "python/module.cpp"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-diag-suppress", "177,550"]

@@ -1,0 +1,597 @@
+// Residual addition and RMSNorm in one pass, with a 16-bit / fp32 or an 8-bit output, and its gradient
+// (include/paras_b200.h, "residual addition and RMSNorm in one pass").  HBM-bound: x and residual are read once, h
+// and y written once; composed of add, rms_norm and a quantising pass the same work moves h three times more.
+//
+//   h = T(x + r)      the sum every later layer sees, so the statistics are taken of the rounded value and the
+//                     backward pass needs h alone
+//   rstd = 1 / sqrt(mean(h^2) + eps)          sums in fp32 per thread (at most 32 squares each), in double across them
+//   y = h * rstd * w                          fp32, rounded once: to T, or to e4m3 of y / scale
+//   scale = max(max|y| / 448, 2^-126)         over a row or over 32 / 64 / 128 columns
+//
+// Backward, with n = h * rstd and a = grad_y * w:
+//   grad_x = rstd * (a - n * mean(a * n)) + grad_h          grad_w = sum over rows of grad_y * n
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "paged_common.cuh"
+
+namespace pb {
+namespace {
+
+struct NormParams {
+    const void *x, *r, *w;
+    void *h, *y;        // y: T, or e4m3 bytes
+    float *rstd, *scales;
+    int64_t rows, H;
+    int64_t groups;     // scales per row
+    int group;          // columns per scale, 0 = the row
+    double eps;
+};
+
+constexpr float kScaleMin = 1.1754943508222875e-38f;   // 2^-126
+__device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax * (1.0f / 448.0f), kScaleMin); }
+
+// TPR threads hold a row in registers, V vectors of 16 bytes each (rows whole and aligned in such vectors).
+template <typename T, int TPR, int V, bool QUANT>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+add_rmsnorm_rows_kernel(const NormParams p) {
+    constexpr int N = Vec16<T>::N;
+    constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
+    constexpr int kW = TPR / 32;
+    static_assert(TPR % 32 == 0, "a row takes whole warps");
+    __shared__ double red[kW > 1 ? kW : 1];
+    __shared__ float redm[kW > 1 ? kW : 1];
+    const int tid = threadIdx.x % TPR, lane = threadIdx.x & 31, warp = tid >> 5;
+    const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / TPR;
+    if (row >= p.rows) return;      // (whole warps leave: with several rows a block, a row is one warp)
+    const int nvec = int(p.H / N);
+    const T* x = static_cast<const T*>(p.x) + row * p.H;
+    const T* r = static_cast<const T*>(p.r) + row * p.H;
+    const T* w = static_cast<const T*>(p.w);
+    T* hrow = static_cast<T*>(p.h) + row * p.H;
+    Vec16<T> hv[V], rv[V], wv[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = i * TPR + tid;
+        if (c < nvec) {
+            hv[i] = ld16_stream(x + int64_t(c) * N);
+            if (p.r) rv[i] = ld16_stream(r + int64_t(c) * N);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = i * TPR + tid;
+        if (c < nvec && w) wv[i] = ld16(w + int64_t(c) * N);
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = i * TPR + tid;
+        if (c < nvec) {
+            if (p.r) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) hv[i].v[e] = from_f32<T>(to_f32<T>(hv[i].v[e]) + to_f32<T>(rv[i].v[e]));
+                st16_stream(hrow + int64_t(c) * N, hv[i]);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float f = to_f32<T>(hv[i].v[e]);
+                ss = fmaf(f, f, ss);
+            }
+        }
+    }
+    double total = warp_sum(double(ss));
+    if constexpr (kW > 1) {
+        if (lane == 0) red[warp] = total;
+        __syncthreads();
+        total = 0.0;
+#pragma unroll
+        for (int i = 0; i < kW; ++i) total += red[i];
+    }
+    const float rstd = float(1.0 / sqrt(total / double(p.H) + p.eps));
+    if (p.rstd && tid == 0) p.rstd[row] = rstd;
+    if constexpr (!QUANT) {
+        T* y = static_cast<T*>(p.y) + row * p.H;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = i * TPR + tid;
+            if (c < nvec) {
+                Vec16<T> o;
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    o.v[e] = from_f32<T>(to_f32<T>(hv[i].v[e]) * rstd * (w ? to_f32<T>(wv[i].v[e]) : 1.0f));
+                st16_stream(y + int64_t(c) * N, o);
+            }
+        }
+    } else {
+        uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.H;
+        float f[V][N], amax[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = i * TPR + tid;
+            amax[i] = 0.f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                f[i][e] = c < nvec ? to_f32<T>(hv[i].v[e]) * rstd * (w ? to_f32<T>(wv[i].v[e]) : 1.0f) : 0.f;
+                amax[i] = fmaxf(amax[i], fabsf(f[i][e]));
+            }
+        }
+        if (p.group == 0) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) m = fmaxf(m, amax[i]);
+            m = warp_max(m);
+            if constexpr (kW > 1) {
+                if (lane == 0) redm[warp] = m;
+                __syncthreads();
+                m = 0.f;
+#pragma unroll
+                for (int i = 0; i < kW; ++i) m = fmaxf(m, redm[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) amax[i] = m;
+            if (tid == 0) p.scales[row] = scale_of(m);
+        } else {
+            const int gl = p.group / N;    // lanes of a group: 4 .. 32, a power of two
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                for (int o = gl >> 1; o > 0; o >>= 1) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
+                const int c = i * TPR + tid;
+                if (c < nvec && (c & (gl - 1)) == 0) p.scales[row * p.groups + c / gl] = scale_of(amax[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = i * TPR + tid;
+            if (c >= nvec) continue;
+            const float inv = 1.0f / scale_of(amax[i]);
+            uint32_t b[N / 4];
+#pragma unroll
+            for (int e = 0; e < N / 4; ++e)
+                b[e] = pack_e4m3(f[i][4 * e] * inv, f[i][4 * e + 1] * inv) |
+                       (pack_e4m3(f[i][4 * e + 2] * inv, f[i][4 * e + 3] * inv) << 16);
+            if constexpr (N == 8) __stcs(reinterpret_cast<uint2*>(q + int64_t(c) * 8), make_uint2(b[0], b[1]));
+            else __stcs(reinterpret_cast<uint32_t*>(q + int64_t(c) * 4), b[0]);
+        }
+    }
+}
+
+// Any row length and alignment: a CTA per row, h kept in memory between the passes (L2 holds it).
+template <typename T, bool QUANT>
+__global__ void __launch_bounds__(256)
+add_rmsnorm_any_kernel(const NormParams p) {
+    __shared__ double red[8];
+    __shared__ float redm[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(p.x) + row * p.H;
+        const T* r = p.r ? static_cast<const T*>(p.r) + row * p.H : nullptr;
+        const T* w = static_cast<const T*>(p.w);
+        T* hrow = p.r ? static_cast<T*>(p.h) + row * p.H : nullptr;
+        // each thread writes and later re-reads the same columns of h: no barrier between
+        auto at = [&](int64_t j) { return to_f32<T>(hrow ? hrow[j] : x[j]); };
+        double acc = 0.0;
+        for (int64_t j = tid; j < p.H; j += 256) {
+            T v = x[j];
+            if (r) {
+                v = from_f32<T>(to_f32<T>(v) + to_f32<T>(r[j]));
+                hrow[j] = v;
+            }
+            const float f = to_f32<T>(v);
+            acc += double(f) * double(f);
+        }
+        acc = warp_sum(acc);
+        if (lane == 0) red[warp] = acc;
+        __syncthreads();
+        double total = 0.0;
+        for (int i = 0; i < 8; ++i) total += red[i];
+        const float rstd = float(1.0 / sqrt(total / double(p.H) + p.eps));
+        if (p.rstd && tid == 0) p.rstd[row] = rstd;
+        auto yv = [&](int64_t j) { return at(j) * rstd * (w ? to_f32<T>(w[j]) : 1.0f); };
+        if constexpr (!QUANT) {
+            T* y = static_cast<T*>(p.y) + row * p.H;
+            for (int64_t j = tid; j < p.H; j += 256) y[j] = from_f32<T>(yv(j));
+        } else {
+            uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.H;
+            if (p.group == 0) {
+                float m = 0.f;
+                for (int64_t j = tid; j < p.H; j += 256) m = fmaxf(m, fabsf(yv(j)));
+                m = warp_max(m);
+                if (lane == 0) redm[warp] = m;
+                __syncthreads();
+                m = 0.f;
+                for (int i = 0; i < 8; ++i) m = fmaxf(m, redm[i]);
+                if (tid == 0) p.scales[row] = scale_of(m);
+                const float inv = 1.0f / scale_of(m);
+                for (int64_t j = tid; j < p.H; j += 256) q[j] = uint8_t(pack_e4m3(yv(j) * inv, 0.f));
+            } else {
+                // a group spans one to four warps: its maximum goes through the warps' own (a column's thread is
+                // j mod 256, so the groups of 256 / group different 32-column pieces are side by side)
+                for (int64_t j0 = 0; j0 < p.H; j0 += 256) {
+                    const int64_t j = j0 + tid;
+                    const float f = j < p.H ? yv(j) : 0.f;
+                    float m = warp_max(fabsf(f));
+                    __syncthreads();
+                    if (lane == 0) redm[warp] = m;
+                    __syncthreads();
+                    const int per = p.group / 32, first = warp / per * per;
+                    m = 0.f;
+                    for (int i = 0; i < per; ++i) m = fmaxf(m, redm[first + i]);
+                    if (j < p.H) {
+                        q[j] = uint8_t(pack_e4m3(f * (1.0f / scale_of(m)), 0.f));
+                        if (j % p.group == 0) p.scales[row * p.groups + j / p.group] = scale_of(m);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, bool QUANT>
+void launch_fwd(const NormParams& p, bool vec, cudaStream_t s) {
+    constexpr int N = Vec16<T>::N;
+    const int64_t nvec = p.H / N;
+    // A row stays in registers up to 4 vectors a thread.  Few threads a row leave more rows in flight on an SM; past
+    // 32 * 4 vectors a warp would have to hold more than that.
+    auto go = [&](auto kernel, int tpr) {
+        const int64_t per = tpr < 128 ? 128 / tpr : 1;
+        kernel<<<unsigned((p.rows + per - 1) / per), tpr < 128 ? 128 : tpr, 0, s>>>(p);
+    };
+    if (vec && nvec <= 32 * 4) {
+        if (nvec <= 32) go(add_rmsnorm_rows_kernel<T, 32, 1, QUANT>, 32);
+        else if (nvec <= 64) go(add_rmsnorm_rows_kernel<T, 32, 2, QUANT>, 32);
+        else go(add_rmsnorm_rows_kernel<T, 32, 4, QUANT>, 32);
+    } else if (vec && nvec <= 128 * 4) {
+        if (nvec <= 256) go(add_rmsnorm_rows_kernel<T, 128, 2, QUANT>, 128);
+        else go(add_rmsnorm_rows_kernel<T, 128, 4, QUANT>, 128);
+    } else if (vec && nvec <= 256 * 4) {
+        if (nvec <= 768) go(add_rmsnorm_rows_kernel<T, 256, 3, QUANT>, 256);
+        else go(add_rmsnorm_rows_kernel<T, 256, 4, QUANT>, 256);
+    } else if (vec && nvec <= 1024 * 4) {
+        if (nvec <= 2048) go(add_rmsnorm_rows_kernel<T, 512, 4, QUANT>, 512);
+        else go(add_rmsnorm_rows_kernel<T, 1024, 4, QUANT>, 1024);
+    } else {
+        const int64_t blocks = std::min<int64_t>(p.rows, 148 * 8);
+        add_rmsnorm_any_kernel<T, QUANT><<<int(blocks), 256, 0, s>>>(p);
+    }
+}
+
+// ---- backward --------------------------------------------------------------------------------
+// A CTA walks rows of its own; every thread owns the same columns of all of them, so grad_weight is summed in its
+// registers and leaves once per CTA (fp32 [parts, H], summed in double by the second kernel: no atomics, one order).
+// The three inputs of the next two rows are in flight (cp.async, each thread copying what it will read itself) while
+// a row is reduced and written; one row for the longest rows, of which no third stage fits into shared memory.
+__host__ __device__ constexpr int bwd_stages(int threads, int v) { return 3 * 3 * threads * v * 16 <= 224 * 1024 ? 3 : 2; }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+struct BwdParams {
+    const void *gy, *gh, *h, *w;
+    const float* rstd;
+    void* gx;
+    float* part;       // [gridDim.x, H], null: no grad_weight wanted
+    int64_t rows, H;
+};
+
+template <typename T, int THREADS, int V>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS)
+add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
+    constexpr int N = Vec16<T>::N;
+    constexpr int kStages = bwd_stages(THREADS, V);
+    constexpr uint32_t kOne = THREADS * V * 16, kStage = 3 * kOne;
+    extern __shared__ __align__(16) unsigned char ring_raw[];
+    __shared__ float red[2][THREADS / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(ring_raw));
+    const int nvec = int(p.H / N);
+    const T *gy = static_cast<const T*>(p.gy), *gh = static_cast<const T*>(p.gh), *h = static_cast<const T*>(p.h);
+    auto issue = [&](int64_t row, int stage) {
+        if (row < p.rows) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = i * THREADS + tid;
+                if (c < nvec) {
+                    const uint32_t dst = ring + stage * kStage + uint32_t(c) * 16;
+                    const int64_t at = row * p.H + int64_t(c) * N;
+                    copy16(dst, gy + at);
+                    copy16(dst + kOne, h + at);
+                    if (gh) copy16(dst + 2 * kOne, gh + at);
+                }
+            }
+        }
+        copy_commit();
+    };
+    Vec16<T> wv[V];
+    float dw[V * N];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = i * THREADS + tid;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            wv[i].v[e] = from_f32<T>(1.0f);
+            dw[i * N + e] = 0.f;
+        }
+        if (p.w && c < nvec) wv[i] = ld16(static_cast<const T*>(p.w) + int64_t(c) * N);
+    }
+    const float inv_h = 1.0f / float(p.H);
+#pragma unroll
+    for (int st = 0; st < kStages - 1; ++st) issue(int64_t(blockIdx.x) + int64_t(st) * gridDim.x, st);
+    int stage = 0, flip = 0;
+    float rr_next = p.rstd[blockIdx.x];
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, flip ^= 1) {
+        issue(row + int64_t(kStages - 1) * gridDim.x, stage == 0 ? kStages - 1 : stage - 1);
+        const float rr = rr_next;
+        rr_next = p.rstd[min(row + int64_t(gridDim.x), p.rows - 1)];
+        copy_wait<kStages - 1>();
+        const unsigned char* buf = ring_raw + stage * kStage;
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        Vec16<T> g[V], x[V];
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = i * THREADS + tid;
+            if (c < nvec) {
+                g[i] = *reinterpret_cast<const Vec16<T>*>(buf + c * 16);
+                x[i] = *reinterpret_cast<const Vec16<T>*>(buf + kOne + c * 16);
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    dot = fmaf(to_f32<T>(g[i].v[e]) * to_f32<T>(wv[i].v[e]), to_f32<T>(x[i].v[e]), dot);
+            }
+        }
+        dot = warp_sum(dot);
+        if (lane == 0) red[flip][warp] = dot;
+        __syncthreads();      // (two buffers in turn: the next row's writes cannot overtake these reads)
+        dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < THREADS / 32; ++i) dot += red[flip][i];
+        const float coef = rr * rr * (inv_h * dot) * rr;
+        T* out = static_cast<T*>(p.gx) + row * p.H;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = i * THREADS + tid;
+            if (c < nvec) {
+                Vec16<T> o, a;
+                if (gh) a = *reinterpret_cast<const Vec16<T>*>(buf + 2 * kOne + c * 16);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float ge = to_f32<T>(g[i].v[e]), xe = to_f32<T>(x[i].v[e]);
+                    o.v[e] = from_f32<T>(fmaf(ge * to_f32<T>(wv[i].v[e]), rr, -coef * xe) + (gh ? to_f32<T>(a.v[e]) : 0.f));
+                    dw[i * N + e] = fmaf(ge * xe, rr, dw[i * N + e]);
+                }
+                st16_stream(out + int64_t(c) * N, o);
+            }
+        }
+    }
+    copy_wait<0>();
+    if (p.part) {
+        float* part = p.part + int64_t(blockIdx.x) * p.H;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = i * THREADS + tid;
+            if (c < nvec)
+#pragma unroll
+                for (int e = 0; e < N; e += 4)
+                    *reinterpret_cast<float4*>(part + int64_t(c) * N + e) =
+                        make_float4(dw[i * N + e], dw[i * N + e + 1], dw[i * N + e + 2], dw[i * N + e + 3]);
+        }
+    }
+}
+
+// Any row length and alignment: grad_x, a CTA per row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+add_rmsnorm_bwd_dx_kernel(const BwdParams p) {
+    __shared__ double red[8];
+    const int tid = threadIdx.x;
+    const T* w = static_cast<const T*>(p.w);
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* gy = static_cast<const T*>(p.gy) + row * p.H;
+        const T* h = static_cast<const T*>(p.h) + row * p.H;
+        const T* gh = p.gh ? static_cast<const T*>(p.gh) + row * p.H : nullptr;
+        double dot = 0.0;
+        for (int64_t j = tid; j < p.H; j += 256)
+            dot += double(to_f32<T>(gy[j]) * (w ? to_f32<T>(w[j]) : 1.0f)) * double(to_f32<T>(h[j]));
+        dot = warp_sum(dot);
+        if ((tid & 31) == 0) red[tid >> 5] = dot;
+        __syncthreads();
+        dot = 0.0;
+        for (int i = 0; i < 8; ++i) dot += red[i];
+        const double rr = p.rstd[row];
+        const float coef = float(rr * rr * rr * dot / double(p.H)), r1 = float(rr);
+        T* out = static_cast<T*>(p.gx) + row * p.H;
+        for (int64_t j = tid; j < p.H; j += 256) {
+            const float a = to_f32<T>(gy[j]) * (w ? to_f32<T>(w[j]) : 1.0f);
+            out[j] = from_f32<T>(fmaf(a, r1, -coef * to_f32<T>(h[j])) + (gh ? to_f32<T>(gh[j]) : 0.f));
+        }
+        __syncthreads();
+    }
+}
+// ... and grad_weight: 32 columns a CTA, the rows over its other 32 threads.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+add_rmsnorm_bwd_dw_kernel(const BwdParams p, T* __restrict__ gw) {
+    __shared__ double part[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t col = int64_t(blockIdx.x) * 32 + tx;
+    double acc = 0.0;
+    if (col < p.H)
+        for (int64_t r = ty; r < p.rows; r += 32)
+            acc += double(to_f32<T>(static_cast<const T*>(p.gy)[r * p.H + col])) *
+                   double(to_f32<T>(static_cast<const T*>(p.h)[r * p.H + col])) * double(p.rstd[r]);
+    part[ty][tx] = acc;
+    __syncthreads();
+    if (ty == 0 && col < p.H) {
+        double t = 0.0;
+        for (int i = 0; i < 32; ++i) t += part[i][tx];
+        gw[col] = from_f32<T>(float(t));
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(1024)
+add_rmsnorm_bwd_dw_sum_kernel(const float* __restrict__ parts, T* __restrict__ gw, int count, int64_t H) {
+    __shared__ double sh[32][33];
+    const int cx = threadIdx.x & 31, py = threadIdx.x >> 5;
+    const int64_t col = int64_t(blockIdx.x) * 32 + cx;
+    double acc = 0.0;
+    if (col < H) {
+#pragma unroll 4
+        for (int i = py; i < count; i += 32) acc += double(__ldcs(parts + int64_t(i) * H + col));
+    }
+    sh[py][cx] = acc;
+    __syncthreads();
+    if (py == 0 && col < H) {
+        double t = 0.0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) t += sh[i][cx];
+        gw[col] = from_f32<T>(float(t));
+    }
+}
+
+template <typename T>
+int launch_bwd(Gpu* g, BwdParams p, void* gw, bool vec, cudaStream_t s) {
+    constexpr int N = Vec16<T>::N;
+    const int64_t nvec = p.H / N;
+    const int sms = g->sm_count > 0 ? g->sm_count : 148;
+    const unsigned dwblocks = unsigned((p.H + 31) / 32);
+    if (vec && nvec <= 512 * 4) {
+        // 128, 256 or 512 threads a row, at most 4 vectors each; the ring (2 or 3 stages of 3 inputs) takes at most
+        // 72 / 144 / 216 KB a CTA; 4 / 2 / 1 CTAs share an SM as registers and shared memory allow
+        const int threads = nvec <= 128 * 4 ? 128 : nvec <= 256 * 4 ? 256 : 512;
+        const int v = int((nvec + threads - 1) / threads);
+        const size_t ring = size_t(bwd_stages(threads, v)) * 3 * threads * v * 16;
+        int per_sm = 512 / threads;
+        while (per_sm > 1 && (ring + 1024) * per_sm > 220 * 1024) --per_sm;
+        const int parts = int(std::min<int64_t>(p.rows, int64_t(sms) * per_sm));
+        void* scratch = nullptr;
+        if (gw) {
+            const int st = paras_b200_malloc_async(g->ordinal, size_t(parts) * size_t(p.H) * sizeof(float), s, &scratch);
+            if (st != PARAS_OK) return st;
+        }
+        p.part = static_cast<float*>(scratch);
+        cudaError_t err = cudaSuccess;
+        auto go = [&](auto kernel) {
+            err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(ring));
+            if (err == cudaSuccess) kernel<<<parts, threads, ring, s>>>(p);
+        };
+        auto by_v = [&](auto th) {
+            constexpr int TH = decltype(th)::value;
+            if (v == 1) go(add_rmsnorm_bwd_rows_kernel<T, TH, 1>);
+            else if (v == 2) go(add_rmsnorm_bwd_rows_kernel<T, TH, 2>);
+            else if (v == 3) go(add_rmsnorm_bwd_rows_kernel<T, TH, 3>);
+            else go(add_rmsnorm_bwd_rows_kernel<T, TH, 4>);
+        };
+        if (threads == 128) by_v(std::integral_constant<int, 128>());
+        else if (threads == 256) by_v(std::integral_constant<int, 256>());
+        else by_v(std::integral_constant<int, 512>());
+        if (err == cudaSuccess && gw)
+            add_rmsnorm_bwd_dw_sum_kernel<T><<<dwblocks, 1024, 0, s>>>(p.part, static_cast<T*>(gw), parts, p.H);
+        if (err == cudaSuccess) err = cudaGetLastError();
+        const int st2 = scratch ? paras_b200_free_async(g->ordinal, scratch, s) : PARAS_OK;
+        if (err != cudaSuccess) return fail(PARAS_E_CUDA, "paras add_rms_norm_backward: launch failed: %s", cudaGetErrorString(err));
+        return st2;
+    }
+    add_rmsnorm_bwd_dx_kernel<T><<<int(std::min<int64_t>(p.rows, int64_t(sms) * 8)), 256, 0, s>>>(p);
+    if (gw) add_rmsnorm_bwd_dw_kernel<T><<<dwblocks, 1024, 0, s>>>(p, static_cast<T*>(gw));
+    PB_LAUNCH_CHECK("add_rmsnorm_bwd kernels");
+    return PARAS_OK;
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int check_sizes(int64_t rows, int64_t H, int dtype, const char* what) {
+    if (rows < 0 || H < 0) return fail(PARAS_E_INVALID, "%s: negative size", what);
+    if (rows >= (int64_t(1) << 31) || H >= (int64_t(1) << 31)) return fail(PARAS_E_UNSUPPORTED, "%s: a size exceeds 2^31 - 1", what);
+    if (dtype != PARAS_F32 && dtype != PARAS_BF16 && dtype != PARAS_F16)
+        return fail(PARAS_E_UNSUPPORTED, "%s: unsupported dtype %d", what, dtype);
+    return PARAS_OK;
+}
+
+template <bool QUANT>
+int forward(int gpu, const void* x, const void* residual, const void* weight, void* h, void* y, float* rstd, float* scales,
+            int64_t rows, int64_t H, double eps, int group, int dtype, void* stream, const char* what) {
+    int st = check_sizes(rows, H, dtype, what);
+    if (st != PARAS_OK) return st;
+    if (QUANT && group != 0 && group != 32 && group != 64 && group != 128)
+        return fail(PARAS_E_INVALID, "%s: group is %d columns, not 0 (a row), 32, 64 or 128", what, group);
+    DeviceRestore restore;
+    Gpu* g = use_gpu(gpu, &st);
+    if (!g) return st;
+    if (rows == 0 || H == 0) return PARAS_OK;
+    if (!x || !y || (residual && !h) || (QUANT && !scales)) return fail(PARAS_E_INVALID, "%s: null pointer", what);
+    NormParams p{};
+    p.x = x; p.r = residual; p.w = weight; p.h = h; p.y = y; p.rstd = rstd; p.scales = scales;
+    p.rows = rows; p.H = H; p.eps = eps; p.group = group;
+    p.groups = group ? (H + group - 1) / group : 1;
+    const int64_t n = 16 / int64_t(dtype_size(dtype));
+    const bool vec = H % n == 0 && al16(x) && (!residual || (al16(residual) && al16(h))) && (!weight || al16(weight)) &&
+                     (QUANT ? reinterpret_cast<uintptr_t>(y) % 8 == 0 : al16(y));
+    cudaStream_t s = pick_stream(g, stream);
+    switch (dtype) {
+        case PARAS_F32: launch_fwd<float, QUANT>(p, vec, s); break;
+        case PARAS_BF16: launch_fwd<__nv_bfloat16, QUANT>(p, vec, s); break;
+        default: launch_fwd<__half, QUANT>(p, vec, s); break;
+    }
+    PB_LAUNCH_CHECK(what);
+    return PARAS_OK;
+}
+
+}  // namespace
+}  // namespace pb
+
+using pb::fail;
+
+extern "C" {
+
+int paras_b200_add_rmsnorm_fwd(int gpu, const void* x, const void* residual, const void* weight, void* h, void* y,
+                               float* rstd, int64_t rows, int64_t H, double eps, int dtype, void* stream) {
+    pb::NvtxRange range("paras_b200_add_rmsnorm_fwd");
+    return pb::forward<false>(gpu, x, residual, weight, h, y, rstd, nullptr, rows, H, eps, 0, dtype, stream, "paras add_rms_norm");
+}
+
+int paras_b200_add_rmsnorm_quant_fwd(int gpu, const void* x, const void* residual, const void* weight, void* h,
+                                     void* q, float* scales, int64_t rows, int64_t H, double eps, int group, int dtype,
+                                     void* stream) {
+    pb::NvtxRange range("paras_b200_add_rmsnorm_quant_fwd");
+    return pb::forward<true>(gpu, x, residual, weight, h, q, nullptr, scales, rows, H, eps, group, dtype, stream,
+                             "paras add_rms_norm_quant");
+}
+
+int paras_b200_add_rmsnorm_bwd(int gpu, const void* grad_y, const void* grad_h, const void* h, const void* weight,
+                               const float* rstd, void* grad_x, void* grad_weight, int64_t rows, int64_t H, int dtype,
+                               void* stream) {
+    pb::NvtxRange range("paras_b200_add_rmsnorm_bwd");
+    const char* what = "paras add_rms_norm_backward";
+    int st = pb::check_sizes(rows, H, dtype, what);
+    if (st != PARAS_OK) return st;
+    pb::DeviceRestore restore;
+    pb::Gpu* g = pb::use_gpu(gpu, &st);
+    if (!g) return st;
+    if (H == 0) return PARAS_OK;
+    if (weight && !grad_weight) return fail(PARAS_E_INVALID, "%s: null pointer", what);
+    cudaStream_t s = pb::pick_stream(g, stream);
+    if (rows == 0) {
+        if (grad_weight) PB_CUDA(cudaMemsetAsync(grad_weight, 0, size_t(H) * pb::dtype_size(dtype), s));
+        return PARAS_OK;
+    }
+    if (!grad_y || !h || !rstd || !grad_x) return fail(PARAS_E_INVALID, "%s: null pointer", what);
+    pb::BwdParams p{};
+    p.gy = grad_y; p.gh = grad_h; p.h = h; p.w = weight; p.rstd = rstd; p.gx = grad_x; p.rows = rows; p.H = H;
+    const int64_t n = 16 / int64_t(pb::dtype_size(dtype));
+    const bool vec = H % n == 0 && pb::al16(grad_y) && pb::al16(grad_h) && pb::al16(h) && pb::al16(weight) && pb::al16(grad_x);
+    void* gw = weight ? grad_weight : nullptr;
+    switch (dtype) {
+        case PARAS_F32: return pb::launch_bwd<float>(g, p, gw, vec, s);
+        case PARAS_BF16: return pb::launch_bwd<__nv_bfloat16>(g, p, gw, vec, s);
+        default: return pb::launch_bwd<__half>(g, p, gw, vec, s);
+    }
+}
+
+}  // extern "C"

@@ -8,6 +8,9 @@
 //   paras::rms_norm_backward                                      fused_ops.cpp:90-157
 //   paras::swiglu(gate, up) / swiglu_backward                     fused_ops.cpp:162-229
 //   paras::rotate_half / rotate_half_backward                     fused_ops.cpp:234-302
+// and, without a counterpart there:
+//   paras::add_rms_norm(x, residual, weight, eps) -> (y, h, rstd), its backward, and the same with an 8-bit output
+//   (add_rms_norm_quant, rms_norm_quant)
 // Note the argument order: torch_paras::swiglu gates its SECOND argument, paras::swiglu its
 // first.  The composite entry points (aten::rms_norm, torch_paras::swiglu) round to the
 // tensor dtype after every step in the reference; the kernels reproduce that
@@ -175,6 +178,92 @@ Tensor rotate_half_backward(const Tensor& grad_out) {
     return rotate_half_impl(grad_out, 1, "rotate_half_backward");
 }
 
+// ---- residual addition and RMSNorm in one pass (no counterpart in the reference, which composes it) --------
+struct NormArgs {
+    Tensor x, r, w;
+    int64_t rows, H;
+    int dt, gpu;
+};
+NormArgs norm_args(const Tensor& x, const Tensor* residual, const Tensor& weight, const char* what) {
+    NormArgs a;
+    TORCH_CHECK(x.dim() >= 1, "paras ", what, ": input must have rank >= 1");
+    a.dt = checked_dtype(x, what);
+    a.gpu = Runtime::get().gpu_of(x);
+    a.H = x.size(-1);
+    a.rows = a.H > 0 ? x.numel() / a.H : 0;
+    if (residual) {
+        TORCH_CHECK(residual->sizes() == x.sizes(), "paras ", what, ": x and residual must have the same shape");
+        TORCH_CHECK(residual->scalar_type() == x.scalar_type() && residual->device() == x.device(),
+                    "paras ", what, ": x and residual must have the same dtype and device");
+        a.r = residual->contiguous();
+    }
+    TORCH_CHECK(weight.dim() == 1 && weight.size(0) == a.H, "paras ", what, ": weight size must match the last dimension");
+    TORCH_CHECK(weight.scalar_type() == x.scalar_type() && weight.device() == x.device(),
+                "paras ", what, ": weight dtype and device must equal the input's");
+    a.x = x.contiguous();
+    a.w = weight.contiguous();
+    return a;
+}
+
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+    PARAS_TRACE_OP("paras::add_rms_norm");
+    c10::DeviceGuard guard(x.device());
+    const NormArgs a = norm_args(x, &residual, weight, "add_rms_norm");
+    Tensor y = at::empty_like(a.x), h = at::empty_like(a.x), rstd = at::empty({a.rows}, x.options().dtype(c10::kFloat));
+    PARAS_ABI(paras_b200_add_rmsnorm_fwd(a.gpu, a.x.data_ptr(), a.r.data_ptr(), a.w.data_ptr(), h.data_ptr(), y.data_ptr(),
+                                         a.rows ? rstd.data_ptr<float>() : nullptr, a.rows, a.H, eps, a.dt, nullptr));
+    return {y, h, rstd};
+}
+
+std::tuple<Tensor, Tensor> add_rms_norm_backward(const Tensor& grad_y, const std::optional<Tensor>& grad_h, const Tensor& h,
+                                                 const Tensor& weight, const Tensor& rstd) {
+    PARAS_TRACE_OP("paras::add_rms_norm_backward");
+    c10::DeviceGuard guard(h.device());
+    const NormArgs a = norm_args(h, &grad_y, weight, "add_rms_norm_backward");
+    const bool has_gh = grad_h.has_value() && grad_h->defined();
+    Tensor gh;
+    if (has_gh) {
+        TORCH_CHECK(grad_h->sizes() == h.sizes() && grad_h->scalar_type() == h.scalar_type() && grad_h->device() == h.device(),
+                    "paras add_rms_norm_backward: grad_h must match h");
+        gh = grad_h->contiguous();
+    }
+    TORCH_CHECK(rstd.numel() == a.rows && rstd.scalar_type() == c10::kFloat && rstd.device() == h.device(),
+                "paras add_rms_norm_backward: rstd must be the fp32 tensor that the forward returned");
+    Tensor rs = rstd.contiguous();
+    Tensor gx = at::empty_like(a.x), gw = at::empty_like(a.w);
+    PARAS_ABI(paras_b200_add_rmsnorm_bwd(a.gpu, a.r.data_ptr(), has_gh ? gh.data_ptr() : nullptr, a.x.data_ptr(), a.w.data_ptr(),
+                                         a.rows ? rs.data_ptr<float>() : nullptr, gx.data_ptr(), gw.data_ptr(), a.rows, a.H,
+                                         a.dt, nullptr));
+    return {gx, gw};
+}
+
+std::tuple<Tensor, Tensor, Tensor> norm_quant(const Tensor& x, const Tensor* residual, const Tensor& weight, double eps,
+                                              int64_t group, const char* what) {
+    c10::DeviceGuard guard(x.device());
+    TORCH_CHECK(group == 0 || group == 32 || group == 64 || group == 128, "paras ", what,
+                ": group must be 0 (one scale per row), 32, 64 or 128");
+    const NormArgs a = norm_args(x, residual, weight, what);
+    Tensor q = at::empty(x.sizes(), x.options().dtype(c10::kFloat8_e4m3fn)), h;
+    if (residual) h = at::empty_like(a.x);
+    Tensor scales = at::empty({a.rows, group ? (a.H + group - 1) / group : 1}, x.options().dtype(c10::kFloat));
+    PARAS_ABI(paras_b200_add_rmsnorm_quant_fwd(a.gpu, a.x.data_ptr(), residual ? a.r.data_ptr() : nullptr, a.w.data_ptr(),
+                                               residual ? h.data_ptr() : nullptr, q.data_ptr(), scales.data_ptr<float>(), a.rows,
+                                               a.H, eps, int(group), a.dt, nullptr));
+    return {q, scales, h};
+}
+
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm_quant(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps,
+                                                      int64_t group) {
+    PARAS_TRACE_OP("paras::add_rms_norm_quant");
+    return norm_quant(x, &residual, weight, eps, group, "add_rms_norm_quant");
+}
+
+std::tuple<Tensor, Tensor> rms_norm_quant(const Tensor& x, const Tensor& weight, double eps, int64_t group) {
+    PARAS_TRACE_OP("paras::rms_norm_quant");
+    auto [q, scales, h] = norm_quant(x, nullptr, weight, eps, group, "rms_norm_quant");
+    return {q, scales};
+}
+
 // ---- autograd for F.rms_norm on `paras` tensors -------------------------------------------
 // The reference's aten::rms_norm is a composition of at:: operators that autograd follows
 // (rms_swiglu_ops.cpp:66-73).  With a fused backend kernel in its place the gradient is tied on
@@ -236,6 +325,10 @@ TORCH_LIBRARY(paras, m) {
     m.def("swiglu_backward(Tensor grad_out, Tensor gate, Tensor up) -> (Tensor, Tensor)");
     m.def("rotate_half(Tensor x) -> Tensor");
     m.def("rotate_half_backward(Tensor grad_out) -> Tensor");
+    m.def("add_rms_norm(Tensor x, Tensor residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
+    m.def("add_rms_norm_backward(Tensor grad_y, Tensor? grad_h, Tensor h, Tensor weight, Tensor rstd) -> (Tensor, Tensor)");
+    m.def("add_rms_norm_quant(Tensor x, Tensor residual, Tensor weight, float eps, int group=0) -> (Tensor, Tensor, Tensor)");
+    m.def("rms_norm_quant(Tensor x, Tensor weight, float eps, int group=0) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(paras, PrivateUse1, m) {
@@ -245,4 +338,8 @@ TORCH_LIBRARY_IMPL(paras, PrivateUse1, m) {
     m.impl("swiglu_backward", &paras::swiglu_backward);
     m.impl("rotate_half", &paras::rotate_half);
     m.impl("rotate_half_backward", &paras::rotate_half_backward);
+    m.impl("add_rms_norm", &paras::add_rms_norm);
+    m.impl("add_rms_norm_backward", &paras::add_rms_norm_backward);
+    m.impl("add_rms_norm_quant", &paras::add_rms_norm_quant);
+    m.impl("rms_norm_quant", &paras::rms_norm_quant);
 }

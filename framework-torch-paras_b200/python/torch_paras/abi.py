@@ -16,7 +16,7 @@ import torch
 _LIB_PATH = os.environ.get("PARAS_B200_LIB") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), "libparas_b200.so")
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, E4M3 = 0, 1, 2, 3
 ROUND_ONCE, ROUND_PER_OP = 0, 1
 SDPA_REF_SCALE, SDPA_FORCE_SIMT, SDPA_FORCE_TENSOR = 1, 2, 4
 
@@ -38,6 +38,9 @@ EXPORTS = [
     "paras_b200_sdpa_split_layout", "paras_b200_selftest_bounded_wait",
     "paras_b200_rms_rstd", "paras_b200_scale_columns", "paras_b200_sdpa_rope_fwd", "paras_b200_rope",
     "paras_b200_sdpa_bwd_general",
+    "paras_b200_paged_kv_write", "paras_b200_paged_kv_read", "paras_b200_paged_attn",
+    "paras_b200_paged_attn_workspace_bytes", "paras_b200_paged_attn_last_kernel",
+    "paras_b200_add_rmsnorm_fwd", "paras_b200_add_rmsnorm_quant_fwd", "paras_b200_add_rmsnorm_bwd",
 ]
 
 
@@ -87,6 +90,36 @@ class SdpaBwdArgs(C.Structure):
         ("B", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("Lq", C.c_int32),
         ("Lk", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32),
         ("scale", C.c_double), ("gpu", C.c_int32), ("reserved", C.c_int32), ("stream", C.c_void_p),
+    ]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+        ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3),
+        ("k_exp_strides", C.c_int64 * 3), ("v_exp_strides", C.c_int64 * 3),
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("cache_dtype", C.c_int32), ("pages", C.c_int32), ("page", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("B", C.c_int32), ("max_pages", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class PagedKvArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_strides", C.c_int64 * 2), ("v_strides", C.c_int64 * 2),
+        ("kv_lens", C.c_void_p), ("cu", C.c_void_p), ("T", C.c_int32), ("dtype", C.c_int32),
+        ("gpu", C.c_int32), ("reserved", C.c_int32), ("stream", C.c_void_p),
+    ]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("q_strides", C.c_int64 * 2), ("o_strides", C.c_int64 * 2),
+        ("kv_lens", C.c_void_p), ("cu", C.c_void_p), ("T", C.c_int32), ("Hq", C.c_int32), ("max_q", C.c_int32),
+        ("dtype", C.c_int32), ("causal", C.c_int32), ("gpu", C.c_int32), ("scale", C.c_double),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p),
     ]
 
 
@@ -140,6 +173,16 @@ def lib() -> C.CDLL:
                                           C.c_int, C.c_void_p]
         L.paras_b200_scale_columns.argtypes = [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
                                                C.c_int, C.c_void_p]
+        L.paras_b200_paged_kv_write.argtypes = [C.POINTER(PagedKvArgs)]
+        L.paras_b200_paged_kv_read.argtypes = [C.POINTER(PagedKvArgs)]
+        L.paras_b200_paged_attn.argtypes = [C.POINTER(PagedAttnArgs)]
+        L.paras_b200_paged_attn_workspace_bytes.argtypes = [C.POINTER(PagedAttnArgs), C.POINTER(C.c_size_t)]
+        L.paras_b200_paged_attn_last_kernel.restype = C.c_char_p
+        L.paras_b200_add_rmsnorm_fwd.argtypes = [C.c_int] + [C.c_void_p] * 6 + [C.c_int64, C.c_int64, C.c_double, C.c_int,
+                                                                                C.c_void_p]
+        L.paras_b200_add_rmsnorm_quant_fwd.argtypes = [C.c_int] + [C.c_void_p] * 6 + [C.c_int64, C.c_int64, C.c_double,
+                                                                                      C.c_int, C.c_int, C.c_void_p]
+        L.paras_b200_add_rmsnorm_bwd.argtypes = [C.c_int] + [C.c_void_p] * 7 + [C.c_int64, C.c_int64, C.c_int, C.c_void_p]
         _lib = L
     return _lib
 
@@ -522,3 +565,196 @@ def rotate_half(x, *, backward=False, stream=None):
     check(lib().paras_b200_rotate_half(_gpu_of(x), x.data_ptr(), out.data_ptr(), x.numel() // d if d else 0,
                                        d, dtype_code(x), 1 if backward else 0, _stream_of(x, stream)))
     return out
+
+
+# ---- paged key / value cache -----------------------------------------------------------------
+def _index_array(t, like, n, what):
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != like.device or \
+            (t.shape[0] > 1 and t.stride(0) != 1):
+        raise RuntimeError(f"paras abi: {what} must be a contiguous int32 vector" + (f" of {n} entries" if n is not None else "")
+                           + " on the tensors' device")
+    return t.data_ptr()
+
+
+def _paged_cache(c, k_cache, v_cache, page_table, k_exp, v_exp, rows):
+    """Fills a ``paras_paged_cache`` and checks what the C side cannot see (shapes, devices, types)."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
+        raise RuntimeError("paras abi: caches must be two [pages, kv heads, page, D] tensors of one type")
+    if shape[3] > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        raise RuntimeError("paras abi: cache rows must be contiguous")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise RuntimeError("paras abi: page_table must be int32 [sequences, pages] with contiguous rows")
+    dev = rows.device
+    if k_cache.device != dev or v_cache.device != dev or page_table.device != dev:
+        raise RuntimeError("paras abi: tensors are on different devices")
+    c.k, c.v = k_cache.data_ptr(), v_cache.data_ptr()
+    c.k_strides[:], c.v_strides[:] = k_cache.stride()[:3], v_cache.stride()[:3]
+    if k_cache.dtype == torch.float8_e4m3fn:
+        c.cache_dtype = E4M3
+        for e in (k_exp, v_exp):
+            if e is None or e.shape != shape[:3] or e.element_size() != 1 or e.device != dev:
+                raise RuntimeError("paras abi: an 8-bit cache needs k_exp and v_exp, bytes of shape [pages, kv heads, page]")
+        c.k_exp, c.v_exp = k_exp.data_ptr(), v_exp.data_ptr()
+        c.k_exp_strides[:], c.v_exp_strides[:] = k_exp.stride(), v_exp.stride()
+    elif k_exp is not None or v_exp is not None:
+        raise RuntimeError("paras abi: k_exp and v_exp belong to an 8-bit cache")
+    else:
+        c.cache_dtype = dtype_code(k_cache)
+    c.pages, c.Hkv, c.page, c.D = shape
+    c.page_table, c.table_stride = page_table.data_ptr(), page_table.stride(0)
+    c.B, c.max_pages = page_table.shape
+
+
+def _token_rows(t, heads, D, what):
+    s = t.shape
+    if len(s) != 3 or (heads is not None and s[1] != heads) or s[2] != D or (D > 1 and t.stride(2) != 1):
+        raise RuntimeError(f"paras abi: {what} must be [tokens, heads, D] with contiguous rows that fit the cache")
+
+
+def paged_kv_write(k, v, k_cache, v_cache, page_table, kv_lens, cu_q, *, k_exp=None, v_exp=None, stream=None):
+    """Writes new tokens' rows k, v [tokens, kv heads, D] into the paged cache in place (rounded to e4m3 with one
+    exponent byte per row when the cache is ``float8_e4m3fn``): row ``cu_q[b] + i`` is position
+    ``kv_lens[b] - (cu_q[b+1] - cu_q[b]) + i`` of sequence b."""
+    a = PagedKvArgs()
+    _paged_cache(a.cache, k_cache, v_cache, page_table, k_exp, v_exp, k)
+    _token_rows(k, a.cache.Hkv, a.cache.D, "k")
+    _token_rows(v, a.cache.Hkv, a.cache.D, "v")
+    if v.dtype != k.dtype or v.shape != k.shape or v.device != k.device:
+        raise RuntimeError("paras abi: k and v must have one type, shape and device")
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    a.k_strides[:], a.v_strides[:] = k.stride()[:2], v.stride()[:2]
+    a.kv_lens, a.cu = _index_array(kv_lens, k, a.cache.B, "kv_lens"), _index_array(cu_q, k, a.cache.B + 1, "cu_q")
+    a.T, a.dtype = k.shape[0], dtype_code(k)
+    a.gpu, a.stream = _gpu_of(k), _stream_of(k, stream)
+    check(lib().paras_b200_paged_kv_write(C.byref(a)))
+
+
+def paged_kv_read(k_cache, v_cache, page_table, cu_kv, total, *, dtype=None, k_exp=None, v_exp=None, out=None, stream=None):
+    """(k, v) [total, kv heads, D]: the first ``cu_kv[b+1] - cu_kv[b]`` positions of every sequence, one after the
+    other.  ``dtype`` is the result's type (the cache's, or bfloat16 for an 8-bit one, when omitted); rows behind the
+    last sequence keep what ``out`` held."""
+    pages, heads, page, D = k_cache.shape
+    if out is None:
+        if dtype is None:
+            dtype = torch.bfloat16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
+        kv = torch.empty((2, total, heads, D), dtype=dtype, device=k_cache.device)
+        out = (kv[0], kv[1])
+    k, v = out
+    a = PagedKvArgs()
+    _paged_cache(a.cache, k_cache, v_cache, page_table, k_exp, v_exp, k)
+    _token_rows(k, heads, D, "k")
+    _token_rows(v, heads, D, "v")
+    if v.dtype != k.dtype or v.shape != k.shape or k.shape[0] != total or v.device != k.device:
+        raise RuntimeError("paras abi: the two outputs must have one type and device and `total` rows")
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    a.k_strides[:], a.v_strides[:] = k.stride()[:2], v.stride()[:2]
+    a.cu = _index_array(cu_kv, k, a.cache.B + 1, "cu_kv")
+    a.T, a.dtype = total, dtype_code(k)
+    a.gpu, a.stream = _gpu_of(k), _stream_of(k, stream)
+    check(lib().paras_b200_paged_kv_read(C.byref(a)))
+    return k, v
+
+
+def paged_attn_args(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, out, *, causal=True, scale=None, k_exp=None,
+                    v_exp=None, lse=None, workspace=None, stream=None) -> PagedAttnArgs:
+    a = PagedAttnArgs()
+    _paged_cache(a.cache, k_cache, v_cache, page_table, k_exp, v_exp, q)
+    D = a.cache.D
+    _token_rows(q, None, D, "q")
+    if out is not q and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or (D > 1 and out.stride(2) != 1)):
+        raise RuntimeError("paras abi: out must have q's shape, type and device and contiguous rows")
+    a.q, a.out = q.data_ptr(), out.data_ptr()
+    a.lse = lse.data_ptr() if lse is not None else None
+    a.q_strides[:], a.o_strides[:] = q.stride()[:2], out.stride()[:2]
+    a.kv_lens, a.cu = _index_array(kv_lens, q, a.cache.B, "kv_lens"), _index_array(cu_q, q, a.cache.B + 1, "cu_q")
+    a.T, a.Hq, a.max_q = q.shape[0], q.shape[1], max_q
+    a.dtype, a.causal = dtype_code(q), 1 if causal else 0
+    a.scale = float(scale) if scale is not None else D ** -0.5
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    a.gpu, a.stream = _gpu_of(q), _stream_of(q, stream)
+    return a
+
+
+def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, *, causal=True, scale=None, k_exp=None,
+                    v_exp=None, out=None, return_lse=False, workspace=None, stream=None):
+    """Attention of the new tokens q [tokens, heads, D] over a paged cache that holds their keys and values already.
+    Row ``cu_q[b] + i`` is the query at position ``kv_lens[b] - (cu_q[b+1] - cu_q[b]) + i`` of sequence b and attends
+    the positions up to its own (all of them with ``causal=False``).  ``max_q`` bounds a sequence's new tokens."""
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    a = paged_attn_args(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, out, causal=causal, scale=scale, k_exp=k_exp,
+                        v_exp=v_exp, lse=lse, workspace=workspace, stream=stream)
+    check(lib().paras_b200_paged_attn(C.byref(a)))
+    return (out, lse) if return_lse else out
+
+
+def paged_attn_workspace_bytes(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, *, causal=True, k_exp=None,
+                               v_exp=None) -> int:
+    a = paged_attn_args(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, q, causal=causal, k_exp=k_exp, v_exp=v_exp)
+    n = C.c_size_t(0)
+    check(lib().paras_b200_paged_attn_workspace_bytes(C.byref(a), C.byref(n)))
+    return int(n.value)
+
+
+def paged_attn_last_kernel() -> str:
+    return lib().paras_b200_paged_attn_last_kernel().decode()
+
+
+# ---- residual addition and RMSNorm -------------------------------------------------------------
+def _norm_operands(x, residual, weight):
+    h = x.shape[-1]
+    for t in (residual, weight):
+        if t is not None and (t.dtype != x.dtype or t.device != x.device or not t.is_contiguous()):
+            raise RuntimeError("paras abi: norm operands must be contiguous, of one type and on one device")
+    if not x.is_contiguous() or (residual is not None and residual.shape != x.shape) or \
+            (weight is not None and weight.shape != (h,)):
+        raise RuntimeError("paras abi: x and residual must be contiguous and of one shape, weight [its last dimension]")
+    return h, x.numel() // h if h else 0
+
+
+def add_rmsnorm_fwd(x, residual, weight, eps=1e-6, *, return_rstd=False, stream=None):
+    """(y, h[, rstd]): h = x + residual in x's type, y = RMSNorm(h) * weight.  ``residual=None`` normalises x itself
+    (h is x); ``weight=None`` stands for ones."""
+    width, rows = _norm_operands(x, residual, weight)
+    y = torch.empty_like(x)
+    h = torch.empty_like(x) if residual is not None else x
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if return_rstd else None
+    check(lib().paras_b200_add_rmsnorm_fwd(
+        _gpu_of(x), x.data_ptr(), residual.data_ptr() if residual is not None else None,
+        weight.data_ptr() if weight is not None else None, h.data_ptr(), y.data_ptr(),
+        rstd.data_ptr() if return_rstd and rows else None, rows, width, float(eps), dtype_code(x), _stream_of(x, stream)))
+    return (y, h, rstd) if return_rstd else (y, h)
+
+
+def add_rmsnorm_quant(x, residual, weight, eps=1e-6, *, group=0, stream=None):
+    """(q, scales, h): the same norm in 8 bits, y ~ q * scales, q ``float8_e4m3fn``; one fp32 scale per row
+    (``group=0``: scales [rows, 1]) or per ``group`` = 32, 64 or 128 columns (scales [rows, ceil(width / group)])."""
+    width, rows = _norm_operands(x, residual, weight)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    h = torch.empty_like(x) if residual is not None else x
+    scales = torch.empty((rows, -(-width // group) if group > 0 else 1), dtype=torch.float32, device=x.device)
+    check(lib().paras_b200_add_rmsnorm_quant_fwd(
+        _gpu_of(x), x.data_ptr(), residual.data_ptr() if residual is not None else None,
+        weight.data_ptr() if weight is not None else None, h.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, width,
+        float(eps), group, dtype_code(x), _stream_of(x, stream)))
+    return q, scales, h
+
+
+def add_rmsnorm_bwd(grad_y, grad_h, h, weight, rstd, *, stream=None):
+    """(grad_x, grad_weight) of ``add_rmsnorm_fwd`` from the gradients that reach y and h (``grad_h=None``: none);
+    grad_x is the gradient of x and of residual alike."""
+    width, rows = _norm_operands(h, grad_y, weight)
+    if grad_h is not None:
+        _norm_operands(h, grad_h, None)
+    if rstd.dtype != torch.float32 or rstd.numel() != rows or not rstd.is_contiguous() or rstd.device != h.device:
+        raise RuntimeError("paras abi: rstd must be the fp32 [rows] that the forward returned")
+    gx = torch.empty_like(h)
+    gw = torch.empty_like(weight) if weight is not None else None
+    check(lib().paras_b200_add_rmsnorm_bwd(
+        _gpu_of(h), grad_y.data_ptr(), grad_h.data_ptr() if grad_h is not None else None, h.data_ptr(),
+        weight.data_ptr() if weight is not None else None, rstd.data_ptr(), gx.data_ptr(),
+        gw.data_ptr() if gw is not None else None, rows, width, dtype_code(h), _stream_of(h, stream)))
+    return gx, gw

@@ -10,7 +10,8 @@ from . import _C  # noqa: F401  (loads the operator registrations)
 
 __all__ = ["rms_norm", "swiglu", "rotate_half", "rope", "attention_rope", "swiglu_linear", "rms_norm_linear",
            "fold_norm_weight",
-           "attention_host", "scaled_dot_product_attention"]
+           "attention_host", "scaled_dot_product_attention", "add_rms_norm", "add_rms_norm_quant", "rms_norm_quant",
+           "paged_kv_write", "paged_kv_read", "paged_attention"]
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -25,6 +26,23 @@ class _RMSNorm(torch.autograd.Function):
         x, weight, rstd = ctx.saved_tensors
         gx, gw = torch.ops.paras.rms_norm_backward(grad.contiguous(), x, weight, rstd)
         return gx, gw, None
+
+
+class _AddRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        y, h, rstd = torch.ops.paras.add_rms_norm(x, residual, weight, eps)
+        ctx.save_for_backward(h, weight, rstd)
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    def backward(ctx, grad_y, grad_h):
+        h, weight, rstd = ctx.saved_tensors
+        if grad_y is None:      # only h was used: the sum passes its gradient on
+            return grad_h, grad_h, None, None
+        gx, gw = torch.ops.paras.add_rms_norm_backward(grad_y.contiguous(), grad_h, h, weight, rstd)
+        return gx, gx, gw, None
 
 
 class _SwiGLU(torch.autograd.Function):
@@ -68,6 +86,55 @@ class _RotateHalf(torch.autograd.Function):
 def rms_norm(input: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """RMSNorm over the last dimension of ``input`` in one kernel."""
     return _RMSNorm.apply(input, weight, eps)
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
+    """``h = x + residual; y = rms_norm(h, weight, eps)`` in one kernel; returns ``(y, h)``, both differentiable.  The
+    statistics are taken of ``h`` as it is returned, rounded to the tensors' dtype."""
+    return _AddRMSNorm.apply(x, residual, weight, eps)
+
+
+def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, group: int = 0):
+    """``add_rms_norm`` with an 8-bit result (forward only): returns ``(q, scales, h)`` with ``y ~ q * scales``, ``q``
+    ``float8_e4m3fn`` and fp32 scales ``[rows, 1]`` (``group=0``), or ``[rows, ceil(width / group)]`` for groups of 32, 64
+    or 128 columns."""
+    return torch.ops.paras.add_rms_norm_quant(x, residual, weight, eps, group)
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, group: int = 0):
+    """``rms_norm`` with an 8-bit result (forward only): ``(q, scales)`` as in ``add_rms_norm_quant``."""
+    return torch.ops.paras.rms_norm_quant(x, weight, eps, group)
+
+
+def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                   kv_lens: torch.Tensor, cu_q: torch.Tensor, *, k_exp: torch.Tensor = None, v_exp: torch.Tensor = None) -> None:
+    """Writes the rows of new tokens into a paged cache, in place.  ``k``, ``v``: ``[tokens, kv_heads, D]``; caches
+    ``[pages, kv_heads, page, D]`` in the same dtype, or ``float8_e4m3fn`` with one exponent byte per row in ``k_exp`` /
+    ``v_exp`` ``[pages, kv_heads, page]`` (uint8): an element is worth ``e4m3 * 2**(byte - 127)``.  int32 on the device:
+    ``page_table`` ``[sequences, pages]`` (a number outside the cache marks an absent page, which takes nothing),
+    ``kv_lens`` ``[sequences]`` counts the positions with the new tokens, ``cu_q`` ``[sequences + 1]`` where each
+    sequence's tokens start.  A page that is written must belong to one sequence."""
+    torch.ops.paras.paged_kv_write(k, v, k_cache, v_cache, page_table, kv_lens, cu_q, k_exp, v_exp)
+
+
+def paged_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_kv: torch.Tensor, total: int, *,
+                  dtype: torch.dtype = None, k_exp: torch.Tensor = None, v_exp: torch.Tensor = None):
+    """Reads sequences back as dense rows: ``(k, v)`` ``[total, kv_heads, D]``, where row ``cu_kv[b] + i`` is position ``i``
+    of sequence ``b``.  8-bit caches are converted to ``dtype`` (bfloat16 when omitted), exactly."""
+    return torch.ops.paras.paged_kv_read(k_cache, v_cache, page_table, cu_kv, total, dtype, k_exp, v_exp)
+
+
+def paged_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    kv_lens: torch.Tensor, cu_q: torch.Tensor, max_q: int, *, is_causal: bool = True, scale: float = None,
+                    k_exp: torch.Tensor = None, v_exp: torch.Tensor = None, return_lse: bool = False):
+    """Attention of new tokens over a paged cache that already holds their own keys and values (``paged_kv_write``); the
+    arguments are laid out as there.  ``query``: ``[tokens, heads, D]``, one token, a few or a chunk per sequence, mixed
+    freely; ``max_q`` bounds a sequence's count.  A token attends the positions up to its own (``is_causal=False``: all of
+    its sequence).  Forward only.  Returns ``[tokens, heads, D]`` and, with ``return_lse``, the fp32 log-sum-exp
+    ``[tokens, heads]``; a token that attends nothing gives zeros and ``-inf``."""
+    out, lse = torch.ops.paras.paged_attention(query, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, is_causal, scale,
+                                               k_exp, v_exp)
+    return (out, lse) if return_lse else out
 
 
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:

@@ -47,6 +47,8 @@ enum {
 };
 
 typedef enum { PARAS_F32 = 0, PARAS_BF16 = 1, PARAS_F16 = 2 } paras_dtype;
+/* Only as the type of a paged cache or of the 8-bit output of a norm: 4 exponent bits, 3 mantissa bits, no infinities. */
+enum { PARAS_E4M3 = 3 };
 
 /* ---- runtime: replaces compat::enumerate_devices / Queue (paras_compat.h:74-218) ---- */
 
@@ -372,6 +374,112 @@ int paras_b200_rms_rstd(int gpu, const void* x, float* rstd, int64_t rows, int64
                         void* stream);
 int paras_b200_scale_columns(int gpu, const void* weight, const void* scale, void* out, int64_t N, int64_t K,
                              int dtype, void* stream);
+
+/* ---- paged key / value cache ----
+ * No counterpart in the reference, whose caches are dense tensors that its attention (attention_ops.cpp:71-136) is
+ * given whole; these calls serve many sequences of different lengths from one pool of pages.
+ *
+ * The cache: k and v are [pages, Hkv, page, D], unit stride on D, element strides *_strides[3] = {page number, kv
+ * head, position in the page} (a [pages, page, Hkv, D] pool is the same call with other strides).  `cache_dtype` is
+ * the type of the rows that go in and come out, or PARAS_E4M3.  An 8-bit cache holds one exponent byte per row (one
+ * position of one kv head) in k_exp / v_exp, [pages, Hkv, page] bytes with strides *_exp_strides[3]; an element is
+ * worth  e4m3 * 2^(byte - 127).  The byte is the smallest exponent that keeps the row's largest magnitude within
+ * e4m3's 448, held between 2^-15 and 2^7, so that what a cache holds is exact in fp32, bf16 and fp16 alike; magnitudes
+ * above 57344, infinities among them, are stored as 57344, NaN stays NaN.
+ *
+ * The sequences, all on the device, so that a captured launch follows them: page_table[b][i] (row stride
+ * table_stride) is the page of positions i*page .. of sequence b, max_pages entries a row.  An entry outside
+ * [0, pages) is an absent page: its positions are not written, read back as zeros and are not attended.
+ * Sequence b owns the ragged rows cu[b] .. cu[b+1]-1 (cu is non-decreasing, B+1 entries) of the token tensors.  Rows
+ * that belong to no sequence (below cu[0], from cu[B] on) are neither read nor written.
+ */
+typedef struct paras_paged_cache {
+    void* k;
+    void* v;
+    uint8_t* k_exp; /* PARAS_E4M3 only */
+    uint8_t* v_exp;
+    int64_t k_strides[3], v_strides[3];
+    int64_t k_exp_strides[3], v_exp_strides[3];
+    const int32_t* page_table;
+    int64_t table_stride;
+    int32_t cache_dtype;
+    int32_t pages, page, Hkv, D;
+    int32_t B, max_pages;
+    int32_t reserved;
+} paras_paged_cache;
+
+/* Writes T new rows k, v [T, Hkv, D] (element strides {token, head}, unit stride on D) into the cache, rounding them
+ * to 8 bits on the way when the cache is PARAS_E4M3.  Row cu[b] + i of sequence b, which then has kv_lens[b]
+ * positions, is position kv_lens[b] - (cu[b+1] - cu[b]) + i.  A page that receives rows must belong to one sequence
+ * only.  Positions outside [0, max_pages * page) are dropped. */
+/* Reads sequences back: row cu[b] + i of the outputs k, v is position i of sequence b, in the rows' type (8-bit caches
+ * are converted).  kv_lens is not used. */
+typedef struct paras_paged_kv_args {
+    paras_paged_cache cache;
+    void* k;
+    void* v;
+    int64_t k_strides[2], v_strides[2];
+    const int32_t* kv_lens;
+    const int32_t* cu;
+    int32_t T;
+    int32_t dtype; /* of the rows */
+    int32_t gpu;
+    int32_t reserved;
+    void* stream;
+} paras_paged_kv_args;
+int paras_b200_paged_kv_write(const paras_paged_kv_args* args);
+int paras_b200_paged_kv_read(const paras_paged_kv_args* args);
+
+/* Attention of new tokens over the cache: q, out [T, Hq, D] (element strides {token, head}), Hq a multiple of Hkv
+ * (query head h reads kv head h / (Hq / Hkv)).  Row cu[b] + i is a query at position p = kv_lens[b] - (cu[b+1] - cu[b])
+ * + i of sequence b and attends positions 0 .. p when `causal`, all of 0 .. kv_lens[b]-1 otherwise; the keys and values
+ * of the new tokens themselves have to be in the cache already.  max_q bounds the new tokens of a sequence (queries
+ * past it are not computed); the route is chosen by it.  A query that attends nothing (no position left, all
+ * pages absent) gives zeros, with lse = -inf.  What lies in the cache past a sequence's last position is never used,
+ * whatever it holds; K and V of the attended positions have to be finite.  `lse` (optional): fp32 [T, Hq] contiguous,
+ * natural log of the sum of the exponentials of the scaled scores.  dtype F32, BF16 or F16; cache_dtype the same or
+ * PARAS_E4M3.  D up to 256.  `workspace`: as for paras_b200_sdpa_fwd; size from paras_b200_paged_attn_workspace_bytes. */
+typedef struct paras_paged_attn_args {
+    paras_paged_cache cache;
+    const void* q;
+    void* out;
+    float* lse;
+    int64_t q_strides[2], o_strides[2];
+    const int32_t* kv_lens;
+    const int32_t* cu;
+    int32_t T, Hq, max_q;
+    int32_t dtype;
+    int32_t causal;
+    int32_t gpu;
+    double scale;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} paras_paged_attn_args;
+int paras_b200_paged_attn(const paras_paged_attn_args* args);
+int paras_b200_paged_attn_workspace_bytes(const paras_paged_attn_args* args, size_t* bytes);
+/* Route of this thread's last successful paras_b200_paged_attn: "paged_simt", "paged_decode", "paged_tcgen05". */
+const char* paras_b200_paged_attn_last_kernel(void);
+
+/* ---- residual addition and RMSNorm in one pass ----
+ * What a decoder layer computes between its projections; the reference composes it from add and rms_norm
+ * (pointwise_ops.cpp:62-85, fused_ops.cpp:43-88).  All tensors [rows, H] contiguous.
+ *   h = x + residual, rounded to `dtype` (residual NULL: h is x and is not written)
+ *   y = h * rstd * weight,  rstd = 1 / sqrt(mean(h^2) + eps) of the rounded h        (weight NULL: ones)
+ * _fwd writes y rounded once to `dtype`, h, and rstd (optional, fp32 [rows]).
+ * _quant_fwd writes y in 8 bits instead, y ~ e4m3 * scale: one fp32 scale per row (group = 0) or per `group` = 32, 64
+ * or 128 consecutive columns (the last group of a row may be shorter), scales [rows, ceil(H / group)] contiguous,
+ * scale = max |y| / 448, at least 2^-126; y is not rounded to 16 bits in between.
+ * _bwd: the gradients of _fwd from grad_y and grad_h (the gradient that arrives at h, NULL: none): grad_x is the
+ * gradient of x and of residual alike, grad_weight [H] in `dtype` (NULL with weight NULL). */
+int paras_b200_add_rmsnorm_fwd(int gpu, const void* x, const void* residual, const void* weight, void* h, void* y,
+                               float* rstd, int64_t rows, int64_t H, double eps, int dtype, void* stream);
+int paras_b200_add_rmsnorm_quant_fwd(int gpu, const void* x, const void* residual, const void* weight, void* h,
+                                     void* q, float* scales, int64_t rows, int64_t H, double eps, int group, int dtype,
+                                     void* stream);
+int paras_b200_add_rmsnorm_bwd(int gpu, const void* grad_y, const void* grad_h, const void* h, const void* weight,
+                               const float* rstd, void* grad_x, void* grad_weight, int64_t rows, int64_t H, int dtype,
+                               void* stream);
 
 /* ---- failure path self-test ----
  * No counterpart in the reference (its kernels have no device-side waits; a stuck queue there

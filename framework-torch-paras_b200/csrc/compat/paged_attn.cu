@@ -102,6 +102,12 @@ int check(const paras_paged_attn_args* args, const char* what) {
     return PARAS_OK;
 }
 
+enum class Route { kSimt, kDecode };
+Route pick_route(const Gpu* g, const paras_paged_attn_args& a) {
+    return paged_decode_supported(g, a) ? Route::kDecode : Route::kSimt;
+}
+int stream_ctas(const Gpu* g) { return g->sm_count > 0 ? g->sm_count : 148; }   // persistent, one per SM
+
 PagedParams make_params(const Gpu* g, const paras_paged_attn_args& a) {
     const paras_paged_cache& c = a.cache;
     PagedParams p{};
@@ -158,7 +164,25 @@ int paras_b200_paged_attn(const paras_paged_attn_args* args) {
     if (!a.q || !a.out || !a.kv_lens || !a.cu) return fail(PARAS_E_INVALID, "%s: null pointer", what);
     const pb::PagedParams p = pb::make_params(g, a);
     cudaStream_t s = pb::pick_stream(g, a.stream);
-    return pb::paged_simt_launch(p, a.dtype, a.cache.cache_dtype == PARAS_E4M3, s);
+    const pb::Route r = pb::pick_route(g, a);
+    if (r == pb::Route::kSimt) return pb::paged_simt_launch(p, a.dtype, a.cache.cache_dtype == PARAS_E4M3, s);
+    const int G = pb::stream_ctas(g), rows = pb::paged_decode_rows();
+    const size_t need = pb::paged_workspace_bytes(G, rows, p.D);
+    void* scratch = a.workspace;
+    if (scratch) {
+        if (a.workspace_bytes < need)
+            return fail(PARAS_E_INVALID, "%s: workspace of %zu bytes is too small, %zu are needed", what, a.workspace_bytes, need);
+        if (reinterpret_cast<uintptr_t>(scratch) & 15u) return fail(PARAS_E_INVALID, "%s: workspace is not 16-byte aligned", what);
+    } else if ((st = paras_b200_malloc_async(a.gpu, need, s, &scratch)) != PARAS_OK) {
+        return st;
+    }
+    st = pb::paged_decode_launch(g, a, p, pb::paged_carve(scratch, G, rows), G, s);
+    if (st == PARAS_OK) pb::tl_paged_kernel = "paged_decode";
+    if (!a.workspace) {
+        const int st2 = paras_b200_free_async(a.gpu, scratch, s);
+        if (st == PARAS_OK) st = st2;
+    }
+    return st;
 }
 
 int paras_b200_paged_attn_workspace_bytes(const paras_paged_attn_args* args, size_t* bytes) {
@@ -166,6 +190,11 @@ int paras_b200_paged_attn_workspace_bytes(const paras_paged_attn_args* args, siz
     if (st != PARAS_OK) return st;
     if (!bytes) return fail(PARAS_E_INVALID, "paras paged_attention: null pointer");
     *bytes = 0;
+    pb::DeviceRestore restore;
+    pb::Gpu* g = pb::use_gpu(args->gpu, &st);
+    if (!g) return st;
+    if (pb::pick_route(g, *args) != pb::Route::kSimt)
+        *bytes = pb::paged_workspace_bytes(pb::stream_ctas(g), pb::paged_decode_rows(), args->cache.D);
     return PARAS_OK;
 }
 

@@ -3,6 +3,8 @@
 
 #include "paged_common.cuh"
 
+struct CUtensorMap_st;
+
 namespace pb {
 
 // What every route needs of the call.
@@ -47,5 +49,134 @@ __device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& 
 }
 
 int paged_simt_launch(const PagedParams& p, int dtype, bool cache8, cudaStream_t s);
+
+// ---- the streaming kernels' shared-out work ------------------------------------------------------
+// Their unit of work is a tile: 128 positions of the cache for one item (the query rows that share a pass over a kv
+// head's keys).  All W tiles of a call stand in one row, sequence by sequence, and CTA c of G takes those from c*W/G to
+// (c+1)*W/G (with fewer tiles than CTAs, G = W of them take one each): every CTA streams the same amount whatever the
+// lengths are, and the host need not know them.  An item cut by
+// such a border leaves partial results in the workspace, at most two per CTA (slot 2c for the item that the CTA starts
+// in the middle of or at its first tile, 2c+1 for a later one that goes on in the next CTA), and a second kernel, whose
+// block c looks after the item that starts in CTA c and goes on, joins them in the order of the CTAs.
+constexpr int kTileKeys = 128;
+
+struct PagedRange {
+    int64_t total, ctas;    // W, G
+    int64_t begin, end;
+    // the CTA that has tile x: the largest c with c * W / G <= x
+    __device__ __forceinline__ int owner(int64_t x) const { return int(((x + 1) * ctas - 1) / total); }
+};
+
+// What block c of the joining kernel has to know; written by CTA c of the streaming kernel.
+struct PagedJoin {
+    int first_slot;   // -1: nothing to join
+    int last_cta;     // parts: first_slot, then slot 2*k for the CTAs up to this one
+    int row0;         // first token row, tokens and kv head of the item
+    int nq, hk;
+    int pad[3];
+};
+static_assert(sizeof(PagedJoin) == 32, "joins are laid out as 32-byte records");
+
+// Workspace of G CTAs with items of `rows` query rows: joins, {max, sum} pairs, partial outputs (fp32, unnormalised).
+struct PagedWorkspace {
+    PagedJoin* join;
+    float2* ml;       // [2G][rows]   maximum of the scores * scale * log2(e), sum of the exponentials
+    float* o;         // [2G][rows][D]
+};
+inline size_t paged_workspace_bytes(int G, int rows, int D) {
+    return size_t(G) * sizeof(PagedJoin) + size_t(2 * G) * rows * (sizeof(float2) + size_t(D) * sizeof(float));
+}
+inline PagedWorkspace paged_carve(void* base, int G, int rows) {
+    PagedWorkspace w;
+    w.join = static_cast<PagedJoin*>(base);
+    w.ml = reinterpret_cast<float2*>(w.join + G);
+    w.o = reinterpret_cast<float*>(w.ml + size_t(2 * G) * rows);   // (G*32 + 2G*rows*8 bytes: a multiple of 16)
+    return w;
+}
+
+// Inclusive sum over a warp.
+__device__ __forceinline__ int64_t warp_scan(int64_t v) {
+    const int lane = int(threadIdx.x) & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// Finds this CTA's range and the sequence in which it begins; every thread of the block calls it.  tiles(b) is the number
+// of tiles of sequence b.  `sums` has a place per warp and three more.  Returns the range; *b0 / *base0: that sequence
+// and the place of its first tile in the row (only where begin < end).
+template <typename Tiles>
+__device__ __forceinline__ PagedRange paged_range(int B, int64_t* sums, Tiles tiles, int* b0, int64_t* base0) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = int(blockDim.x) >> 5;
+    int64_t* total = sums + nw;   // total, found sequence, its base
+    int64_t W = 0;
+    for (int chunk = 0; chunk < B; chunk += int(blockDim.x)) {
+        const int b = chunk + tid;
+        W += b < B ? tiles(b) : 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) W += __shfl_xor_sync(0xffffffffu, W, o);
+    if (lane == 0) sums[warp] = W;
+    __syncthreads();
+    W = 0;
+    for (int i = 0; i < nw; ++i) W += sums[i];
+    PagedRange r;
+    r.total = W;
+    r.ctas = min(W, int64_t(gridDim.x));
+    r.begin = r.end = 0;
+    if (int64_t(blockIdx.x) < r.ctas) {
+        r.begin = int64_t(blockIdx.x) * W / r.ctas;
+        r.end = (int64_t(blockIdx.x) + 1) * W / r.ctas;
+    }
+    if (tid == 0) {
+        total[1] = 0;
+        total[2] = 0;
+    }
+    if (r.begin < r.end) {        // (the same for the whole block)
+        int64_t base = 0;
+        for (int chunk = 0; chunk < B && base <= r.begin; chunk += int(blockDim.x)) {
+            const int b = chunk + tid;
+            const int64_t n = b < B ? tiles(b) : 0;
+            const int64_t incl = warp_scan(n);
+            __syncthreads();      // sums is free
+            if (lane == 31) sums[warp] = incl;
+            __syncthreads();
+            int64_t before = base, all = base;
+            for (int i = 0; i < nw; ++i) {
+                if (i < warp) before += sums[i];
+                all += sums[i];
+            }
+            const int64_t at = before + incl - n;
+            if (n > 0 && at <= r.begin && r.begin < at + n) {
+                total[1] = b;
+                total[2] = at;
+            }
+            base = all;
+        }
+    }
+    __syncthreads();
+    *b0 = int(total[1]);
+    *base0 = total[2];
+    return r;
+}
+
+// Joins the partial results of cut items: a launch of G blocks after the streaming kernel on the same stream.
+int paged_join_launch(const PagedParams& p, const PagedWorkspace& ws, int G, int rows, int dtype, cudaStream_t s);
+
+bool paged_decode_supported(const Gpu* g, const paras_paged_attn_args& a);
+int paged_decode_rows();     // query rows of an item in the workspace
+int paged_decode_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p, const PagedWorkspace& ws, int G, cudaStream_t s);
+
+// Can the cache be read by TMA in tiles of 128 positions (page size, alignment, strides)?
+bool paged_tma_ok(const paras_paged_cache& c);
+// Map of the cache's K (which = 0) or V: {D, position, head, page}, box of one page's (at most 128) rows by 128 bytes (the
+// row, where it is shorter).  16-bit rows: slabs of 64 elements; 8-bit rows: the whole row.
+int paged_cache_map(CUtensorMap_st* map, const paras_paged_cache& c, int which);
+// Map of q seen as {D, group, kv head, token}: box {64, group, 1, tokens}.
+bool paged_q_tma_ok(const paras_paged_attn_args& a);
+int paged_q_map(CUtensorMap_st* map, const paras_paged_attn_args& a, int tokens);
 
 }  // namespace pb

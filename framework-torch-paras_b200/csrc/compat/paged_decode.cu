@@ -1,0 +1,656 @@
+// Attention of one or a few new tokens per sequence over a paged cache: HBM-bound streaming of K and V.
+//
+// The group x tokens (at most 16) query rows that share a kv head are the M = 16 rows of one mma.sync tile, so every K
+// and V byte is read once.  16 FLOP per byte with 4x row padding is far below what mma.sync gives; a 128-row tcgen05
+// tile would be seven eighths empty and its TMEM round trip longer than the tile's loads.
+//
+// A persistent CTA per SM takes its part of all tiles (128 positions of one item; paged_attn.cuh says how they are
+// shared out), whatever items these belong to, and its ring of tiles never drains between items.
+//   warp 8      loads: page numbers of the next tile while this one waits for its slot; a TMA box per page; an 8-bit
+//               cache's exponent bytes; what the consumers have to know of the tile
+//   warps 0-7   16 keys of every tile each: S = Q K^T, online softmax in registers, O += P V with P straight from the
+//               accumulators; at the end of an item the eight states are merged through shared memory
+//
+// 8-bit rows become fp16, not the query's type: e4m3 -> fp16 is one exact instruction, and the rows' 2^e (exact in
+// fp16) are multiplied into S for K, into the fragments for V.  bf16 queries are brought to fp16 scaled by a power of
+// two per row, so that only elements below 2^-14 of the row's largest lose bits (2^-25 of it at most).  P is rounded to
+// the 16-bit type that multiplies V, as in the dense kernels; maxima, sums and accumulators are fp32.
+#include <cmath>
+
+#include "paged_attn.cuh"
+#include "tc_prims.cuh"
+#include "tma_host.cuh"
+
+namespace pb {
+namespace {
+
+using namespace tc;
+
+constexpr int kConsumers = 8;
+constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kRows = 16;
+constexpr int kMergeBytes = 16 * 1024;
+constexpr int kMaxStages = 8;
+constexpr int kMetaBytes = 48;
+
+// What a stage of the ring holds: K tile, V tile, the query rows (first tile of an item), exponents.
+template <bool E8, int HD> struct Ring {
+    static constexpr int kRow = E8 ? HD : 128;                    // bytes of a swizzled row
+    static constexpr int kSlabs = E8 ? 1 : HD / 64;
+    static constexpr int kSlab = kTileKeys * kRow;
+    static constexpr int kTile = kSlabs * kSlab;
+    static constexpr int kQ = 2 * kTile;                           // offset of the query rows
+    static constexpr int kExp = kQ + (HD / 64) * kRows * 128;      // offsets: K's 2^e (fp32), V's 2^e (fp16)
+    static constexpr int kBytes = kExp + (E8 ? 1024 : 0);          // a multiple of 1024
+    static constexpr int kStages = (208 * 1024) / kBytes < kMaxStages ? (208 * 1024) / kBytes : kMaxStages;
+    static constexpr int kMerge = kStages * kBytes;
+    static constexpr int kMl = kMerge + kMergeBytes;               // [8][16] maxima, [8][16] sums
+    static constexpr int kMeta = kMl + 2 * kConsumers * kRows * 4;
+    static constexpr int kSums = kMeta + kMaxStages * kMetaBytes;
+    static constexpr int kBars = kSums + (kThreads / 32 + 3) * 8;
+    static constexpr int kMisc = kBars + (2 * kMaxStages + 1) * 8 + 8;
+    static constexpr int kLaunch = kMisc + 16 + 1024;
+    static_assert(kLaunch <= 227 * 1024, "shared memory of a CTA");
+    static_assert(kBytes % 1024 == 0 && kSums % 8 == 0, "alignment");
+};
+
+struct TileMeta {        // kMetaBytes, one per stage
+    int row0, nq, hk, key0;
+    int kend;            // positions the item attends: keys from here on are not
+    int pos0;
+    uint32_t pages;      // bit i: page i of the tile is there
+    int flags;           // 1 first tile of the item here, 2 last, 4 the item is not whole here
+    int slot;
+    int pad[3];
+};
+static_assert(sizeof(TileMeta) == kMetaBytes, "");
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t r;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 r;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+    return r;
+}
+
+// Byte offset of 16-byte unit c of row r in a tile that TMA wrote with the 128- or 64-byte swizzle.
+template <int ROW>
+__device__ __forceinline__ uint32_t swz(int r, int c) {
+    if constexpr (ROW == 128) return uint32_t(r * 128 + ((c ^ (r & 7)) << 4));
+    else return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+
+// Tiles of a sequence's items: one item per kv head.  A sequence with new tokens and nothing to attend has one empty tile
+// per item (its rows are zeros), one without new tokens none.
+__device__ __forceinline__ int seq_keys(const PagedParams& p, const PagedSeq& s) { return paged_keys(p, s, s.nq - 1); }
+__device__ __forceinline__ int seq_tiles(const PagedParams& p, const PagedSeq& s) {
+    return s.nq <= 0 ? 0 : max(1, (seq_keys(p, s) + kTileKeys - 1) / kTileKeys);
+}
+
+template <bool BF16, bool E8, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v, const PagedParams p, const PagedWorkspace ws) {
+    using R = Ring<E8, HD>;
+    constexpr bool kBfOps = BF16 && !E8;     // type of the MMA operands
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    auto full = [&](int s) { return base + R::kBars + 8u * s; };
+    auto empty = [&](int s) { return base + R::kBars + 8u * (kMaxStages + s); };
+    const uint32_t merge_bar = base + R::kBars + 8u * (2 * kMaxStages);
+    TileMeta* meta = reinterpret_cast<TileMeta*>(gen + R::kMeta);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + R::kMisc);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < R::kStages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), kConsumers);
+        }
+        mbar_init(merge_bar, kConsumers);
+        *abort_flag = 0;
+        mbar_fence_init();
+        fence_proxy_async_smem();
+    }
+    int b0;
+    int64_t base0;
+    const PagedRange range = paged_range(p.B, reinterpret_cast<int64_t*>(gen + R::kSums),
+                                         [&](int b) { return int64_t(p.Hkv) * seq_tiles(p, paged_seq(p, b)); }, &b0, &base0);
+    const int ntiles = int(range.end - range.begin);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (warp == kConsumers) {
+        // ------------------------------ producer ------------------------------
+        if (lane == 0) {
+            tma_prefetch_desc(&map_q);
+            tma_prefetch_desc(&map_k);
+            tma_prefetch_desc(&map_v);
+        }
+        PagedJoin join{};
+        join.first_slot = -1;
+        const int box = min(p.page, kTileKeys), npg = kTileKeys / box;   // rows and number of boxes of a tile
+        const bool exp4 = E8 && p.eks[2] == 1 && p.evs[2] == 1 && ((p.eks[0] | p.eks[1] | p.evs[0] | p.evs[1]) & 3) == 0 &&
+                          ((reinterpret_cast<uintptr_t>(p.ek) | reinterpret_cast<uintptr_t>(p.ev)) & 3) == 0;
+        // where the tile to be asked for next stands
+        PagedSeq sq{};
+        int b = b0, hk = 0, tile = 0, nt = 0, kend = 0;
+        int64_t item0 = 0;       // place of the item's first tile
+        auto enter = [&]() {     // the first sequence from b on that has tiles
+            for (; b < p.B; ++b) {
+                sq = paged_seq(p, b);
+                nt = seq_tiles(p, sq);
+                if (nt > 0) break;
+            }
+            kend = nt > 0 ? seq_keys(p, sq) : 0;
+        };
+        if (ntiles > 0) {
+            enter();
+            const int64_t in = range.begin - base0;
+            hk = int(in / nt);
+            tile = int(in - int64_t(hk) * nt);
+            item0 = base0 + int64_t(hk) * nt;
+        }
+        // lane i: page number of box i of the tile, -1 when it is not to be read
+        auto page_of = [&]() -> int {
+            const int key = tile * kTileKeys + lane * box;
+            if (lane >= npg || key >= kend) return -1;
+            const int pg = __ldg(p.table + int64_t(b) * p.table_stride + key / p.page);
+            return uint32_t(pg) < uint32_t(p.pages) ? pg : -1;
+        };
+        int pg = ntiles > 0 ? page_of() : -1;
+        uint32_t ek4 = 0, ev4 = 0;
+        // lane l: exponent bytes of the tile's keys 4l .. 4l+3, 127 where there is no key
+        auto exps_of = [&]() {
+            if constexpr (E8) {
+                const int key = 4 * lane;
+                const int mine = __shfl_sync(0xffffffffu, pg, key / box);
+                const int at = tile * kTileKeys + key, off = at % p.page;
+                ek4 = ev4 = 0x7f7f7f7fu;
+                if (mine >= 0) {
+                    const uint8_t* k = p.ek + int64_t(mine) * p.eks[0] + int64_t(hk) * p.eks[1] + int64_t(off) * p.eks[2];
+                    const uint8_t* v = p.ev + int64_t(mine) * p.evs[0] + int64_t(hk) * p.evs[1] + int64_t(off) * p.evs[2];
+                    const int live = kend - at;
+                    if (exp4) {
+                        const uint32_t keep = live >= 4 ? 0xffffffffu : live <= 0 ? 0u : (1u << (8 * live)) - 1u;
+                        ek4 = (__ldg(reinterpret_cast<const uint32_t*>(k)) & keep) | (ek4 & ~keep);
+                        ev4 = (__ldg(reinterpret_cast<const uint32_t*>(v)) & keep) | (ev4 & ~keep);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (e < live) {
+                                ek4 = (ek4 & ~(0xffu << (8 * e))) | (uint32_t(k[e * p.eks[2]]) << (8 * e));
+                                ev4 = (ev4 & ~(0xffu << (8 * e))) | (uint32_t(v[e * p.evs[2]]) << (8 * e));
+                            }
+                    }
+                }
+            }
+        };
+        if (ntiles > 0) exps_of();
+        bool first = true;
+        for (int i = 0; i < ntiles; ++i) {
+            // this tile, and the way to the next one with its loads asked for
+            const int c_pg = pg, c_tile = tile, c_hk = hk, c_kend = kend, c_nt = nt;
+            const PagedSeq c_sq = sq;
+            const uint32_t c_ek = ek4, c_ev = ev4;
+            const int64_t c_item0 = item0;
+            if (i + 1 < ntiles) {
+                if (++tile == nt) {
+                    tile = 0;
+                    item0 += nt;
+                    if (++hk == p.Hkv) {
+                        hk = 0;
+                        ++b;
+                        enter();
+                    }
+                }
+                pg = page_of();
+                exps_of();
+            }
+            const int s = i % R::kStages;
+            if (!__all_sync(0xffffffffu, mbar_wait(empty(s), ((i / R::kStages) & 1) ^ 1u, abort_flag, 2))) break;
+            const uint32_t dst = base + s * R::kBytes;
+            const uint32_t there = __ballot_sync(0xffffffffu, c_pg >= 0);
+            const bool last = c_tile + 1 == c_nt || i + 1 == ntiles;
+            if constexpr (E8) {
+                // (a row's exponent is within [-15, 7]: normal in fp32, 2^-15 the one subnormal in fp16)
+                uint32_t kf[4], vh[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    kf[e] = __float_as_uint(pow2f(max(kExpLo, min(kExpHi, int((c_ek >> (8 * e)) & 0xffu) - 127))));
+                    const int x = max(kExpLo, min(kExpHi, int((c_ev >> (8 * e)) & 0xffu) - 127));
+                    vh[e] = x >= -14 ? uint32_t(x + 15) << 10 : 0x200u;
+                }
+                st_shared_v4(dst + R::kExp + lane * 16, make_uint4(kf[0], kf[1], kf[2], kf[3]));
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + R::kExp + 512 + lane * 8), "r"(vh[0] | (vh[1] << 16)),
+                             "r"(vh[2] | (vh[3] << 16)) : "memory");
+            }
+            if (lane == 0) {
+                TileMeta m{};
+                m.row0 = c_sq.row0;
+                m.nq = c_sq.nq;
+                m.hk = c_hk;
+                m.key0 = c_tile * kTileKeys;
+                m.kend = c_kend;
+                m.pos0 = c_sq.pos0;
+                m.pages = there;
+                const bool whole = c_item0 >= range.begin && c_item0 + c_nt <= range.end;
+                m.flags = (first ? 1 : 0) | (last ? 2 : 0) | (whole ? 0 : 4);
+                // the item the range begins with leaves its part in slot 2c, a later one that goes on in 2c+1
+                m.slot = 2 * int(blockIdx.x) + (c_item0 > range.begin ? 1 : 0);
+                if (!whole && c_item0 >= range.begin) {
+                    join.first_slot = m.slot;
+                    join.last_cta = range.owner(c_item0 + c_nt - 1);
+                    join.row0 = c_sq.row0;
+                    join.nq = c_sq.nq;
+                    join.hk = c_hk;
+                }
+                meta[s] = m;
+            }
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive_expect_tx(full(s), 2 * R::kTile + (first ? (HD / 64) * p.max_q * p.group * 128 : 0));
+            __syncwarp();
+            if (lane < npg) {
+                // (pages outside the tensor read as zeros)
+                const int page = c_pg >= 0 ? c_pg : p.pages;
+                const int row = (c_tile * kTileKeys + lane * box) % p.page;
+#pragma unroll
+                for (int c = 0; c < R::kSlabs; ++c) {
+                    const uint32_t at = dst + c * R::kSlab + lane * box * R::kRow;
+                    tma_load_4d(at, &map_k, full(s), 64 * c, row, c_hk, page);
+                    tma_load_4d(at + R::kTile, &map_v, full(s), 64 * c, row, c_hk, page);
+                }
+            }
+            if (first && lane == 0) {
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c)
+                    tma_load_4d(dst + R::kQ + c * kRows * 128, &map_q, full(s), 64 * c, 0, c_hk, c_sq.row0);
+            }
+            first = last;
+        }
+        if (lane == 0) ws.join[blockIdx.x] = join;
+    } else {
+        // ------------------------------ consumers ------------------------------
+        const int r0 = lane >> 2, t = lane & 3;
+        const int krow = warp * 16;             // this warp's keys in a tile
+        float* merge = reinterpret_cast<float*>(gen + R::kMerge);
+        float* m_sm = reinterpret_cast<float*>(gen + R::kMl);
+        float* l_sm = m_sm + kConsumers * kRows;
+        uint32_t qf[HD / 16][4];
+        float acc[HD / 8][4];
+        float m_run[2], l_run[2], c2[2];
+        int lim[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            m_run[h] = -INFINITY;
+            l_run[h] = 0.f;
+            c2[h] = p.scale_log2;
+            lim[h] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qf[i][e] = 0u;
+        // a barrier of the consumer warps, bounded like every other wait (a hardware barrier would not be)
+        bool ok = true;
+        uint32_t merge_phase = 0;
+        auto merge_sync = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(merge_bar);
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(merge_bar, merge_phase & 1u, abort_flag, 4));
+            ++merge_phase;
+        };
+        for (int i = 0; ok && i < ntiles; ++i) {
+            const int s = i % R::kStages;
+            if (!__all_sync(0xffffffffu, mbar_wait(full(s), (i / R::kStages) & 1, abort_flag, 3))) break;
+            const uint32_t kt = base + s * R::kBytes, vt = kt + R::kTile;
+            const TileMeta& md = meta[s];
+            const int flags = md.flags, key0 = md.key0, kend = md.kend;
+            if (flags & 1) {
+                // ---- a new item: query fragments, limits, empty state ----
+                const uint32_t qt = kt + R::kQ;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = r0 + 8 * h, tok = r / p.group;
+                    m_run[h] = -INFINITY;
+                    l_run[h] = 0.f;
+                    lim[h] = p.causal ? min(kend, md.pos0 + tok + 1) : kend;
+                    if constexpr (!E8) {
+                        // a0/a1: d = 16 ks + 2t (+1); a2/a3: d + 8
+#pragma unroll
+                        for (int ks = 0; ks < HD / 16; ++ks) {
+                            const uint32_t a = qt + (ks >> 2) * kRows * 128 + t * 4;
+                            qf[ks][h] = lds32(a + swz<128>(r, (ks & 3) * 2));
+                            qf[ks][2 + h] = lds32(a + swz<128>(r, (ks & 3) * 2 + 1));
+                        }
+                    } else {
+                        // the contraction index is free to choose: k = 2t, 2t+1 stand for d = 16 ks + 4t, +1 and
+                        // k + 8 for d + 2, +3, which is how four e4m3 bytes of a fragment lie
+                        float amax = 0.f;
+#pragma unroll
+                        for (int ks = 0; ks < HD / 16; ++ks) {
+                            const uint32_t a = qt + (ks >> 2) * kRows * 128 + swz<128>(r, (ks & 3) * 2 + (t >> 1)) + (t & 1) * 8;
+                            const uint2 w = lds64(a);
+                            qf[ks][h] = w.x;
+                            qf[ks][2 + h] = w.y;
+                            if constexpr (BF16) {
+                                const float2 x = pair16_to_f32<true>(w.x), y = pair16_to_f32<true>(w.y);
+                                amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
+                            }
+                        }
+                        if constexpr (BF16) {
+                            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                            // largest magnitude to [1, 2)
+                            const int ex = max(-120, min(120, int(__float_as_uint(amax) >> 23) - 127));
+                            const float f = pow2f(-ex);
+                            c2[h] = p.scale_log2 * pow2f(ex);
+#pragma unroll
+                            for (int ks = 0; ks < HD / 16; ++ks) {
+                                const float2 x = pair16_to_f32<true>(qf[ks][h]), y = pair16_to_f32<true>(qf[ks][2 + h]);
+                                qf[ks][h] = pack16<false>(x.x * f, x.y * f);
+                                qf[ks][2 + h] = pack16<false>(y.x * f, y.y * f);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < HD / 8; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[x][e] = 0.f;
+            }
+            // ---- S = Q K^T for 16 keys: two n-tiles of 8 keys ----
+            float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            if constexpr (!E8) {
+#pragma unroll
+                for (int k2 = 0; k2 < HD / 32; ++k2) {
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const int row = krow + nt * 8 + (lane & 7), c = k2 * 4 + (lane >> 3);
+                        uint32_t bf[4];
+                        ldsm4(kt + (c >> 3) * R::kSlab + swz<128>(row, c & 7), bf);
+                        mma<kBfOps>(sc[nt], qf[2 * k2], bf[0], bf[1]);
+                        mma<kBfOps>(sc[nt], qf[2 * k2 + 1], bf[2], bf[3]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k4 = 0; k4 < HD / 64; ++k4) {
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const int row = krow + nt * 8 + (lane & 7), c = k4 * 4 + (lane >> 3);
+                        uint32_t bf[4];
+                        ldsm4(kt + swz<R::kRow>(row, c), bf);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            mma<false>(sc[nt], qf[4 * k4 + e], e4m3x2_to_f16x2(bf[e] & 0xffffu), e4m3x2_to_f16x2(bf[e] >> 16));
+                    }
+                }
+                // this thread's columns: keys 2t, 2t+1 of each n-tile
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    const uint2 w = lds64(kt + R::kExp + (krow + nt * 8 + 2 * t) * 4);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        sc[nt][2 * h] *= __uint_as_float(w.x);
+                        sc[nt][2 * h + 1] *= __uint_as_float(w.y);
+                    }
+                }
+            }
+            // ---- mask, online softmax (x = score * scale * log2 e) ----
+            const int kb = key0 + krow + 2 * t;
+            const int shift = 31 - __clz(min(p.page, kTileKeys));
+            const uint32_t here0 = (md.pages >> ((krow) >> shift)) & 1u;              // pages hold whole 8-key groups
+            const uint32_t here1 = (md.pages >> ((krow + 8) >> shift)) & 1u;
+            float pr[2][4], alpha[2];
+            bool moved = false;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float v = sc[nt][2 * h + e] * c2[h];
+                        if (kb + nt * 8 + e >= lim[h] || !(nt ? here1 : here0)) v = -INFINITY;
+                        sc[nt][2 * h + e] = v;
+                        mx = fmaxf(mx, v);
+                    }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float m_new = fmaxf(m_run[h], mx);
+                alpha[h] = m_new == m_run[h] ? 1.f : ex2_approx(m_run[h] - m_new);
+                moved |= m_new != m_run[h];
+                const float ref = m_new == -INFINITY ? 0.f : m_new;
+                float sum = 0.f;
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float pv = ex2_approx(sc[nt][2 * h + e] - ref);
+                        pr[nt][2 * h + e] = pv;
+                        sum += pv;
+                    }
+                l_run[h] = l_run[h] * alpha[h] + sum;     // this thread's keys; the quad is added up at the end of the item
+                m_run[h] = m_new;
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int x = 0; x < HD / 8; ++x) {
+                    acc[x][0] *= alpha[0];
+                    acc[x][1] *= alpha[0];
+                    acc[x][2] *= alpha[1];
+                    acc[x][3] *= alpha[1];
+                }
+            }
+            // ---- O += P V ----
+            uint32_t pa[4];
+            pa[0] = pack16<kBfOps>(pr[0][0], pr[0][1]);
+            pa[1] = pack16<kBfOps>(pr[0][2], pr[0][3]);
+            pa[2] = pack16<kBfOps>(pr[1][0], pr[1][1]);
+            pa[3] = pack16<kBfOps>(pr[1][2], pr[1][3]);
+            // past the end of the sequence the page holds anything, NaN too: 0 * NaN must not reach the sum
+            const bool edge = key0 + kTileKeys > kend;
+            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+            if (edge) {
+                keep0 = (kb < kend ? 0xffffu : 0u) | (kb + 1 < kend ? 0xffff0000u : 0u);
+                keep1 = (kb + 8 < kend ? 0xffffu : 0u) | (kb + 9 < kend ? 0xffff0000u : 0u);
+            }
+            if constexpr (!E8) {
+#pragma unroll
+                for (int n2 = 0; n2 < HD / 16; ++n2) {
+                    const int row = krow + ((lane >> 3) & 1) * 8 + (lane & 7), c = n2 * 2 + (lane >> 4);
+                    uint32_t bf[4];
+                    ldsm4_t(vt + (c >> 3) * R::kSlab + swz<128>(row, c & 7), bf);
+                    if (edge) {
+                        bf[0] &= keep0;
+                        bf[1] &= keep1;
+                        bf[2] &= keep0;
+                        bf[3] &= keep1;
+                    }
+                    mma<kBfOps>(acc[2 * n2], pa, bf[0], bf[1]);
+                    mma<kBfOps>(acc[2 * n2 + 1], pa, bf[2], bf[3]);
+                }
+            } else {
+                const uint32_t sv0 = lds32(kt + R::kExp + 512 + (krow + 2 * t) * 2);
+                const uint32_t sv1 = lds32(kt + R::kExp + 512 + (krow + 8 + 2 * t) * 2);
+#pragma unroll
+                for (int n2 = 0; n2 < HD / 32; ++n2) {
+                    const int row = krow + ((lane >> 3) & 1) * 8 + (lane & 7), c = n2 * 2 + (lane >> 4);
+                    uint32_t bf[4];
+                    ldsm4_t(vt + swz<R::kRow>(row, c), bf);   // a register: (d, d+1) of key 2t, (d, d+1) of key 2t+1
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        uint32_t lo = bf[2 * x], hi = bf[2 * x + 1];
+                        if (edge) {
+                            lo &= keep0;
+                            hi &= keep1;
+                        }
+                        lo = __byte_perm(lo, 0, 0x3120);       // d of both keys, then d + 1
+                        hi = __byte_perm(hi, 0, 0x3120);
+                        // n-tile "even": columns d = 16 c + 2n; n-tile "odd": d + 1
+                        mma<false>(acc[4 * n2 + 2 * x], pa, hmul2(e4m3x2_to_f16x2(lo & 0xffffu), sv0),
+                                   hmul2(e4m3x2_to_f16x2(hi & 0xffffu), sv1));
+                        mma<false>(acc[4 * n2 + 2 * x + 1], pa, hmul2(e4m3x2_to_f16x2(lo >> 16), sv0),
+                                   hmul2(e4m3x2_to_f16x2(hi >> 16), sv1));
+                    }
+                }
+            }
+            const int nq = md.nq, row_tok = md.row0, hk = md.hk, slot = md.slot;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(s));
+            if (flags & 2) {
+                // ---- the item ends here: the eight warps' states become one ----
+                const int rows = nq * p.group;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
+                    l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
+                }
+                merge_sync();       // the previous item's merge has been read
+                if (t == 0) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        m_sm[warp * kRows + r0 + 8 * h] = m_run[h];
+                        l_sm[warp * kRows + r0 + 8 * h] = l_run[h];
+                    }
+                }
+                merge_sync();
+                float f[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float M = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, m_sm[w * kRows + r0 + 8 * h]);
+                    f[h] = m_run[h] == -INFINITY ? 0.f : ex2_approx(m_run[h] - M);
+                }
+                // 32 columns at a time: [warp][row][32] fp32
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    if (c > 0) merge_sync();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = r0 + 8 * h;
+                        if (r < rows) {
+                            float* dst = merge + (warp * kRows + r) * 32;
+                            if constexpr (!E8) {
+#pragma unroll
+                                for (int x = 0; x < 4; ++x)
+                                    *reinterpret_cast<float2*>(dst + 8 * x + 2 * t) =
+                                        make_float2(acc[4 * c + x][2 * h] * f[h], acc[4 * c + x][2 * h + 1] * f[h]);
+                            } else {
+                                // two 16-byte units of e4m3: columns 4t .. 4t+3 of each
+#pragma unroll
+                                for (int x = 0; x < 2; ++x)
+                                    *reinterpret_cast<float4*>(dst + 16 * x + 4 * t) =
+                                        make_float4(acc[4 * c + 2 * x][2 * h] * f[h], acc[4 * c + 2 * x + 1][2 * h] * f[h],
+                                                    acc[4 * c + 2 * x][2 * h + 1] * f[h], acc[4 * c + 2 * x + 1][2 * h + 1] * f[h]);
+                            }
+                        }
+                    }
+                    merge_sync();
+                    // 16 rows x 16 column pairs: a pair per thread
+                    const int r = threadIdx.x >> 4, cp = threadIdx.x & 15;
+                    if (r < rows) {
+                        float M = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+                        for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, m_sm[w * kRows + r]);
+#pragma unroll
+                        for (int w = 0; w < kConsumers; ++w) {
+                            const float mw = m_sm[w * kRows + r];
+                            if (mw != -INFINITY) l = fmaf(l_sm[w * kRows + r], ex2_approx(mw - M), l);
+                            const float2 v = *reinterpret_cast<const float2*>(merge + (w * kRows + r) * 32 + 2 * cp);
+                            o0 += v.x;
+                            o1 += v.y;
+                        }
+                        const int d = 32 * c + 2 * cp;
+                        if (flags & 4) {
+                            const size_t at = size_t(slot) * kRows + r;
+                            *reinterpret_cast<float2*>(ws.o + at * HD + d) = make_float2(o0, o1);
+                            if (d == 0) ws.ml[at] = make_float2(M, l);
+                        } else {
+                            const int tok = row_tok + r / p.group, h = hk * p.group + r % p.group;
+                            const float inv = M == -INFINITY ? 0.f : 1.0f / l;
+                            uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.os[0] + int64_t(h) * p.os[1] + d;
+                            const uint32_t w = pack16<BF16>(o0 * inv, o1 * inv);
+                            out[0] = uint16_t(w);
+                            out[1] = uint16_t(w >> 16);
+                            if (p.lse && d == 0)
+                                p.lse[int64_t(tok) * p.Hq + h] = M == -INFINITY ? -INFINITY : M * 0.6931471805599453f + logf(l);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) {
+        *p.status = *abort_flag;
+        __threadfence_system();
+    }
+}
+
+}  // namespace
+
+int paged_decode_rows() { return kRows; }
+
+bool paged_decode_supported(const Gpu* g, const paras_paged_attn_args& a) {
+    return g->cc_major >= 9 && a.dtype != PARAS_F32 && paged_tma_ok(a.cache) && paged_q_tma_ok(a) &&
+           int64_t(a.max_q) * (a.Hq / a.cache.Hkv) <= kRows && g->smem_optin >= 227 * 1024;
+}
+
+int paged_decode_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p, const PagedWorkspace& ws, int G, cudaStream_t s) {
+    int st = check_status_word(g);
+    if (st != PARAS_OK) return st;
+    CUtensorMap mq, mk, mv;
+    if ((st = paged_q_map(&mq, a, p.max_q)) != PARAS_OK) return st;
+    if ((st = paged_cache_map(&mk, a.cache, 0)) != PARAS_OK) return st;
+    if ((st = paged_cache_map(&mv, a.cache, 1)) != PARAS_OK) return st;
+    auto go = [&](auto kernel, int bytes) -> int {
+        PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        kernel<<<G, kThreads, bytes, s>>>(mq, mk, mv, p, ws);
+        PB_LAUNCH_CHECK("paged_decode_kernel");
+        return PARAS_OK;
+    };
+    const bool bf = a.dtype == PARAS_BF16, e8 = a.cache.cache_dtype == PARAS_E4M3;
+#define PB_GO(B, E, H) go(paged_decode_kernel<B, E, H>, Ring<E, H>::kLaunch)
+    if (p.D == 128) st = bf ? (e8 ? PB_GO(true, true, 128) : PB_GO(true, false, 128)) : (e8 ? PB_GO(false, true, 128) : PB_GO(false, false, 128));
+    else st = bf ? (e8 ? PB_GO(true, true, 64) : PB_GO(true, false, 64)) : (e8 ? PB_GO(false, true, 64) : PB_GO(false, false, 64));
+#undef PB_GO
+    if (st != PARAS_OK) return st;
+    return paged_join_launch(p, ws, G, kRows, a.dtype, s);
+}
+
+}  // namespace pb

@@ -27,7 +27,7 @@ OBJ = os.path.join(HERE, "build")
 
 CUDA_SOURCES = ["runtime.cu", "elementwise.cu", "rmsnorm.cu", "sdpa.cu", "sdpa_simt.cu",
                 "sdpa_tc.cu", "sdpa_decode.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_skinny.cu", "sdpa_bwd.cu", "sdpa_bwd_tc.cu", "sdpa_bwd_general.cu", "sdpa_weights.cu", "selftest.cu",
-                "paged_kv.cu", "paged_attn.cu", "paged_join.cu", "paged_decode.cu", "add_rmsnorm.cu"]
+                "paged_kv.cu", "paged_attn.cu", "paged_join.cu", "paged_decode.cu", "paged_tc.cu", "add_rmsnorm.cu"]
 EXT_SOURCES = ["core/device_runtime.cpp", "ops/lifecycle_ops.cpp", "ops/attention_ops.cpp",
                "ops/norm_glu_ops.cpp", "ops/matmul_ops.cpp", "ops/paged_ops.cpp", "python/module.cpp"]
 

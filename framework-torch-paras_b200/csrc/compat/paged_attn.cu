@@ -102,10 +102,13 @@ int check(const paras_paged_attn_args* args, const char* what) {
     return PARAS_OK;
 }
 
-enum class Route { kSimt, kDecode };
+// At most 16 query rows per kv head stream through mma.sync tiles, more go to the tensor-core tiles of 128 rows; fp32,
+// other head dims than 64 and 128, pages that no tile of 128 positions is made of, and unaligned tensors to CUDA cores.
+enum class Route { kSimt, kDecode, kTc };
 Route pick_route(const Gpu* g, const paras_paged_attn_args& a) {
-    return paged_decode_supported(g, a) ? Route::kDecode : Route::kSimt;
+    return paged_decode_supported(g, a) ? Route::kDecode : paged_tc_supported(g, a) ? Route::kTc : Route::kSimt;
 }
+int route_rows(Route r) { return r == Route::kDecode ? paged_decode_rows() : paged_tc_rows(); }
 int stream_ctas(const Gpu* g) { return g->sm_count > 0 ? g->sm_count : 148; }   // persistent, one per SM
 
 PagedParams make_params(const Gpu* g, const paras_paged_attn_args& a) {
@@ -166,7 +169,7 @@ int paras_b200_paged_attn(const paras_paged_attn_args* args) {
     cudaStream_t s = pb::pick_stream(g, a.stream);
     const pb::Route r = pb::pick_route(g, a);
     if (r == pb::Route::kSimt) return pb::paged_simt_launch(p, a.dtype, a.cache.cache_dtype == PARAS_E4M3, s);
-    const int G = pb::stream_ctas(g), rows = pb::paged_decode_rows();
+    const int G = pb::stream_ctas(g), rows = pb::route_rows(r);
     const size_t need = pb::paged_workspace_bytes(G, rows, p.D);
     void* scratch = a.workspace;
     if (scratch) {
@@ -176,8 +179,9 @@ int paras_b200_paged_attn(const paras_paged_attn_args* args) {
     } else if ((st = paras_b200_malloc_async(a.gpu, need, s, &scratch)) != PARAS_OK) {
         return st;
     }
-    st = pb::paged_decode_launch(g, a, p, pb::paged_carve(scratch, G, rows), G, s);
-    if (st == PARAS_OK) pb::tl_paged_kernel = "paged_decode";
+    const pb::PagedWorkspace ws = pb::paged_carve(scratch, G, rows);
+    st = r == pb::Route::kDecode ? pb::paged_decode_launch(g, a, p, ws, G, s) : pb::paged_tc_launch(g, a, p, ws, G, s);
+    if (st == PARAS_OK) pb::tl_paged_kernel = r == pb::Route::kDecode ? "paged_decode" : "paged_tcgen05";
     if (!a.workspace) {
         const int st2 = paras_b200_free_async(a.gpu, scratch, s);
         if (st == PARAS_OK) st = st2;
@@ -193,8 +197,8 @@ int paras_b200_paged_attn_workspace_bytes(const paras_paged_attn_args* args, siz
     pb::DeviceRestore restore;
     pb::Gpu* g = pb::use_gpu(args->gpu, &st);
     if (!g) return st;
-    if (pb::pick_route(g, *args) != pb::Route::kSimt)
-        *bytes = pb::paged_workspace_bytes(pb::stream_ctas(g), pb::paged_decode_rows(), args->cache.D);
+    const pb::Route r = pb::pick_route(g, *args);
+    if (r != pb::Route::kSimt) *bytes = pb::paged_workspace_bytes(pb::stream_ctas(g), pb::route_rows(r), args->cache.D);
     return PARAS_OK;
 }
 

@@ -170,6 +170,10 @@ bool paged_decode_supported(const Gpu* g, const paras_paged_attn_args& a);
 int paged_decode_rows();     // query rows of an item in the workspace
 int paged_decode_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p, const PagedWorkspace& ws, int G, cudaStream_t s);
 
+bool paged_tc_supported(const Gpu* g, const paras_paged_attn_args& a);
+int paged_tc_rows();
+int paged_tc_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p, const PagedWorkspace& ws, int G, cudaStream_t s);
+
 // Can the cache be read by TMA in tiles of 128 positions (page size, alignment, strides)?
 bool paged_tma_ok(const paras_paged_cache& c);
 // Map of the cache's K (which = 0) or V: {D, position, head, page}, box of one page's (at most 128) rows by 128 bytes (the

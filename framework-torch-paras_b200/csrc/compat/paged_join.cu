@@ -34,7 +34,8 @@ paged_join_kernel(const PagedParams p, const PagedWorkspace ws, int rows_per_slo
             for (int i = 0; i < parts; ++i) {
                 const size_t at = size_t(slot(i)) * rows_per_slot + r;
                 const float2 ml = __ldcg(&ws.ml[at]);
-                const float w = ml.x == -INFINITY ? 0.f : tc::ex2_approx(ml.x - M);
+                if (ml.x == -INFINITY) continue;      // a part that saw no key: its outputs may not have been written
+                const float w = tc::ex2_approx(ml.x - M);
                 l = fmaf(w, ml.y, l);
 #pragma unroll
                 for (int e = 0; e < E; e += 2) {

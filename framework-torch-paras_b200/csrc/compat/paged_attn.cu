@@ -130,6 +130,11 @@ PagedParams make_params(const Gpu* g, const paras_paged_attn_args& a) {
     p.scale = float(a.scale);
     p.scale_log2 = p.scale * 1.4426950408889634f;
     p.status = g->status_dev;
+    const int box = c.page < kTileKeys ? c.page : kTileKeys;
+    p.box_shift = 0;
+    while ((2 << p.box_shift) <= box) ++p.box_shift;
+    p.npg = kTileKeys >> p.box_shift;
+    p.tpp = c.page > kTileKeys ? c.page / kTileKeys : 1;
     return p;
 }
 

@@ -1,6 +1,8 @@
 // Internal interfaces of the attention kernels over a paged cache.
 #pragma once
 
+#include <atomic>
+
 #include "paged_common.cuh"
 
 struct CUtensorMap_st;
@@ -23,6 +25,9 @@ struct PagedParams {
     int causal;
     float scale, scale_log2;
     int* status;
+    // Pages as the TMA routes see them: a tile of 128 positions is `npg` boxes of 2^box_shift positions, one per page, or
+    // one box of a page that holds `tpp` tiles.
+    int box_shift, npg, tpp;
 };
 
 // The new tokens of sequence b: first row, count (at most max_q), positions in the cache.  Whatever the device arrays
@@ -161,6 +166,17 @@ __device__ __forceinline__ PagedRange paged_range(int B, int64_t* sums, Tiles ti
     *b0 = int(total[1]);
     *base0 = total[2];
     return r;
+}
+
+// Lets `Kernel` use `bytes` of dynamic shared memory on the current device `gpu`; asked of the driver once per device.
+template <auto Kernel>
+cudaError_t paged_allow_smem(int gpu, int bytes) {
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = uint64_t(1) << (gpu & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // Joins the partial results of cut items: a launch of G blocks after the streaming kernel on the same stream.

@@ -59,7 +59,7 @@ struct TileMeta {        // kMetaBytes, one per stage
     int kend;            // positions the item attends: keys from here on are not
     int pos0;
     uint32_t pages;      // bit i: page i of the tile is there
-    int flags;           // 1 first tile of the item here, 2 last, 4 the item is not whole here
+    int flags;           // 1 first tile of the item here, 2 last, 4 the item is not whole here, 8 keys are to be masked
     int slot;
     int pad[3];
 };
@@ -76,11 +76,11 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
 template <bool BF16>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (BF16) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     } else {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
@@ -156,7 +156,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         PagedJoin join{};
         join.first_slot = -1;
-        const int box = min(p.page, kTileKeys), npg = kTileKeys / box;   // rows and number of boxes of a tile
         const bool exp4 = E8 && p.eks[2] == 1 && p.evs[2] == 1 && ((p.eks[0] | p.eks[1] | p.evs[0] | p.evs[1]) & 3) == 0 &&
                           ((reinterpret_cast<uintptr_t>(p.ek) | reinterpret_cast<uintptr_t>(p.ev)) & 3) == 0;
         // where the tile to be asked for next stands
@@ -178,11 +177,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tile = int(in - int64_t(hk) * nt);
             item0 = base0 + int64_t(hk) * nt;
         }
-        // lane i: page number of box i of the tile, -1 when it is not to be read
+        // lane i: page number of box i of the tile, -1 when it is not to be read; `prow`: the tile's first row in its page
+        int prow = 0;
         auto page_of = [&]() -> int {
-            const int key = tile * kTileKeys + lane * box;
-            if (lane >= npg || key >= kend) return -1;
-            const int pg = __ldg(p.table + int64_t(b) * p.table_stride + key / p.page);
+            int entry = tile * p.npg + lane;
+            if (p.tpp > 1) {
+                entry = tile / p.tpp + lane;
+                prow = (tile - (entry - lane) * p.tpp) * kTileKeys;
+            }
+            if (lane >= p.npg || tile * kTileKeys + (lane << p.box_shift) >= kend) return -1;
+            const int pg = __ldg(p.table + int64_t(b) * p.table_stride + entry);
             return uint32_t(pg) < uint32_t(p.pages) ? pg : -1;
         };
         int pg = ntiles > 0 ? page_of() : -1;
@@ -191,35 +195,32 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         auto exps_of = [&]() {
             if constexpr (E8) {
                 const int key = 4 * lane;
-                const int mine = __shfl_sync(0xffffffffu, pg, key / box);
-                const int at = tile * kTileKeys + key, off = at % p.page;
+                const int mine = __shfl_sync(0xffffffffu, pg, key >> p.box_shift);
+                const int off = prow + (key & ((1 << p.box_shift) - 1));
                 ek4 = ev4 = 0x7f7f7f7fu;
                 if (mine >= 0) {
                     const uint8_t* k = p.ek + int64_t(mine) * p.eks[0] + int64_t(hk) * p.eks[1] + int64_t(off) * p.eks[2];
                     const uint8_t* v = p.ev + int64_t(mine) * p.evs[0] + int64_t(hk) * p.evs[1] + int64_t(off) * p.evs[2];
-                    const int live = kend - at;
                     if (exp4) {
-                        const uint32_t keep = live >= 4 ? 0xffffffffu : live <= 0 ? 0u : (1u << (8 * live)) - 1u;
-                        ek4 = (__ldg(reinterpret_cast<const uint32_t*>(k)) & keep) | (ek4 & ~keep);
-                        ev4 = (__ldg(reinterpret_cast<const uint32_t*>(v)) & keep) | (ev4 & ~keep);
+                        ek4 = __ldg(reinterpret_cast<const uint32_t*>(k));
+                        ev4 = __ldg(reinterpret_cast<const uint32_t*>(v));
                     } else {
+                        ek4 = ev4 = 0;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (e < live) {
-                                ek4 = (ek4 & ~(0xffu << (8 * e))) | (uint32_t(k[e * p.eks[2]]) << (8 * e));
-                                ev4 = (ev4 & ~(0xffu << (8 * e))) | (uint32_t(v[e * p.evs[2]]) << (8 * e));
-                            }
+                        for (int e = 0; e < 4; ++e) {
+                            ek4 |= uint32_t(k[e * p.eks[2]]) << (8 * e);
+                            ev4 |= uint32_t(v[e * p.evs[2]]) << (8 * e);
+                        }
                     }
                 }
             }
         };
-        if (ntiles > 0) exps_of();
+        exps_of();
         bool first = true;
         for (int i = 0; i < ntiles; ++i) {
-            // this tile, and the way to the next one with its loads asked for
-            const int c_pg = pg, c_tile = tile, c_hk = hk, c_kend = kend, c_nt = nt;
+            // this tile, and the way to the next one, whose page numbers are asked for
+            const int c_pg = pg, c_tile = tile, c_hk = hk, c_kend = kend, c_nt = nt, c_prow = prow;
             const PagedSeq c_sq = sq;
-            const uint32_t c_ek = ek4, c_ev = ev4;
             const int64_t c_item0 = item0;
             if (i + 1 < ntiles) {
                 if (++tile == nt) {
@@ -232,20 +233,38 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                 }
                 pg = page_of();
-                exps_of();
             }
             const int s = i % R::kStages;
             if (!__all_sync(0xffffffffu, mbar_wait(empty(s), ((i / R::kStages) & 1) ^ 1u, abort_flag, 2))) break;
             const uint32_t dst = base + s * R::kBytes;
+            if (lane == 0)   // (the arrival itself comes last: what is stored below is part of the stage)
+                asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(full(s)),
+                             "r"(2 * R::kTile + (first ? (HD / 64) * p.max_q * p.group * 128 : 0)) : "memory");
+            __syncwarp();
+            if (lane < p.npg) {
+                const int page = c_pg >= 0 ? c_pg : p.pages;       // (pages outside the tensor read as zeros)
+#pragma unroll
+                for (int c = 0; c < R::kSlabs; ++c) {
+                    const uint32_t at = dst + c * R::kSlab + (lane << p.box_shift) * R::kRow;
+                    tma_load_4d(at, &map_k, full(s), 64 * c, c_prow, c_hk, page);
+                    tma_load_4d(at + R::kTile, &map_v, full(s), 64 * c, c_prow, c_hk, page);
+                }
+            }
+            if (first && lane == 0) {
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c)
+                    tma_load_4d(dst + R::kQ + c * kRows * 128, &map_q, full(s), 64 * c, 0, c_hk, c_sq.row0);
+            }
             const uint32_t there = __ballot_sync(0xffffffffu, c_pg >= 0);
             const bool last = c_tile + 1 == c_nt || i + 1 == ntiles;
             if constexpr (E8) {
-                // (a row's exponent is within [-15, 7]: normal in fp32, 2^-15 the one subnormal in fp16)
+                // A row's exponent is within [-15, 7] (2^-15 the one subnormal in fp16); what lies past the sequence's
+                // end may be any byte, and is held within too: nothing infinite may meet the zeros there.
                 uint32_t kf[4], vh[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    kf[e] = __float_as_uint(pow2f(max(kExpLo, min(kExpHi, int((c_ek >> (8 * e)) & 0xffu) - 127))));
-                    const int x = max(kExpLo, min(kExpHi, int((c_ev >> (8 * e)) & 0xffu) - 127));
+                    kf[e] = __float_as_uint(pow2f(max(kExpLo, min(kExpHi, int((ek4 >> (8 * e)) & 0xffu) - 127))));
+                    const int x = max(kExpLo, min(kExpHi, int((ev4 >> (8 * e)) & 0xffu) - 127));
                     vh[e] = x >= -14 ? uint32_t(x + 15) << 10 : 0x200u;
                 }
                 st_shared_v4(dst + R::kExp + lane * 16, make_uint4(kf[0], kf[1], kf[2], kf[3]));
@@ -262,9 +281,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 m.pos0 = c_sq.pos0;
                 m.pages = there;
                 const bool whole = c_item0 >= range.begin && c_item0 + c_nt <= range.end;
-                m.flags = (first ? 1 : 0) | (last ? 2 : 0) | (whole ? 0 : 4);
                 // the item the range begins with leaves its part in slot 2c, a later one that goes on in 2c+1
                 m.slot = 2 * int(blockIdx.x) + (c_item0 > range.begin ? 1 : 0);
+                // every row attends every key of the tile, and all of it is there
+                const int all = p.causal ? min(c_kend, c_sq.pos0 + 1) : c_kend;
+                const bool full_tile = m.key0 + kTileKeys <= all && there == (1u << p.npg) - 1u;
+                m.flags = (first ? 1 : 0) | (last ? 2 : 0) | (whole ? 0 : 4) | (full_tile ? 0 : 8);
                 if (!whole && c_item0 >= range.begin) {
                     join.first_slot = m.slot;
                     join.last_cta = range.owner(c_item0 + c_nt - 1);
@@ -275,25 +297,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 meta[s] = m;
             }
             __syncwarp();
-            if (lane == 0)
-                mbar_arrive_expect_tx(full(s), 2 * R::kTile + (first ? (HD / 64) * p.max_q * p.group * 128 : 0));
-            __syncwarp();
-            if (lane < npg) {
-                // (pages outside the tensor read as zeros)
-                const int page = c_pg >= 0 ? c_pg : p.pages;
-                const int row = (c_tile * kTileKeys + lane * box) % p.page;
-#pragma unroll
-                for (int c = 0; c < R::kSlabs; ++c) {
-                    const uint32_t at = dst + c * R::kSlab + lane * box * R::kRow;
-                    tma_load_4d(at, &map_k, full(s), 64 * c, row, c_hk, page);
-                    tma_load_4d(at + R::kTile, &map_v, full(s), 64 * c, row, c_hk, page);
-                }
-            }
-            if (first && lane == 0) {
-#pragma unroll
-                for (int c = 0; c < HD / 64; ++c)
-                    tma_load_4d(dst + R::kQ + c * kRows * 128, &map_q, full(s), 64 * c, 0, c_hk, c_sq.row0);
-            }
+            if (lane == 0) mbar_arrive(full(s));
+            if (i + 1 < ntiles) exps_of();    // of the next tile, whose page numbers have come by now
             first = last;
         }
         if (lane == 0) ws.join[blockIdx.x] = join;
@@ -391,63 +396,75 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[x][e] = 0.f;
             }
-            // ---- S = Q K^T for 16 keys: two n-tiles of 8 keys ----
-            float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-            if constexpr (!E8) {
+            // All fragments of a product are asked for before its first MMA, and V's before the softmax: with two warps
+            // on a scheduler nothing else would hide the loads.
+            constexpr int kLd = R::kTile / 4096;     // ldmatrix.x4 of a warp's 16 rows
+            uint32_t kf[kLd][4], vf[kLd][4];
 #pragma unroll
-                for (int k2 = 0; k2 < HD / 32; ++k2) {
+            for (int x = 0; x < kLd; ++x) {
+                const int row = krow + (x & 1) * 8 + (lane & 7), c = (x >> 1) * 4 + (lane >> 3);   // 16-byte unit of the row
+                ldsm4(kt + (E8 ? 0 : (c >> 3) * R::kSlab) + swz<R::kRow>(row, E8 ? c : c & 7), kf[x]);
+            }
+            // ---- S = Q K^T for 16 keys: two n-tiles of 8 keys, even and odd steps summed apart ----
+            float sc[2][4], sd[2][4];
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const int row = krow + nt * 8 + (lane & 7), c = k2 * 4 + (lane >> 3);
-                        uint32_t bf[4];
-                        ldsm4(kt + (c >> 3) * R::kSlab + swz<128>(row, c & 7), bf);
-                        mma<kBfOps>(sc[nt], qf[2 * k2], bf[0], bf[1]);
-                        mma<kBfOps>(sc[nt], qf[2 * k2 + 1], bf[2], bf[3]);
-                    }
-                }
-            } else {
+            for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                for (int k4 = 0; k4 < HD / 64; ++k4) {
+                for (int e = 0; e < 4; ++e) sc[nt][e] = sd[nt][e] = 0.f;
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const int row = krow + nt * 8 + (lane & 7), c = k4 * 4 + (lane >> 3);
-                        uint32_t bf[4];
-                        ldsm4(kt + swz<R::kRow>(row, c), bf);
+            for (int x = 0; x < kLd; ++x) {
+                const int nt = x & 1, k = x >> 1;
+                if constexpr (!E8) {
+                    mma<kBfOps>(sc[nt], qf[2 * k], kf[x][0], kf[x][1]);
+                    mma<kBfOps>(sd[nt], qf[2 * k + 1], kf[x][2], kf[x][3]);
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            mma<false>(sc[nt], qf[4 * k4 + e], e4m3x2_to_f16x2(bf[e] & 0xffffu), e4m3x2_to_f16x2(bf[e] >> 16));
-                    }
-                }
-                // this thread's columns: keys 2t, 2t+1 of each n-tile
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    const uint2 w = lds64(kt + R::kExp + (krow + nt * 8 + 2 * t) * 4);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        sc[nt][2 * h] *= __uint_as_float(w.x);
-                        sc[nt][2 * h + 1] *= __uint_as_float(w.y);
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        mma<false>((e & 1) ? sd[nt] : sc[nt], qf[4 * k + e], e4m3x2_to_f16x2(kf[x][e] & 0xffffu), e4m3x2_to_f16x2(kf[x][e] >> 16));
                 }
             }
-            // ---- mask, online softmax (x = score * scale * log2 e) ----
+#pragma unroll
+            for (int x = 0; x < kLd; ++x) {
+                const int row = krow + ((lane >> 3) & 1) * 8 + (lane & 7), c = x * 2 + (lane >> 4);
+                ldsm4_t(vt + (E8 ? 0 : (c >> 3) * R::kSlab) + swz<R::kRow>(row, E8 ? c : c & 7), vf[x]);
+            }
+            uint32_t sv0 = 0, sv1 = 0;
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+                float2 ks = make_float2(1.f, 1.f);
+                if constexpr (E8) {     // this thread's columns: keys 2t, 2t+1 of each n-tile
+                    const uint2 w = lds64(kt + R::kExp + (krow + nt * 8 + 2 * t) * 4);
+                    ks = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    // x = score * scale * log2 e
+                    sc[nt][2 * h] = (sc[nt][2 * h] + sd[nt][2 * h]) * (ks.x * c2[h]);
+                    sc[nt][2 * h + 1] = (sc[nt][2 * h + 1] + sd[nt][2 * h + 1]) * (ks.y * c2[h]);
+                }
+            }
+            if constexpr (E8) {
+                sv0 = lds32(kt + R::kExp + 512 + (krow + 2 * t) * 2);
+                sv1 = lds32(kt + R::kExp + 512 + (krow + 8 + 2 * t) * 2);
+            }
+            // ---- mask, online softmax ----
             const int kb = key0 + krow + 2 * t;
-            const int shift = 31 - __clz(min(p.page, kTileKeys));
-            const uint32_t here0 = (md.pages >> ((krow) >> shift)) & 1u;              // pages hold whole 8-key groups
-            const uint32_t here1 = (md.pages >> ((krow + 8) >> shift)) & 1u;
+            if (flags & 8) {
+                // (pages hold whole groups of 8 keys)
+                const uint32_t here0 = (md.pages >> (krow >> p.box_shift)) & 1u, here1 = (md.pages >> ((krow + 8) >> p.box_shift)) & 1u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (kb + nt * 8 + e >= lim[h] || !(nt ? here1 : here0)) sc[nt][2 * h + e] = -INFINITY;
+            }
             float pr[2][4], alpha[2];
             bool moved = false;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float v = sc[nt][2 * h + e] * c2[h];
-                        if (kb + nt * 8 + e >= lim[h] || !(nt ? here1 : here0)) v = -INFINITY;
-                        sc[nt][2 * h + e] = v;
-                        mx = fmaxf(mx, v);
-                    }
+                float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float m_new = fmaxf(m_run[h], mx);
@@ -481,49 +498,32 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             pa[1] = pack16<kBfOps>(pr[0][2], pr[0][3]);
             pa[2] = pack16<kBfOps>(pr[1][0], pr[1][1]);
             pa[3] = pack16<kBfOps>(pr[1][2], pr[1][3]);
-            // past the end of the sequence the page holds anything, NaN too: 0 * NaN must not reach the sum
-            const bool edge = key0 + kTileKeys > kend;
-            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-            if (edge) {
-                keep0 = (kb < kend ? 0xffffu : 0u) | (kb + 1 < kend ? 0xffff0000u : 0u);
-                keep1 = (kb + 8 < kend ? 0xffffu : 0u) | (kb + 9 < kend ? 0xffff0000u : 0u);
-            }
-            if constexpr (!E8) {
+            if (key0 + kTileKeys > kend) {
+                // past the end of the sequence the page holds anything, NaN too: 0 * NaN must not reach the sum
+                const uint32_t keep0 = (kb < kend ? 0xffffu : 0u) | (kb + 1 < kend ? 0xffff0000u : 0u);
+                const uint32_t keep1 = (kb + 8 < kend ? 0xffffu : 0u) | (kb + 9 < kend ? 0xffff0000u : 0u);
 #pragma unroll
-                for (int n2 = 0; n2 < HD / 16; ++n2) {
-                    const int row = krow + ((lane >> 3) & 1) * 8 + (lane & 7), c = n2 * 2 + (lane >> 4);
-                    uint32_t bf[4];
-                    ldsm4_t(vt + (c >> 3) * R::kSlab + swz<128>(row, c & 7), bf);
-                    if (edge) {
-                        bf[0] &= keep0;
-                        bf[1] &= keep1;
-                        bf[2] &= keep0;
-                        bf[3] &= keep1;
-                    }
-                    mma<kBfOps>(acc[2 * n2], pa, bf[0], bf[1]);
-                    mma<kBfOps>(acc[2 * n2 + 1], pa, bf[2], bf[3]);
+                for (int x = 0; x < kLd; ++x) {
+                    vf[x][0] &= keep0;
+                    vf[x][1] &= keep1;
+                    vf[x][2] &= keep0;
+                    vf[x][3] &= keep1;
                 }
-            } else {
-                const uint32_t sv0 = lds32(kt + R::kExp + 512 + (krow + 2 * t) * 2);
-                const uint32_t sv1 = lds32(kt + R::kExp + 512 + (krow + 8 + 2 * t) * 2);
+            }
 #pragma unroll
-                for (int n2 = 0; n2 < HD / 32; ++n2) {
-                    const int row = krow + ((lane >> 3) & 1) * 8 + (lane & 7), c = n2 * 2 + (lane >> 4);
-                    uint32_t bf[4];
-                    ldsm4_t(vt + swz<R::kRow>(row, c), bf);   // a register: (d, d+1) of key 2t, (d, d+1) of key 2t+1
+            for (int x = 0; x < kLd; ++x) {
+                if constexpr (!E8) {
+                    mma<kBfOps>(acc[2 * x], pa, vf[x][0], vf[x][1]);
+                    mma<kBfOps>(acc[2 * x + 1], pa, vf[x][2], vf[x][3]);
+                } else {
+                    // a register: (d, d+1) of key 2t, (d, d+1) of key 2t+1; made into d of both keys, d + 1 of both.
+                    // n-tile "even": columns d = 16 c + 2n; n-tile "odd": d + 1
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        uint32_t lo = bf[2 * x], hi = bf[2 * x + 1];
-                        if (edge) {
-                            lo &= keep0;
-                            hi &= keep1;
-                        }
-                        lo = __byte_perm(lo, 0, 0x3120);       // d of both keys, then d + 1
-                        hi = __byte_perm(hi, 0, 0x3120);
-                        // n-tile "even": columns d = 16 c + 2n; n-tile "odd": d + 1
-                        mma<false>(acc[4 * n2 + 2 * x], pa, hmul2(e4m3x2_to_f16x2(lo & 0xffffu), sv0),
+                    for (int y = 0; y < 2; ++y) {
+                        const uint32_t lo = __byte_perm(vf[x][2 * y], 0, 0x3120), hi = __byte_perm(vf[x][2 * y + 1], 0, 0x3120);
+                        mma<false>(acc[4 * x + 2 * y], pa, hmul2(e4m3x2_to_f16x2(lo & 0xffffu), sv0),
                                    hmul2(e4m3x2_to_f16x2(hi & 0xffffu), sv1));
-                        mma<false>(acc[4 * n2 + 2 * x + 1], pa, hmul2(e4m3x2_to_f16x2(lo >> 16), sv0),
+                        mma<false>(acc[4 * x + 2 * y + 1], pa, hmul2(e4m3x2_to_f16x2(lo >> 16), sv0),
                                    hmul2(e4m3x2_to_f16x2(hi >> 16), sv1));
                     }
                 }
@@ -622,6 +622,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
 }
 
+template <bool BF16, bool E8, int HD>
+int launch(int gpu, int G, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
+           const PagedWorkspace& ws) {
+    constexpr int bytes = Ring<E8, HD>::kLaunch;
+    PB_CUDA((paged_allow_smem<paged_decode_kernel<BF16, E8, HD>>(gpu, bytes)));
+    paged_decode_kernel<BF16, E8, HD><<<G, kThreads, bytes, s>>>(mq, mk, mv, p, ws);
+    PB_LAUNCH_CHECK("paged_decode_kernel");
+    return PARAS_OK;
+}
+
 }  // namespace
 
 int paged_decode_rows() { return kRows; }
@@ -638,14 +648,8 @@ int paged_decode_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParam
     if ((st = paged_q_map(&mq, a, p.max_q)) != PARAS_OK) return st;
     if ((st = paged_cache_map(&mk, a.cache, 0)) != PARAS_OK) return st;
     if ((st = paged_cache_map(&mv, a.cache, 1)) != PARAS_OK) return st;
-    auto go = [&](auto kernel, int bytes) -> int {
-        PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        kernel<<<G, kThreads, bytes, s>>>(mq, mk, mv, p, ws);
-        PB_LAUNCH_CHECK("paged_decode_kernel");
-        return PARAS_OK;
-    };
     const bool bf = a.dtype == PARAS_BF16, e8 = a.cache.cache_dtype == PARAS_E4M3;
-#define PB_GO(B, E, H) go(paged_decode_kernel<B, E, H>, Ring<E, H>::kLaunch)
+#define PB_GO(B, E, H) launch<B, E, H>(g->ordinal, G, s, mq, mk, mv, p, ws)
     if (p.D == 128) st = bf ? (e8 ? PB_GO(true, true, 128) : PB_GO(true, false, 128)) : (e8 ? PB_GO(false, true, 128) : PB_GO(false, false, 128));
     else st = bf ? (e8 ? PB_GO(true, true, 64) : PB_GO(true, false, 64)) : (e8 ? PB_GO(false, true, 64) : PB_GO(false, false, 64));
 #undef PB_GO

@@ -58,9 +58,9 @@ template <bool E8> struct Layout {
     static constexpr int kBars = kSums + (kThreads / 32 + 3) * 8 + 8;
     static constexpr int kMisc = kBars + kNumBars * 8;
     static constexpr int kLaunch = kMisc + 16 + 1024;
-    // Registers per thread after setmaxnreg, of 168 at launch: their sum stays below what the CTA was launched with
-    // (384 * 168 = 64512): 256 * 200 + 128 * 96 = 63488, 256 * 192 + 128 * 112 = 63488.
-    static constexpr int kRegsSoftmax = E8 ? 192 : 200, kRegsOther = E8 ? 112 : 96;
+    // Registers per thread after setmaxnreg, of 168 at launch: their sum, 256 * 200 + 128 * 96 = 63488, stays below what
+    // the CTA was launched with, 384 * 168 = 64512.  (A softmax thread with 192 spills a third of its row.)
+    static constexpr int kRegsSoftmax = 200, kRegsOther = 96;
     static_assert(256 * kRegsSoftmax + 128 * kRegsOther < 384 * 168, "register split");
     static_assert(kLaunch <= 227 * 1024, "shared memory of a CTA");
     static_assert(kItem % 16 == 0 && kSums % 8 == 0 && kBars % 8 == 0, "alignment");
@@ -153,14 +153,24 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const uint32_t tmem = *tmem_slot;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    const int box = min(p.page, BN), npg = BN / box;   // rows and number of pages (or of their pieces) in a tile
-    // item i of this CTA for the warps that wait for it; false at the end.  release() after its last use.
-    auto get_item = [&](uint32_t i, Item* it, int tag) -> bool {
+    const int npg = p.npg;              // pages (or, of larger pages, pieces) in a tile
+    // Item i of this CTA for the warps that wait for it, false at the end; its descriptor stays until they let it go.
+    auto wait_item = [&](uint32_t i, int tag) -> bool {
         if (!__all_sync(0xffffffffu, mbar_wait(bar(kBarItemFull + i % kItems), (i / kItems) & 1, abort_flag, tag))) return false;
-        *it = items[i % kItems];
+        if (items[i % kItems].n > 0) return true;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarItemEmpty + i % kItems));
-        return it->n > 0;
+        return false;
+    };
+    auto drop_item = [&](uint32_t i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kBarItemEmpty + i % kItems));
+    };
+    auto get_item = [&](uint32_t i, Item* it, int tag) -> bool {
+        if (!wait_item(i, tag)) return false;
+        *it = items[i % kItems];
+        drop_item(i);
+        return true;
     };
 
     if (warp >= kMmaWarp) {
@@ -198,9 +208,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             bool ok = true;
             // lane i: page of box i of kv tile `t`, -1 where nothing is to be read
             auto page_of = [&](const Item& it, int t) -> int {
-                const int key = t * BN + lane * box;
-                if (lane >= npg || key >= it.kfin) return -1;
-                const int pg = __ldg(p.table + int64_t(it.b) * p.table_stride + key / p.page);
+                if (lane >= npg || t * BN + (lane << p.box_shift) >= it.kfin) return -1;
+                const int entry = p.tpp > 1 ? t / p.tpp : t * npg + lane;
+                const int pg = __ldg(p.table + int64_t(it.b) * p.table_stride + entry);
                 return uint32_t(pg) < uint32_t(p.pages) ? pg : -1;
             };
             // entry: K (which = 0) or V of kv tile t, whose pages are pg
@@ -218,8 +228,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 if (lane == 0) mbar_arrive_expect_tx(full, kChunks * kChunkBytes);
                 __syncwarp();
                 if (lane < npg) {
-                    const uint32_t dst = base + kSmemKV + slot * kPairBytes + (which ? 0 : kTileBytes) + lane * box * 128;
-                    const int page = pg >= 0 ? pg : p.pages, row = (t * BN + lane * box) % p.page;   // (outside: zeros)
+                    const uint32_t dst = base + kSmemKV + slot * kPairBytes + (which ? 0 : kTileBytes) + (lane << p.box_shift) * 128;
+                    const int page = pg >= 0 ? pg : p.pages, row = p.tpp > 1 ? (t % p.tpp) * BN : 0;   // (outside: zeros)
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) tma_load_4d(dst + c * kChunkBytes, which ? &map_v : &map_k, full, 64 * c, row, it.hk, page);
                 }
@@ -259,7 +269,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 // the item the range begins with leaves its part in slot 2c, a later one that goes on in 2c + 1
                 it.slot = 2 * int(blockIdx.x) + (at > range.begin ? 1 : 0);
                 const int end_key = (tile + it.n) * BN;
-                it.edge = !E8 && end_key > it.kfin && it.kfin > end_key - BN && it.kfin % box != 0;
+                it.edge = !E8 && end_key > it.kfin && it.kfin > end_key - BN && (it.kfin & ((1 << p.box_shift) - 1)) != 0;
                 if (it.partial && tile == 0) {
                     join.first_slot = it.slot;
                     join.last_cta = range.owner(at + nt - 1);
@@ -413,7 +423,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 if (!__all_sync(0xffffffffu, mbar_wait(bar(kBarVLand + slot), phase & 1u, abort_flag, 15))) break;
                 if (slot) ++ecnt[1];
                 else ++ecnt[0];
-                const int r0 = it.kfin - (it.kv0 + it.n - 1) * BN, r1 = (r0 + box - 1) / box * box;   // the page's rest
+                const int r0 = it.kfin - (it.kv0 + it.n - 1) * BN, r1 = (r0 + (1 << p.box_shift) - 1) >> p.box_shift << p.box_shift;   // the page's rest
                 for (int i = lane; i < (r1 - r0) * kChunks * 8; i += 32) {
                     const int row = r0 + i / (kChunks * 8), u = i % (kChunks * 8);
                     st_shared_v4(base + kSmemKV + slot * kPairBytes + (u >> 3) * kChunkBytes + row * 128 + (u & 7) * 16, make_uint4(0, 0, 0, 0));
@@ -431,30 +441,39 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const uint32_t raw = base + L::kRaw + w * 8192, scales = base + L::kScale + w * 256;
             int r = 0;
             // Entry x of an item: K_0, then V_j (odd x), K_j+1 (even x): kv tile x / 2.
-            // lane l: page of the warp's rows 2l, 2l+1, and their exponent bytes
+            // lane l looks after the warp's rows 2l and 2l+1: their page, ...
             auto page_for = [&](const Item& it, int x) -> int {
-                const int key = (it.kv0 + (x >> 1)) * BN + w * 64 + 2 * lane;
-                if (key >= it.kfin) return -1;
-                const int pg = __ldg(p.table + int64_t(it.b) * p.table_stride + key / p.page);
+                const int t = it.kv0 + (x >> 1), key = w * 64 + 2 * lane;
+                if (t * BN + key >= it.kfin) return -1;
+                const int pg = __ldg(p.table + int64_t(it.b) * p.table_stride + (p.tpp > 1 ? t / p.tpp : t * npg + (key >> p.box_shift)));
                 return uint32_t(pg) < uint32_t(p.pages) ? pg : -1;
             };
+            auto row_in_page = [&](const Item& it, int x) -> int {
+                const int t = it.kv0 + (x >> 1), key = w * 64 + 2 * lane;
+                return (p.tpp > 1 ? (t % p.tpp) * BN : 0) + (key & ((1 << p.box_shift) - 1));
+            };
+            // ... their exponent bytes (127 where there is no row), ...
             auto exps_for = [&](const Item& it, int x, int pg) -> uint32_t {
-                const int key = (it.kv0 + (x >> 1)) * BN + w * 64 + 2 * lane, off = key % p.page;
                 if (pg < 0) return 0x7f7fu;
                 const int64_t* st = (x & 1) ? p.evs : p.eks;
-                const uint8_t* e = ((x & 1) ? p.ev : p.ek) + int64_t(pg) * st[0] + int64_t(it.hk) * st[1] + int64_t(off) * st[2];
-                const uint32_t hi = key + 1 < it.kfin ? __ldg(e + st[2]) : 0x7fu;
-                return uint32_t(__ldg(e)) | (hi << 8);
+                const uint8_t* e = ((x & 1) ? p.ev : p.ek) + int64_t(pg) * st[0] + int64_t(it.hk) * st[1] + int64_t(row_in_page(it, x)) * st[2];
+                return uint32_t(__ldg(e)) | (uint32_t(__ldg(e + st[2])) << 8);    // (a page holds whole pairs)
             };
-            // asks for unit u (rows u * 32 / kPer ..) of entry x
-            auto fetch = [&](const Item& it, int x, int pg, int u) {
-                const int row = u * (32 / kPer) + lane / kPer, c = lane % kPer;
-                const int page = __shfl_sync(0xffffffffu, pg, row >> 1);
-                const int key = (it.kv0 + (x >> 1)) * BN + w * 64 + row;
-                const bool live = page >= 0 && key < it.kfin;
+            // ... and where they lie: the address of row 2l, with the number of the two that exist in its low bits
+            auto rows_for = [&](const Item& it, int x, int pg) -> uint64_t {
                 const int64_t* st = (x & 1) ? p.cvs : p.cks;
-                const char* src = ((x & 1) ? p.cv : p.ck) +
-                                  (live ? int64_t(page) * st[0] + int64_t(it.hk) * st[1] + int64_t(key % p.page) * st[2] + c * 16 : 0);
+                const char* src = (x & 1) ? p.cv : p.ck;
+                if (pg < 0) return reinterpret_cast<uint64_t>(src);
+                const int live = min(2, it.kfin - ((it.kv0 + (x >> 1)) * BN + w * 64 + 2 * lane));
+                return reinterpret_cast<uint64_t>(src + int64_t(pg) * st[0] + int64_t(it.hk) * st[1] + int64_t(row_in_page(it, x)) * st[2]) | uint64_t(live);
+            };
+            const int my_row = lane / kPer, my_c = lane % kPer;       // of a unit's 32 / kPer rows
+            // asks for unit u (rows u * 32 / kPer ..): `rows` as rows_for gave it, `pitch` the next row's distance
+            auto fetch = [&](uint64_t rows, int64_t pitch, int u) {
+                const int row = u * (32 / kPer) + my_row;
+                const uint64_t at = __shfl_sync(0xffffffffu, rows, row >> 1);
+                const bool live = (row & 1) < int(at & 3);
+                const uint64_t src = (at & ~uint64_t(15)) + (live ? uint64_t((row & 1) * pitch + my_c * 16) : 0);
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + u * 512 + lane * 16), "l"(src), "r"(live ? 16 : 0)
                              : "memory");
             };
@@ -466,7 +485,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (more) {
                 pg = page_for(it, 0);
                 ex = exps_for(it, 0, pg);
-                for (int u = 0; u < kUnits; ++u) fetch(it, 0, pg, u);
+                const uint64_t rows = rows_for(it, 0, pg);
+                for (int u = 0; u < kUnits; ++u) fetch(rows, p.cks[2], u);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             while (ok && more) {
@@ -483,8 +503,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     const bool go = !have_next || next_more;
                     int pg2 = -1;
                     uint32_t ex2 = 0x7f7fu;
+                    uint64_t rows2 = 0;
+                    const int64_t pitch2 = (nxx & 1) ? p.cvs[2] : p.cks[2];
                     if (go) {
                         pg2 = (nxx & 1) ? pg : page_for(nx, nxx);      // V_j lies where K_j does
+                        rows2 = rows_for(nx, nxx, pg2);
                         ex2 = exps_for(nx, nxx, pg2);
                     }
                     const int g = (r + 1) >> 1, slot = g & 1;
@@ -495,9 +518,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     }
                     if (!(x & 1)) {
                         // bit i: page i of the tile is there, from both warps' rows
-                        const int l0 = box >= 64 ? 0 : lane * box / 2;
-                        const int mine = __shfl_sync(0xffffffffu, pg, l0 & 31);
-                        const uint32_t there = __ballot_sync(0xffffffffu, lane < max(1, 64 / box) && mine >= 0);
+                        const int mine = __shfl_sync(0xffffffffu, pg, ((lane << p.box_shift) >> 1) & 31);
+                        const uint32_t there = __ballot_sync(0xffffffffu, lane < max(1, 64 >> p.box_shift) && mine >= 0);
                         if (lane == 0) reinterpret_cast<volatile uint16_t*>(gen + L::kBits)[2 * (g & 3) + w] = uint16_t(there);
                     }
                     // 2^e of this lane's two rows, fp16 twice
@@ -512,11 +534,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     const uint32_t dst = base + kSmemKV + slot * kPairBytes + ((x & 1) ? 0 : kTileBytes);
 #pragma unroll 4
                     for (int u = 0; u < kUnits; ++u) {
-                        const int row = u * (32 / kPer) + lane / kPer, c = lane % kPer;
+                        const int row = u * (32 / kPer) + my_row, c = my_c;
                         const uint4 v = lds128(raw + u * 512 + lane * 16);
                         uint32_t sc;
                         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sc) : "r"(scales + row * 4));
-                        if (go) fetch(nx, nxx, pg2, u);
                         const uint32_t in[4] = {v.x, v.y, v.z, v.w};
                         uint32_t o[8];
 #pragma unroll
@@ -527,6 +548,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                             o[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
                             o[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&bb);
                         }
+                        if (go) fetch(rows2, pitch2, u);      // (what it will overwrite has been read)
                         // 16 elements are two 16-byte units of a 64-element slab; odd slabs write theirs in the other
                         // order, which keeps the eight lanes of a row on different banks
                         const int R = w * 64 + row, odd = (c >> 2) & 1, un = (c & 3) * 2;
@@ -557,22 +579,21 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const uint32_t s_addr = tmem + lane_base + kColS + t * 128, o_addr = tmem + lane_base + kColO + t * 128;
         const uint32_t stage = base + kSmemO + warp * L::kOStage;
         const int row = wq * 32 + lane;                   // of the tile
-        const int shift = 31 - __clz(box);
-        const uint32_t all_pages = npg == 32 ? 0xffffffffu : (1u << npg) - 1u;
+        const uint32_t all_pages = (1u << npg) - 1u;
         bool ok = true;
         uint32_t scnt = 0, ocnt = 0, G = 0;
-        Item it;
-        for (uint32_t seq = 0; ok && get_item(seq, &it, 14); ++seq) {
-            const int nt = t ? it.ntile[1] : it.ntile[0];
-            const uint32_t g0 = G;                          // pair of K_0
+        for (uint32_t seq = 0; ok && wait_item(seq, 14); ++seq, drop_item(seq - 1)) {
+            const Item& it = items[seq % kItems];
+            const int nt = it.ntile[t];
+            uint32_t g = G;                                  // pair of K_j
             G += uint32_t(it.n);
-            const int live = min(pt, it.nq - t * pt) * p.group;            // rows of this tile that are tokens
-            const int crow = t * pt * p.group + row;                       // row of the item
             if (nt == 0) {
                 // a cut item's range that lies beyond this query tile's keys
-                if (it.partial && row < live) ws.ml[size_t(it.slot) * 256 + crow] = make_float2(-INFINITY, 0.f);
+                if (it.partial && row < min(pt, it.nq - t * pt) * p.group)
+                    ws.ml[size_t(it.slot) * 256 + t * pt * p.group + row] = make_float2(-INFINITY, 0.f);
                 continue;
             }
+            int col0 = it.kv0 * BN;
             const int my_keys = keys_at(p, it.kv, it.pos + t * pt + row / p.group);
             const int min_keys = keys_at(p, it.kv, it.pos + t * pt);      // of the tile's first token
             float c2 = p.scale_log2;
@@ -613,9 +634,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 if (lane == 0) mbar_arrive(bar(kBarQConv + t));
             }
             const float inv_c2 = 1.0f / c2;
-            float m = -INFINITY, m_next = -INFINITY, l = 0.f;    // m: reference in units of S, -inf: no key seen yet
+            float m = -INFINITY, m_next = -INFINITY, l = 0.f;     // m: reference in units of S, -inf: no key seen yet
             bool move_ref = false, unseen = true;
-            for (int j = 0; j < nt; ++j) {
+            for (int j = 0; j < nt; ++j, ++g, col0 += BN) {
                 ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarSFull + t), scnt & 1u, abort_flag, 10 + t));
                 if (!ok) break;
                 ++scnt;
@@ -639,9 +660,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     rescale_o(alpha);
                     m = m_next;
                 }
-                const int col0 = (it.kv0 + j) * BN;
-                uint32_t there = bits[(g0 + j) & 3];
-                if (E8) there = box < BN ? (there & 0xffffu) | ((there >> 16) << (64 / box)) : there & 0xffffu;   // (a half per warp)
+                uint32_t there = bits[g & 3];
+                if (E8) there = npg > 1 ? (there & 0xffffu) | ((there >> 16) << (64 >> p.box_shift)) : there & 0xffffu;   // (a half per warp)
                 uint32_t pk[BN / 2];
                 float l_tile;
                 bool bad = false;
@@ -662,7 +682,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     if (there != all_pages) {
 #pragma unroll
                         for (int i = 0; i < BN; ++i)
-                            if (!((there >> (i >> shift)) & 1u)) s[i] = 0xff800000u;
+                            if (!((there >> (i >> p.box_shift)) & 1u)) s[i] = 0xff800000u;
                     }
                     const bool look = unseen || attempt == 1;        // (the same for the whole warp)
                     if (look) {
@@ -715,6 +735,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             ++ocnt;
             tc_fence_after_sync();
             const bool none = m == -INFINITY;
+            const int live = min(pt, it.nq - t * pt) * p.group;            // rows of this tile that are tokens
+            const int crow = t * pt * p.group;                             // its first row in the item
             // Rows leave through the warp's staging buffer, so that a store writes whole pieces of kORow bytes of
             // neighbouring rows: 16-byte unit u of row r sits at u ^ (r mod units).
             constexpr int kUnitsRow = L::kORow / 16;        // 8 or 4 lanes take a row
@@ -744,10 +766,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         const int rr = i * kRowsAt + rr0, tr = wq * 32 + rr;
                         const uint4 v = lds128(stage + rr * L::kORow + ((u0 ^ (rr % kUnitsRow)) << 4));
                         if (tr < live)
-                            *reinterpret_cast<uint4*>(ws.o + (size_t(it.slot) * 256 + t * pt * p.group + tr) * HD + kCols * c + 4 * u0) = v;
+                            *reinterpret_cast<uint4*>(ws.o + (size_t(it.slot) * 256 + crow + tr) * HD + kCols * c + 4 * u0) = v;
                     }
                 }
-                if (row < live) ws.ml[size_t(it.slot) * 256 + crow] = make_float2(none ? -INFINITY : m * c2, l);
+                if (row < live) ws.ml[size_t(it.slot) * 256 + crow + row] = make_float2(none ? -INFINITY : m * c2, l);
             } else {
                 constexpr int kCols = L::kORow / 2;
                 const float inv = none ? 0.f : 1.0f / l;
@@ -803,6 +825,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
 }
 
+template <bool BF16, bool E8, int HD>
+int launch(int gpu, int G, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
+           const PagedWorkspace& ws) {
+    constexpr int bytes = Layout<E8>::kLaunch;
+    PB_CUDA((paged_allow_smem<paged_tc_kernel<BF16, E8, HD>>(gpu, bytes)));
+    paged_tc_kernel<BF16, E8, HD><<<G, kThreads, bytes, s>>>(mq, mk, mv, p, ws);
+    PB_LAUNCH_CHECK("paged_tc_kernel");
+    return PARAS_OK;
+}
+
 }  // namespace
 
 int paged_tc_rows() { return 256; }
@@ -821,14 +853,8 @@ int paged_tc_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p
     if ((st = paged_q_map(&mq, a, BM / p.group)) != PARAS_OK) return st;
     if ((st = paged_cache_map(&mk, a.cache, 0)) != PARAS_OK) return st;
     if ((st = paged_cache_map(&mv, a.cache, 1)) != PARAS_OK) return st;
-    auto go = [&](auto kernel, int bytes) -> int {
-        PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        kernel<<<G, kThreads, bytes, s>>>(mq, mk, mv, p, ws);
-        PB_LAUNCH_CHECK("paged_tc_kernel");
-        return PARAS_OK;
-    };
     const bool bf = a.dtype == PARAS_BF16, e8 = a.cache.cache_dtype == PARAS_E4M3;
-#define PB_GO(B, E, H) go(paged_tc_kernel<B, E, H>, Layout<E>::kLaunch)
+#define PB_GO(B, E, H) launch<B, E, H>(g->ordinal, G, s, mq, mk, mv, p, ws)
     if (p.D == 128) st = bf ? (e8 ? PB_GO(true, true, 128) : PB_GO(true, false, 128)) : (e8 ? PB_GO(false, true, 128) : PB_GO(false, false, 128));
     else st = bf ? (e8 ? PB_GO(true, true, 64) : PB_GO(true, false, 64)) : (e8 ? PB_GO(false, true, 64) : PB_GO(false, false, 64));
 #undef PB_GO

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -173,10 +174,10 @@ def lib() -> C.CDLL:
                                           C.c_int, C.c_void_p]
         L.paras_b200_scale_columns.argtypes = [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
                                                C.c_int, C.c_void_p]
-        L.paras_b200_paged_kv_write.argtypes = [C.POINTER(PagedKvArgs)]
-        L.paras_b200_paged_kv_read.argtypes = [C.POINTER(PagedKvArgs)]
-        L.paras_b200_paged_attn.argtypes = [C.POINTER(PagedAttnArgs)]
-        L.paras_b200_paged_attn_workspace_bytes.argtypes = [C.POINTER(PagedAttnArgs), C.POINTER(C.c_size_t)]
+        L.paras_b200_paged_kv_write.argtypes = [C.c_void_p]
+        L.paras_b200_paged_kv_read.argtypes = [C.c_void_p]
+        L.paras_b200_paged_attn.argtypes = [C.c_void_p]
+        L.paras_b200_paged_attn_workspace_bytes.argtypes = [C.c_void_p, C.POINTER(C.c_size_t)]
         L.paras_b200_paged_attn_last_kernel.restype = C.c_char_p
         L.paras_b200_add_rmsnorm_fwd.argtypes = [C.c_int] + [C.c_void_p] * 6 + [C.c_int64, C.c_int64, C.c_double, C.c_int,
                                                                                 C.c_void_p]
@@ -207,8 +208,8 @@ def _stream_of(t: torch.Tensor, stream) -> int:
     the kernel is ordered with the torch work that produced its inputs and reads its outputs."""
     if stream is not None:
         return int(stream)
-    if t.is_cuda:
-        return int(torch.cuda.current_stream(t.device).cuda_stream) or _LEGACY_DEFAULT_STREAM
+    if t.is_cuda:   # (the raw handle: building a torch.cuda.Stream object costs 2 us a call)
+        return torch._C._cuda_getCurrentRawStream(_gpu_of(t)) or _LEGACY_DEFAULT_STREAM
     return 0
 
 
@@ -568,113 +569,108 @@ def rotate_half(x, *, backward=False, stream=None):
 
 
 # ---- paged key / value cache -----------------------------------------------------------------
-def _index_array(t, like, n, what):
-    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != like.device or \
-            (t.shape[0] > 1 and t.stride(0) != 1):
-        raise RuntimeError(f"paras abi: {what} must be a contiguous int32 vector" + (f" of {n} entries" if n is not None else "")
-                           + " on the tensors' device")
+# The argument blocks are packed in one go: filling some fifty ctypes fields one by one costs several microseconds,
+# more than the smallest of these kernels runs.  The layouts are those of PagedCache, PagedKvArgs and PagedAttnArgs.
+_PACK_CACHE = "4Q12qQq8i"
+_PACK_KV = struct.Struct("=" + _PACK_CACHE + "2Q4q2Q4iQ")
+_PACK_ATTN = struct.Struct("=" + _PACK_CACHE + "3Q4q2Q6id2QQ")
+_ZERO6 = (0,) * 6
+
+
+def _index_array(t, dev, n, what):
+    if t.dtype != torch.int32 or t.shape != (n,) or t.device != dev or not t.is_contiguous():
+        raise RuntimeError(f"paras abi: {what} must be a contiguous int32 vector of {n} entries on the tensors' device")
     return t.data_ptr()
 
 
-def _paged_cache(c, k_cache, v_cache, page_table, k_exp, v_exp, rows):
-    """Fills a ``paras_paged_cache`` and checks what the C side cannot see (shapes, devices, types)."""
-    shape = k_cache.shape
-    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
+def _paged_cache(k_cache, v_cache, page_table, k_exp, v_exp, dev):
+    """The values of a ``paras_paged_cache``, after the checks that the C side cannot make (shapes, devices, types)."""
+    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
+    dtype = k_cache.dtype
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != dtype:
         raise RuntimeError("paras abi: caches must be two [pages, kv heads, page, D] tensors of one type")
-    if shape[3] > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+    if shape[3] > 1 and (ks[3] != 1 or vs[3] != 1):
         raise RuntimeError("paras abi: cache rows must be contiguous")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    ts = page_table.shape
+    if page_table.dtype != torch.int32 or len(ts) != 2 or (ts[1] > 1 and page_table.stride(1) != 1):
         raise RuntimeError("paras abi: page_table must be int32 [sequences, pages] with contiguous rows")
-    dev = rows.device
     if k_cache.device != dev or v_cache.device != dev or page_table.device != dev:
         raise RuntimeError("paras abi: tensors are on different devices")
-    c.k, c.v = k_cache.data_ptr(), v_cache.data_ptr()
-    c.k_strides[:], c.v_strides[:] = k_cache.stride()[:3], v_cache.stride()[:3]
-    if k_cache.dtype == torch.float8_e4m3fn:
-        c.cache_dtype = E4M3
+    if dtype == torch.float8_e4m3fn:
         for e in (k_exp, v_exp):
             if e is None or e.shape != shape[:3] or e.element_size() != 1 or e.device != dev:
                 raise RuntimeError("paras abi: an 8-bit cache needs k_exp and v_exp, bytes of shape [pages, kv heads, page]")
-        c.k_exp, c.v_exp = k_exp.data_ptr(), v_exp.data_ptr()
-        c.k_exp_strides[:], c.v_exp_strides[:] = k_exp.stride(), v_exp.stride()
+        code, kp, vp, es = E4M3, k_exp.data_ptr(), v_exp.data_ptr(), k_exp.stride() + v_exp.stride()
     elif k_exp is not None or v_exp is not None:
         raise RuntimeError("paras abi: k_exp and v_exp belong to an 8-bit cache")
     else:
-        c.cache_dtype = dtype_code(k_cache)
-    c.pages, c.Hkv, c.page, c.D = shape
-    c.page_table, c.table_stride = page_table.data_ptr(), page_table.stride(0)
-    c.B, c.max_pages = page_table.shape
+        code, kp, vp, es = dtype_code(k_cache), 0, 0, _ZERO6
+    return (k_cache.data_ptr(), v_cache.data_ptr(), kp, vp, *ks[:3], *vs[:3], *es, page_table.data_ptr(), page_table.stride(0),
+            code, shape[0], shape[2], shape[1], shape[3], ts[0], ts[1], 0)
 
 
-def _token_rows(t, heads, D, what):
-    s = t.shape
-    if len(s) != 3 or (heads is not None and s[1] != heads) or s[2] != D or (D > 1 and t.stride(2) != 1):
+def _token_rows(t, shape, what):
+    """Strides of {token, head} rows [tokens, heads, D]; `shape` is the cache's."""
+    s, st = t.shape, t.stride()
+    if len(s) != 3 or (what != "q" and s[1] != shape[1]) or s[2] != shape[3] or (s[2] > 1 and st[2] != 1):
         raise RuntimeError(f"paras abi: {what} must be [tokens, heads, D] with contiguous rows that fit the cache")
+    return st[0], st[1]
 
 
 def paged_kv_write(k, v, k_cache, v_cache, page_table, kv_lens, cu_q, *, k_exp=None, v_exp=None, stream=None):
     """Writes new tokens' rows k, v [tokens, kv heads, D] into the paged cache in place (rounded to e4m3 with one
     exponent byte per row when the cache is ``float8_e4m3fn``): row ``cu_q[b] + i`` is position
     ``kv_lens[b] - (cu_q[b+1] - cu_q[b]) + i`` of sequence b."""
-    a = PagedKvArgs()
-    _paged_cache(a.cache, k_cache, v_cache, page_table, k_exp, v_exp, k)
-    _token_rows(k, a.cache.Hkv, a.cache.D, "k")
-    _token_rows(v, a.cache.Hkv, a.cache.D, "v")
-    if v.dtype != k.dtype or v.shape != k.shape or v.device != k.device:
+    dev, shape = k.device, k_cache.shape
+    cache = _paged_cache(k_cache, v_cache, page_table, k_exp, v_exp, dev)
+    ks, vs = _token_rows(k, shape, "k"), _token_rows(v, shape, "v")
+    if v.dtype != k.dtype or v.shape != k.shape or v.device != dev:
         raise RuntimeError("paras abi: k and v must have one type, shape and device")
-    a.k, a.v = k.data_ptr(), v.data_ptr()
-    a.k_strides[:], a.v_strides[:] = k.stride()[:2], v.stride()[:2]
-    a.kv_lens, a.cu = _index_array(kv_lens, k, a.cache.B, "kv_lens"), _index_array(cu_q, k, a.cache.B + 1, "cu_q")
-    a.T, a.dtype = k.shape[0], dtype_code(k)
-    a.gpu, a.stream = _gpu_of(k), _stream_of(k, stream)
-    check(lib().paras_b200_paged_kv_write(C.byref(a)))
+    n = page_table.shape[0]
+    check(lib().paras_b200_paged_kv_write(_PACK_KV.pack(
+        *cache, k.data_ptr(), v.data_ptr(), *ks, *vs, _index_array(kv_lens, dev, n, "kv_lens"),
+        _index_array(cu_q, dev, n + 1, "cu_q"), k.shape[0], dtype_code(k), _gpu_of(k), 0, _stream_of(k, stream))))
 
 
 def paged_kv_read(k_cache, v_cache, page_table, cu_kv, total, *, dtype=None, k_exp=None, v_exp=None, out=None, stream=None):
     """(k, v) [total, kv heads, D]: the first ``cu_kv[b+1] - cu_kv[b]`` positions of every sequence, one after the
     other.  ``dtype`` is the result's type (the cache's, or bfloat16 for an 8-bit one, when omitted); rows behind the
     last sequence keep what ``out`` held."""
-    pages, heads, page, D = k_cache.shape
+    dev, shape = k_cache.device, k_cache.shape
+    cache = _paged_cache(k_cache, v_cache, page_table, k_exp, v_exp, dev)
     if out is None:
         if dtype is None:
             dtype = torch.bfloat16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
-        kv = torch.empty((2, total, heads, D), dtype=dtype, device=k_cache.device)
-        out = (kv[0], kv[1])
+        out = torch.empty((2, total, shape[1], shape[3]), dtype=dtype, device=dev).unbind(0)
     k, v = out
-    a = PagedKvArgs()
-    _paged_cache(a.cache, k_cache, v_cache, page_table, k_exp, v_exp, k)
-    _token_rows(k, heads, D, "k")
-    _token_rows(v, heads, D, "v")
-    if v.dtype != k.dtype or v.shape != k.shape or k.shape[0] != total or v.device != k.device:
-        raise RuntimeError("paras abi: the two outputs must have one type and device and `total` rows")
-    a.k, a.v = k.data_ptr(), v.data_ptr()
-    a.k_strides[:], a.v_strides[:] = k.stride()[:2], v.stride()[:2]
-    a.cu = _index_array(cu_kv, k, a.cache.B + 1, "cu_kv")
-    a.T, a.dtype = total, dtype_code(k)
-    a.gpu, a.stream = _gpu_of(k), _stream_of(k, stream)
-    check(lib().paras_b200_paged_kv_read(C.byref(a)))
+    ks, vs = _token_rows(k, shape, "k"), _token_rows(v, shape, "v")
+    if v.dtype != k.dtype or v.shape != k.shape or k.shape[0] != total or v.device != dev or k.device != dev:
+        raise RuntimeError("paras abi: the two outputs must have one type, the cache's device and `total` rows")
+    check(lib().paras_b200_paged_kv_read(_PACK_KV.pack(
+        *cache, k.data_ptr(), v.data_ptr(), *ks, *vs, 0, _index_array(cu_kv, dev, page_table.shape[0] + 1, "cu_kv"), total,
+        dtype_code(k), _gpu_of(k), 0, _stream_of(k, stream))))
     return k, v
 
 
 def paged_attn_args(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, out, *, causal=True, scale=None, k_exp=None,
-                    v_exp=None, lse=None, workspace=None, stream=None) -> PagedAttnArgs:
-    a = PagedAttnArgs()
-    _paged_cache(a.cache, k_cache, v_cache, page_table, k_exp, v_exp, q)
-    D = a.cache.D
-    _token_rows(q, None, D, "q")
-    if out is not q and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or (D > 1 and out.stride(2) != 1)):
-        raise RuntimeError("paras abi: out must have q's shape, type and device and contiguous rows")
-    a.q, a.out = q.data_ptr(), out.data_ptr()
-    a.lse = lse.data_ptr() if lse is not None else None
-    a.q_strides[:], a.o_strides[:] = q.stride()[:2], out.stride()[:2]
-    a.kv_lens, a.cu = _index_array(kv_lens, q, a.cache.B, "kv_lens"), _index_array(cu_q, q, a.cache.B + 1, "cu_q")
-    a.T, a.Hq, a.max_q = q.shape[0], q.shape[1], max_q
-    a.dtype, a.causal = dtype_code(q), 1 if causal else 0
-    a.scale = float(scale) if scale is not None else D ** -0.5
-    if workspace is not None:
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    a.gpu, a.stream = _gpu_of(q), _stream_of(q, stream)
-    return a
+                    v_exp=None, lse=None, workspace=None, stream=None) -> bytes:
+    """A ``paras_paged_attn_args`` as bytes."""
+    dev, shape = q.device, k_cache.shape
+    cache = _paged_cache(k_cache, v_cache, page_table, k_exp, v_exp, dev)
+    qs = _token_rows(q, shape, "q")
+    if out is q:
+        os_ = qs
+    else:
+        os_ = _token_rows(out, shape, "q")
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+            raise RuntimeError("paras abi: out must have q's shape, type and device and contiguous rows")
+    n = page_table.shape[0]
+    return _PACK_ATTN.pack(
+        *cache, q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else 0, *qs, *os_,
+        _index_array(kv_lens, dev, n, "kv_lens"), _index_array(cu_q, dev, n + 1, "cu_q"), q.shape[0], q.shape[1], max_q,
+        dtype_code(q), 1 if causal else 0, _gpu_of(q), shape[3] ** -0.5 if scale is None else scale,
+        workspace.data_ptr() if workspace is not None else 0,
+        workspace.numel() * workspace.element_size() if workspace is not None else 0, _stream_of(q, stream))
 
 
 def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, *, causal=True, scale=None, k_exp=None,
@@ -685,17 +681,18 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, *, ca
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    a = paged_attn_args(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, out, causal=causal, scale=scale, k_exp=k_exp,
-                        v_exp=v_exp, lse=lse, workspace=workspace, stream=stream)
-    check(lib().paras_b200_paged_attn(C.byref(a)))
+    check(lib().paras_b200_paged_attn(paged_attn_args(
+        q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, out, causal=causal, scale=scale, k_exp=k_exp, v_exp=v_exp,
+        lse=lse, workspace=workspace, stream=stream)))
     return (out, lse) if return_lse else out
 
 
 def paged_attn_workspace_bytes(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, *, causal=True, k_exp=None,
                                v_exp=None) -> int:
-    a = paged_attn_args(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, q, causal=causal, k_exp=k_exp, v_exp=v_exp)
     n = C.c_size_t(0)
-    check(lib().paras_b200_paged_attn_workspace_bytes(C.byref(a), C.byref(n)))
+    check(lib().paras_b200_paged_attn_workspace_bytes(
+        paged_attn_args(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, q, causal=causal, k_exp=k_exp, v_exp=v_exp),
+        C.byref(n)))
     return int(n.value)
 
 
@@ -706,8 +703,9 @@ def paged_attn_last_kernel() -> str:
 # ---- residual addition and RMSNorm -------------------------------------------------------------
 def _norm_operands(x, residual, weight):
     h = x.shape[-1]
+    dtype, dev = x.dtype, x.device
     for t in (residual, weight):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device or not t.is_contiguous()):
+        if t is not None and (t.dtype != dtype or t.device != dev or not t.is_contiguous()):
             raise RuntimeError("paras abi: norm operands must be contiguous, of one type and on one device")
     if not x.is_contiguous() or (residual is not None and residual.shape != x.shape) or \
             (weight is not None and weight.shape != (h,)):
@@ -733,7 +731,7 @@ def add_rmsnorm_quant(x, residual, weight, eps=1e-6, *, group=0, stream=None):
     """(q, scales, h): the same norm in 8 bits, y ~ q * scales, q ``float8_e4m3fn``; one fp32 scale per row
     (``group=0``: scales [rows, 1]) or per ``group`` = 32, 64 or 128 columns (scales [rows, ceil(width / group)])."""
     width, rows = _norm_operands(x, residual, weight)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
     h = torch.empty_like(x) if residual is not None else x
     scales = torch.empty((rows, -(-width // group) if group > 0 else 1), dtype=torch.float32, device=x.device)
     check(lib().paras_b200_add_rmsnorm_quant_fwd(

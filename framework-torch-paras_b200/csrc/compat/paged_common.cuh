@@ -46,6 +46,11 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(uint16_t(two)));
     return r;
 }
+// Four bytes -> two pairs, low bytes first.
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four, uint32_t* lo, uint32_t* hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(*lo), "=r"(*hi) : "r"(four));
+}
 __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
     const uint32_t h = e4m3x2_to_f16x2(two);
     return __half22float2(*reinterpret_cast<const __half2*>(&h));

@@ -6,8 +6,8 @@
 //
 // A persistent CTA per SM takes its part of all tiles (128 positions of one item; paged_attn.cuh says how they are
 // shared out), whatever items these belong to, and its ring of tiles never drains between items.
-//   warp 8      loads: page numbers of the next tile while this one waits for its slot; a TMA box per page; an 8-bit
-//               cache's exponent bytes; what the consumers have to know of the tile
+//   warps 8-10  loads, K, V and an 8-bit cache's exponent bytes: page numbers of the next tile are on their way while
+//               this one waits for its slot; a TMA box per page; what the consumers have to know of the tile
 //   warps 0-7   16 keys of every tile each: S = Q K^T, online softmax in registers, O += P V with P straight from the
 //               accumulators; at the end of an item the eight states are merged through shared memory
 //
@@ -27,7 +27,7 @@ namespace {
 using namespace tc;
 
 constexpr int kConsumers = 8;
-constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int threads_of(bool e8) { return (kConsumers + (e8 ? 3 : 2)) * 32; }
 constexpr int kRows = 16;
 constexpr int kMergeBytes = 16 * 1024;
 constexpr int kMaxStages = 8;
@@ -47,6 +47,7 @@ template <bool E8, int HD> struct Ring {
     static constexpr int kMl = kMerge + kMergeBytes;               // [8][16] maxima, [8][16] sums
     static constexpr int kMeta = kMl + 2 * kConsumers * kRows * 4;
     static constexpr int kSums = kMeta + kMaxStages * kMetaBytes;
+    static constexpr int kThreads = threads_of(E8);
     static constexpr int kBars = kSums + (kThreads / 32 + 3) * 8;
     static constexpr int kMisc = kBars + (2 * kMaxStages + 1) * 8 + 8;
     static constexpr int kLaunch = kMisc + 16 + 1024;
@@ -55,12 +56,13 @@ template <bool E8, int HD> struct Ring {
 };
 
 struct TileMeta {        // kMetaBytes, one per stage
-    int row0, nq, hk, key0;
-    int kend;            // positions the item attends: keys from here on are not
-    int pos0;
-    uint32_t pages;      // bit i: page i of the tile is there
+    int key0;
     int flags;           // 1 first tile of the item here, 2 last, 4 the item is not whole here, 8 keys are to be masked
-    int slot;
+    uint32_t pages;      // bit i: page i of the tile is there
+    int kend;            // positions the item attends: keys from here on are not
+    // with an item's first and last tile only
+    int row0, nq, hk, slot;
+    int pos0;
     int pad[3];
 };
 static_assert(sizeof(TileMeta) == kMetaBytes, "");
@@ -71,6 +73,12 @@ __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// Two 16 x 16 matrices of bytes, transposed: lane l of a row group g = l / 4, t = l % 4 gets, of the first, bytes
+// (row 4t .. 4t+3, column g) and (.., column g + 8), then the same of the second.  Lanes 0-15 and 16-31 name their rows.
+__device__ __forceinline__ void ldsm2_t8(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 template <bool BF16>
@@ -94,6 +102,11 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
     return r;
 }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 r;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+    return r;
+}
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
     uint2 r;
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
@@ -115,7 +128,7 @@ __device__ __forceinline__ int seq_tiles(const PagedParams& p, const PagedSeq& s
 }
 
 template <bool BF16, bool E8, int HD>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Ring<E8, HD>::kThreads, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, const PagedParams p, const PagedWorkspace ws) {
     using R = Ring<E8, HD>;
@@ -132,7 +145,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < R::kStages; ++s) {
-            mbar_init(full(s), 1);
+            mbar_init(full(s), E8 ? 3 : 2);      // the producers
             mbar_init(empty(s), kConsumers);
         }
         mbar_init(merge_bar, kConsumers);
@@ -147,13 +160,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const int ntiles = int(range.end - range.begin);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    if (warp == kConsumers) {
-        // ------------------------------ producer ------------------------------
+    if (warp >= kConsumers) {
+        // ------------------------------ producers ------------------------------
+        // Each walks the same tiles: warp 8 issues K's boxes (and the queries') and describes the tile, warp 9 V's, warp 10
+        // brings the exponents of an 8-bit cache.
         if (lane == 0) {
             tma_prefetch_desc(&map_q);
             tma_prefetch_desc(&map_k);
             tma_prefetch_desc(&map_v);
         }
+        const int role = warp - kConsumers;
         PagedJoin join{};
         join.first_slot = -1;
         const bool exp4 = E8 && p.eks[2] == 1 && p.evs[2] == 1 && ((p.eks[0] | p.eks[1] | p.evs[0] | p.evs[1]) & 3) == 0 &&
@@ -177,7 +193,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tile = int(in - int64_t(hk) * nt);
             item0 = base0 + int64_t(hk) * nt;
         }
-        // lane i: page number of box i of the tile, -1 when it is not to be read; `prow`: the tile's first row in its page
+        // lane i: page number of box i of the tile, -1 when it is not to be read; `prow`: the tile's first row in its page.
+        // (A number out of range is looked at where it is used: here that would wait for the load.)
         int prow = 0;
         auto page_of = [&]() -> int {
             int entry = tile * p.npg + lane;
@@ -186,122 +203,151 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 prow = (tile - (entry - lane) * p.tpp) * kTileKeys;
             }
             if (lane >= p.npg || tile * kTileKeys + (lane << p.box_shift) >= kend) return -1;
-            const int pg = __ldg(p.table + int64_t(b) * p.table_stride + entry);
-            return uint32_t(pg) < uint32_t(p.pages) ? pg : -1;
+            return __ldg(p.table + int64_t(b) * p.table_stride + entry);
+        };
+        auto advance = [&]() {
+            if (++tile == nt) {
+                tile = 0;
+                item0 += nt;
+                if (++hk == p.Hkv) {
+                    hk = 0;
+                    ++b;
+                    enter();
+                }
+            }
         };
         int pg = ntiles > 0 ? page_of() : -1;
-        uint32_t ek4 = 0, ev4 = 0;
         // lane l: exponent bytes of the tile's keys 4l .. 4l+3, 127 where there is no key
-        auto exps_of = [&]() {
-            if constexpr (E8) {
-                const int key = 4 * lane;
-                const int mine = __shfl_sync(0xffffffffu, pg, key >> p.box_shift);
-                const int off = prow + (key & ((1 << p.box_shift) - 1));
-                ek4 = ev4 = 0x7f7f7f7fu;
-                if (mine >= 0) {
-                    const uint8_t* k = p.ek + int64_t(mine) * p.eks[0] + int64_t(hk) * p.eks[1] + int64_t(off) * p.eks[2];
-                    const uint8_t* v = p.ev + int64_t(mine) * p.evs[0] + int64_t(hk) * p.evs[1] + int64_t(off) * p.evs[2];
-                    if (exp4) {
-                        ek4 = __ldg(reinterpret_cast<const uint32_t*>(k));
-                        ev4 = __ldg(reinterpret_cast<const uint32_t*>(v));
-                    } else {
-                        ek4 = ev4 = 0;
+        auto exps_of = [&](uint32_t& ek4, uint32_t& ev4) {
+            const int key = 4 * lane;
+            const int mine = __shfl_sync(0xffffffffu, pg, key >> p.box_shift);
+            const int off = prow + (key & ((1 << p.box_shift) - 1));
+            ek4 = ev4 = 0x7f7f7f7fu;
+            if (uint32_t(mine) < uint32_t(p.pages)) {
+                const uint8_t* k = p.ek + int64_t(mine) * p.eks[0] + int64_t(hk) * p.eks[1] + int64_t(off) * p.eks[2];
+                const uint8_t* v = p.ev + int64_t(mine) * p.evs[0] + int64_t(hk) * p.evs[1] + int64_t(off) * p.evs[2];
+                if (exp4) {
+                    ek4 = __ldg(reinterpret_cast<const uint32_t*>(k));
+                    ev4 = __ldg(reinterpret_cast<const uint32_t*>(v));
+                } else {
+                    ek4 = ev4 = 0;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            ek4 |= uint32_t(k[e * p.eks[2]]) << (8 * e);
-                            ev4 |= uint32_t(v[e * p.evs[2]]) << (8 * e);
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        ek4 |= uint32_t(k[e * p.eks[2]]) << (8 * e);
+                        ev4 |= uint32_t(v[e * p.evs[2]]) << (8 * e);
                     }
                 }
             }
         };
-        exps_of();
-        bool first = true;
-        for (int i = 0; i < ntiles; ++i) {
-            // this tile, and the way to the next one, whose page numbers are asked for
-            const int c_pg = pg, c_tile = tile, c_hk = hk, c_kend = kend, c_nt = nt, c_prow = prow;
-            const PagedSeq c_sq = sq;
-            const int64_t c_item0 = item0;
-            if (i + 1 < ntiles) {
-                if (++tile == nt) {
-                    tile = 0;
-                    item0 += nt;
-                    if (++hk == p.Hkv) {
-                        hk = 0;
-                        ++b;
-                        enter();
-                    }
-                }
-                pg = page_of();
-            }
-            const int s = i % R::kStages;
-            if (!__all_sync(0xffffffffu, mbar_wait(empty(s), ((i / R::kStages) & 1) ^ 1u, abort_flag, 2))) break;
-            const uint32_t dst = base + s * R::kBytes;
-            if (lane == 0)   // (the arrival itself comes last: what is stored below is part of the stage)
-                asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(full(s)),
-                             "r"(2 * R::kTile + (first ? (HD / 64) * p.max_q * p.group * 128 : 0)) : "memory");
-            __syncwarp();
-            if (lane < p.npg) {
-                const int page = c_pg >= 0 ? c_pg : p.pages;       // (pages outside the tensor read as zeros)
-#pragma unroll
-                for (int c = 0; c < R::kSlabs; ++c) {
-                    const uint32_t at = dst + c * R::kSlab + (lane << p.box_shift) * R::kRow;
-                    tma_load_4d(at, &map_k, full(s), 64 * c, c_prow, c_hk, page);
-                    tma_load_4d(at + R::kTile, &map_v, full(s), 64 * c, c_prow, c_hk, page);
+        if (role == 2) {
+            // Exponents, two tiles ahead: a load of them is as slow as one of a whole tile.
+            uint32_t ek[2] = {0, 0}, ev[2] = {0, 0};
+            for (int i = 0; i < 2 && i < ntiles; ++i) {
+                exps_of(ek[i], ev[i]);
+                if (i + 1 < ntiles) {
+                    advance();
+                    pg = page_of();
                 }
             }
-            if (first && lane == 0) {
-#pragma unroll
-                for (int c = 0; c < HD / 64; ++c)
-                    tma_load_4d(dst + R::kQ + c * kRows * 128, &map_q, full(s), 64 * c, 0, c_hk, c_sq.row0);
-            }
-            const uint32_t there = __ballot_sync(0xffffffffu, c_pg >= 0);
-            const bool last = c_tile + 1 == c_nt || i + 1 == ntiles;
-            if constexpr (E8) {
+            for (int i = 0; i < ntiles; ++i) {
+                const int s = i % R::kStages;
+                if (!__all_sync(0xffffffffu, mbar_wait(empty(s), ((i / R::kStages) & 1) ^ 1u, abort_flag, 2))) break;
+                const uint32_t dst = base + s * R::kBytes;
                 // A row's exponent is within [-15, 7] (2^-15 the one subnormal in fp16); what lies past the sequence's
                 // end may be any byte, and is held within too: nothing infinite may meet the zeros there.
                 uint32_t kf[4], vh[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    kf[e] = __float_as_uint(pow2f(max(kExpLo, min(kExpHi, int((ek4 >> (8 * e)) & 0xffu) - 127))));
-                    const int x = max(kExpLo, min(kExpHi, int((ev4 >> (8 * e)) & 0xffu) - 127));
+                    kf[e] = __float_as_uint(pow2f(max(kExpLo, min(kExpHi, int((ek[0] >> (8 * e)) & 0xffu) - 127))));
+                    const int x = max(kExpLo, min(kExpHi, int((ev[0] >> (8 * e)) & 0xffu) - 127));
                     vh[e] = x >= -14 ? uint32_t(x + 15) << 10 : 0x200u;
                 }
                 st_shared_v4(dst + R::kExp + lane * 16, make_uint4(kf[0], kf[1], kf[2], kf[3]));
                 asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + R::kExp + 512 + lane * 8), "r"(vh[0] | (vh[1] << 16)),
                              "r"(vh[2] | (vh[3] << 16)) : "memory");
-            }
-            if (lane == 0) {
-                TileMeta m{};
-                m.row0 = c_sq.row0;
-                m.nq = c_sq.nq;
-                m.hk = c_hk;
-                m.key0 = c_tile * kTileKeys;
-                m.kend = c_kend;
-                m.pos0 = c_sq.pos0;
-                m.pages = there;
-                const bool whole = c_item0 >= range.begin && c_item0 + c_nt <= range.end;
-                // the item the range begins with leaves its part in slot 2c, a later one that goes on in 2c+1
-                m.slot = 2 * int(blockIdx.x) + (c_item0 > range.begin ? 1 : 0);
-                // every row attends every key of the tile, and all of it is there
-                const int all = p.causal ? min(c_kend, c_sq.pos0 + 1) : c_kend;
-                const bool full_tile = m.key0 + kTileKeys <= all && there == (1u << p.npg) - 1u;
-                m.flags = (first ? 1 : 0) | (last ? 2 : 0) | (whole ? 0 : 4) | (full_tile ? 0 : 8);
-                if (!whole && c_item0 >= range.begin) {
-                    join.first_slot = m.slot;
-                    join.last_cta = range.owner(c_item0 + c_nt - 1);
-                    join.row0 = c_sq.row0;
-                    join.nq = c_sq.nq;
-                    join.hk = c_hk;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full(s));
+                ek[0] = ek[1];
+                ev[0] = ev[1];
+                if (i + 2 < ntiles) exps_of(ek[1], ev[1]);    // whose page numbers have come by now
+                if (i + 3 < ntiles) {
+                    advance();
+                    pg = page_of();
                 }
-                meta[s] = m;
             }
+        }
+        bool first = true;
+        for (int i = 0; role != 2 && i < ntiles; ++i) {
+            // this tile, and the way to the next one, whose page numbers are asked for
+            const int c_pg = pg, c_tile = tile, c_hk = hk, c_kend = kend, c_nt = nt, c_prow = prow;
+            const PagedSeq c_sq = sq;
+            const int64_t c_item0 = item0;
+            if (i + 1 < ntiles) {
+                advance();
+                pg = page_of();
+            }
+            const int s = i % R::kStages;
+            if (!__all_sync(0xffffffffu, mbar_wait(empty(s), ((i / R::kStages) & 1) ^ 1u, abort_flag, 2))) break;
+            const uint32_t dst = base + s * R::kBytes;
+            const bool last = c_tile + 1 == c_nt || i + 1 == ntiles;
+            // (pages outside the tensor read as zeros)
+            const bool has = uint32_t(c_pg) < uint32_t(p.pages);
+            const int page = has ? c_pg : p.pages;
+            if (role == 0) {
+                const uint32_t there = __ballot_sync(0xffffffffu, has);
+                if (lane == 0) {
+                    TileMeta& m = meta[s];
+                    const int key0 = c_tile * kTileKeys;
+                    // every row attends every key of the tile, and all of it is there
+                    const int all = p.causal ? min(c_kend, c_sq.pos0 + 1) : c_kend;
+                    const bool full_tile = key0 + kTileKeys <= all && there == (1u << p.npg) - 1u;
+                    int flags = (first ? 1 : 0) | (last ? 2 : 0) | (full_tile ? 0 : 8);
+                    if (first || last) {
+                        const bool whole = c_item0 >= range.begin && c_item0 + c_nt <= range.end;
+                        flags |= whole ? 0 : 4;
+                        // the item the range begins with leaves its part in slot 2c, a later one that goes on in 2c+1
+                        const int slot = 2 * int(blockIdx.x) + (c_item0 > range.begin ? 1 : 0);
+                        m.row0 = c_sq.row0;
+                        m.nq = c_sq.nq;
+                        m.hk = c_hk;
+                        m.slot = slot;
+                        m.pos0 = c_sq.pos0;
+                        if (!whole && c_item0 >= range.begin) {
+                            join.first_slot = slot;
+                            join.last_cta = range.owner(c_item0 + c_nt - 1);
+                            join.row0 = c_sq.row0;
+                            join.nq = c_sq.nq;
+                            join.hk = c_hk;
+                        }
+                    }
+                    m.key0 = key0;
+                    m.flags = flags;
+                    m.pages = there;
+                    m.kend = c_kend;
+                }
+            }
+            const CUtensorMap* map = role ? &map_v : &map_k;
+            const uint32_t at = dst + (role ? R::kTile : 0);
+            if (lane == 0)
+                mbar_arrive_expect_tx(full(s), R::kTile + (role == 0 && first ? (HD / 64) * p.max_q * p.group * 128 : 0));
             __syncwarp();
-            if (lane == 0) mbar_arrive(full(s));
-            if (i + 1 < ntiles) exps_of();    // of the next tile, whose page numbers have come by now
+            // one lane issues: a box per lane would be issued one after the other too, with a loop around it
+            for (int x = 0; x < p.npg; ++x) {
+                const int pgx = __shfl_sync(0xffffffffu, page, x);
+                if (lane == 0) {
+#pragma unroll
+                    for (int c = 0; c < R::kSlabs; ++c)
+                        tma_load_4d(at + c * R::kSlab + (x << p.box_shift) * R::kRow, map, full(s), 64 * c, c_prow, c_hk, pgx);
+                }
+            }
+            if (role == 0 && first && lane == 0) {
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c)
+                    tma_load_4d(dst + R::kQ + c * kRows * 128, &map_q, full(s), 64 * c, 0, c_hk, c_sq.row0);
+            }
             first = last;
         }
-        if (lane == 0) ws.join[blockIdx.x] = join;
+        if (role == 0 && lane == 0) ws.join[blockIdx.x] = join;
     } else {
         // ------------------------------ consumers ------------------------------
         const int r0 = lane >> 2, t = lane & 3;
@@ -402,7 +448,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             uint32_t kf[kLd][4], vf[kLd][4];
 #pragma unroll
             for (int x = 0; x < kLd; ++x) {
-                const int row = krow + (x & 1) * 8 + (lane & 7), c = (x >> 1) * 4 + (lane >> 3);   // 16-byte unit of the row
+                // column n of an n-tile is any key: key n of 8, or, where four keys of V share a register, the one that
+                // leaves a thread with keys 4t, 4t+1 of the first n-tile and 4t+2, 4t+3 of the second
+                const int row = krow + (E8 ? 4 * ((lane & 7) >> 1) + 2 * (x & 1) + (lane & 1) : (x & 1) * 8 + (lane & 7));
+                const int c = (x >> 1) * 4 + (lane >> 3);   // 16-byte unit of the row
                 ldsm4(kt + (E8 ? 0 : (c >> 3) * R::kSlab) + swz<R::kRow>(row, E8 ? c : c & 7), kf[x]);
             }
             // ---- S = Q K^T for 16 keys: two n-tiles of 8 keys, even and odd steps summed apart ----
@@ -419,46 +468,50 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     mma<kBfOps>(sd[nt], qf[2 * k + 1], kf[x][2], kf[x][3]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        mma<false>((e & 1) ? sd[nt] : sc[nt], qf[4 * k + e], e4m3x2_to_f16x2(kf[x][e] & 0xffffu), e4m3x2_to_f16x2(kf[x][e] >> 16));
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t lo, hi;
+                        e4m3x4_to_f16x4(kf[x][e], &lo, &hi);
+                        mma<false>((e & 1) ? sd[nt] : sc[nt], qf[4 * k + e], lo, hi);
+                    }
                 }
             }
 #pragma unroll
             for (int x = 0; x < kLd; ++x) {
                 const int row = krow + ((lane >> 3) & 1) * 8 + (lane & 7), c = x * 2 + (lane >> 4);
-                ldsm4_t(vt + (E8 ? 0 : (c >> 3) * R::kSlab) + swz<R::kRow>(row, E8 ? c : c & 7), vf[x]);
+                if constexpr (E8) ldsm2_t8(vt + swz<R::kRow>(row, c), vf[x]);
+                else ldsm4_t(vt + (c >> 3) * R::kSlab + swz<128>(row, c & 7), vf[x]);
             }
-            uint32_t sv0 = 0, sv1 = 0;
+            // this thread's columns of n-tile nt: keys first + step * nt, + 1
+            const int first = krow + (E8 ? 4 : 2) * t;
+            constexpr int kStep = E8 ? 2 : 8;
+            uint4 ks = make_uint4(0, 0, 0, 0);
+            uint2 sv = make_uint2(0, 0);
+            if constexpr (E8) {
+                ks = lds128(kt + R::kExp + first * 4);
+                sv = lds64(kt + R::kExp + 512 + first * 2);
+            }
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
-                float2 ks = make_float2(1.f, 1.f);
-                if constexpr (E8) {     // this thread's columns: keys 2t, 2t+1 of each n-tile
-                    const uint2 w = lds64(kt + R::kExp + (krow + nt * 8 + 2 * t) * 4);
-                    ks = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
-                }
+                const float k0 = E8 ? __uint_as_float(nt ? ks.z : ks.x) : 1.f, k1 = E8 ? __uint_as_float(nt ? ks.w : ks.y) : 1.f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     // x = score * scale * log2 e
-                    sc[nt][2 * h] = (sc[nt][2 * h] + sd[nt][2 * h]) * (ks.x * c2[h]);
-                    sc[nt][2 * h + 1] = (sc[nt][2 * h + 1] + sd[nt][2 * h + 1]) * (ks.y * c2[h]);
+                    sc[nt][2 * h] = (sc[nt][2 * h] + sd[nt][2 * h]) * (k0 * c2[h]);
+                    sc[nt][2 * h + 1] = (sc[nt][2 * h + 1] + sd[nt][2 * h + 1]) * (k1 * c2[h]);
                 }
             }
-            if constexpr (E8) {
-                sv0 = lds32(kt + R::kExp + 512 + (krow + 2 * t) * 2);
-                sv1 = lds32(kt + R::kExp + 512 + (krow + 8 + 2 * t) * 2);
-            }
             // ---- mask, online softmax ----
-            const int kb = key0 + krow + 2 * t;
+            const int kb = key0 + first;
             if (flags & 8) {
-                // (pages hold whole groups of 8 keys)
-                const uint32_t here0 = (md.pages >> (krow >> p.box_shift)) & 1u, here1 = (md.pages >> ((krow + 8) >> p.box_shift)) & 1u;
+                // (a page holds whole groups of 8 keys, so both of an n-tile's)
+                const uint32_t here0 = (md.pages >> (first >> p.box_shift)) & 1u, here1 = (md.pages >> ((first + kStep) >> p.box_shift)) & 1u;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
-                            if (kb + nt * 8 + e >= lim[h] || !(nt ? here1 : here0)) sc[nt][2 * h + e] = -INFINITY;
+                            if (kb + nt * kStep + e >= lim[h] || !(nt ? here1 : here0)) sc[nt][2 * h + e] = -INFINITY;
             }
             float pr[2][4], alpha[2];
             bool moved = false;
@@ -500,14 +553,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             pa[3] = pack16<kBfOps>(pr[1][2], pr[1][3]);
             if (key0 + kTileKeys > kend) {
                 // past the end of the sequence the page holds anything, NaN too: 0 * NaN must not reach the sum
-                const uint32_t keep0 = (kb < kend ? 0xffffu : 0u) | (kb + 1 < kend ? 0xffff0000u : 0u);
-                const uint32_t keep1 = (kb + 8 < kend ? 0xffffu : 0u) | (kb + 9 < kend ? 0xffff0000u : 0u);
+                if constexpr (E8) {
+                    const int live = kend - kb;      // of the four keys of a register
+                    const uint32_t keep = live >= 4 ? 0xffffffffu : live <= 0 ? 0u : (1u << (8 * live)) - 1u;
 #pragma unroll
-                for (int x = 0; x < kLd; ++x) {
-                    vf[x][0] &= keep0;
-                    vf[x][1] &= keep1;
-                    vf[x][2] &= keep0;
-                    vf[x][3] &= keep1;
+                    for (int x = 0; x < kLd; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) vf[x][e] &= keep;
+                } else {
+                    const uint32_t keep0 = (kb < kend ? 0xffffu : 0u) | (kb + 1 < kend ? 0xffff0000u : 0u);
+                    const uint32_t keep1 = (kb + 8 < kend ? 0xffffu : 0u) | (kb + 9 < kend ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int x = 0; x < kLd; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) vf[x][e] &= (e & 1) ? keep1 : keep0;
                 }
             }
 #pragma unroll
@@ -516,19 +575,21 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     mma<kBfOps>(acc[2 * x], pa, vf[x][0], vf[x][1]);
                     mma<kBfOps>(acc[2 * x + 1], pa, vf[x][2], vf[x][3]);
                 } else {
-                    // a register: (d, d+1) of key 2t, (d, d+1) of key 2t+1; made into d of both keys, d + 1 of both.
-                    // n-tile "even": columns d = 16 c + 2n; n-tile "odd": d + 1
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const uint32_t lo = __byte_perm(vf[x][2 * y], 0, 0x3120), hi = __byte_perm(vf[x][2 * y + 1], 0, 0x3120);
-                        mma<false>(acc[4 * x + 2 * y], pa, hmul2(e4m3x2_to_f16x2(lo & 0xffffu), sv0),
-                                   hmul2(e4m3x2_to_f16x2(hi & 0xffffu), sv1));
-                        mma<false>(acc[4 * x + 2 * y + 1], pa, hmul2(e4m3x2_to_f16x2(lo >> 16), sv0),
-                                   hmul2(e4m3x2_to_f16x2(hi >> 16), sv1));
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t lo, hi;
+                        e4m3x4_to_f16x4(vf[x][e], &lo, &hi);
+                        mma<false>(acc[4 * x + e], pa, hmul2(lo, sv.x), hmul2(hi, sv.y));
                     }
                 }
             }
-            const int nq = md.nq, row_tok = md.row0, hk = md.hk, slot = md.slot;
+            int nq = 0, row_tok = 0, hk = 0, slot = 0;
+            if (flags & 2) {
+                nq = md.nq;
+                row_tok = md.row0;
+                hk = md.hk;
+                slot = md.slot;
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(s));
             if (flags & 2) {
@@ -565,19 +626,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         const int r = r0 + 8 * h;
                         if (r < rows) {
                             float* dst = merge + (warp * kRows + r) * 32;
-                            if constexpr (!E8) {
 #pragma unroll
-                                for (int x = 0; x < 4; ++x)
-                                    *reinterpret_cast<float2*>(dst + 8 * x + 2 * t) =
-                                        make_float2(acc[4 * c + x][2 * h] * f[h], acc[4 * c + x][2 * h + 1] * f[h]);
-                            } else {
-                                // two 16-byte units of e4m3: columns 4t .. 4t+3 of each
-#pragma unroll
-                                for (int x = 0; x < 2; ++x)
-                                    *reinterpret_cast<float4*>(dst + 16 * x + 4 * t) =
-                                        make_float4(acc[4 * c + 2 * x][2 * h] * f[h], acc[4 * c + 2 * x + 1][2 * h] * f[h],
-                                                    acc[4 * c + 2 * x][2 * h + 1] * f[h], acc[4 * c + 2 * x + 1][2 * h + 1] * f[h]);
-                            }
+                            for (int x = 0; x < 4; ++x)
+                                *reinterpret_cast<float2*>(dst + 8 * x + 2 * t) =
+                                    make_float2(acc[4 * c + x][2 * h] * f[h], acc[4 * c + x][2 * h + 1] * f[h]);
                         }
                     }
                     merge_sync();
@@ -627,7 +679,7 @@ int launch(int gpu, int G, cudaStream_t s, const CUtensorMap& mq, const CUtensor
            const PagedWorkspace& ws) {
     constexpr int bytes = Ring<E8, HD>::kLaunch;
     PB_CUDA((paged_allow_smem<paged_decode_kernel<BF16, E8, HD>>(gpu, bytes)));
-    paged_decode_kernel<BF16, E8, HD><<<G, kThreads, bytes, s>>>(mq, mk, mv, p, ws);
+    paged_decode_kernel<BF16, E8, HD><<<G, Ring<E8, HD>::kThreads, bytes, s>>>(mq, mk, mv, p, ws);
     PB_LAUNCH_CHECK("paged_decode_kernel");
     return PARAS_OK;
 }

@@ -72,8 +72,9 @@ paged_kv_write_kernel(const KvParams p) {
     if (l16 * N < p.D) load_row<T, N>(row + l16 * N, f);
     int page = 0, off = 0;
     if (!locate<true>(p, t, &page, &off) || uint32_t(page) >= uint32_t(p.pages)) return;
-    const int64_t* cs = half ? p.cvs : p.cks;
-    const int64_t at = int64_t(page) * cs[0] + int64_t(h) * cs[1] + int64_t(off) * cs[2];
+    // (strides are selected one by one: a pointer into the parameters would copy them to local memory)
+    const int64_t at = int64_t(page) * (half ? p.cvs[0] : p.cks[0]) + int64_t(h) * (half ? p.cvs[1] : p.cks[1]) +
+                       int64_t(off) * (half ? p.cvs[2] : p.cks[2]);
     if constexpr (CACHE8) {
         float amax = 0.f;   // (fmaxf skips NaN)
 #pragma unroll
@@ -101,8 +102,8 @@ paged_kv_write_kernel(const KvParams p) {
             }
         }
         if (l16 == 0) {
-            const int64_t* es = half ? p.evs : p.eks;
-            (half ? p.ev : p.ek)[int64_t(page) * es[0] + int64_t(h) * es[1] + int64_t(off) * es[2]] = uint8_t(ex + 127);
+            (half ? p.ev : p.ek)[int64_t(page) * (half ? p.evs[0] : p.eks[0]) + int64_t(h) * (half ? p.evs[1] : p.eks[1]) +
+                                 int64_t(off) * (half ? p.evs[2] : p.eks[2])] = uint8_t(ex + 127);
         }
     } else {
         T* out = reinterpret_cast<T*>(half ? p.cv : p.ck) + at;
@@ -134,14 +135,14 @@ paged_kv_read_kernel(const KvParams p) {
     const int b = warp_count_le(p.cu + 1, p.B, t);
     if (b >= p.B || t < __ldg(p.cu + b)) return;   // a row of no sequence
     const bool have = locate<false>(p, t, &page, &off) && uint32_t(page) < uint32_t(p.pages);
-    const int64_t* cs = half ? p.cvs : p.cks;
-    const int64_t at = have ? int64_t(page) * cs[0] + int64_t(h) * cs[1] + int64_t(off) * cs[2] : 0;
+    const int64_t at = have ? int64_t(page) * (half ? p.cvs[0] : p.cks[0]) + int64_t(h) * (half ? p.cvs[1] : p.cks[1]) +
+                                  int64_t(off) * (half ? p.cvs[2] : p.cks[2]) : 0;
     T* row = half ? reinterpret_cast<T*>(p.v) + int64_t(t) * p.vs[0] + int64_t(h) * p.vs[1]
                   : reinterpret_cast<T*>(p.k) + int64_t(t) * p.ks[0] + int64_t(h) * p.ks[1];
     float s = 0.f;
     if (CACHE8 && have) {
-        const int64_t* es = half ? p.evs : p.eks;
-        s = exp_byte((half ? p.ev : p.ek)[int64_t(page) * es[0] + int64_t(h) * es[1] + int64_t(off) * es[2]]);
+        s = exp_byte((half ? p.ev : p.ek)[int64_t(page) * (half ? p.evs[0] : p.eks[0]) + int64_t(h) * (half ? p.evs[1] : p.eks[1]) +
+                                          int64_t(off) * (half ? p.evs[2] : p.eks[2])]);
     }
     for (int d = l16 * N; d < p.D; d += 16 * N) {
         float f[N];

@@ -441,31 +441,43 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const uint32_t raw = base + L::kRaw + w * 8192, scales = base + L::kScale + w * 256;
             int r = 0;
             // Entry x of an item: K_0, then V_j (odd x), K_j+1 (even x): kv tile x / 2.
+            struct Part { int b, hk, kv0, n, kfin; };      // what this role needs of an item
+            auto get_part = [&](uint32_t i, Part* it) -> bool {
+                it->n = 0;
+                if (!wait_item(i, 14)) return false;
+                const Item& src = items[i % kItems];
+                *it = Part{src.b, src.hk, src.kv0, src.n, src.kfin};
+                drop_item(i);
+                return true;
+            };
             // lane l looks after the warp's rows 2l and 2l+1: their page, ...
-            auto page_for = [&](const Item& it, int x) -> int {
+            auto page_for = [&](const Part& it, int x) -> int {
                 const int t = it.kv0 + (x >> 1), key = w * 64 + 2 * lane;
                 if (t * BN + key >= it.kfin) return -1;
                 const int pg = __ldg(p.table + int64_t(it.b) * p.table_stride + (p.tpp > 1 ? t / p.tpp : t * npg + (key >> p.box_shift)));
                 return uint32_t(pg) < uint32_t(p.pages) ? pg : -1;
             };
-            auto row_in_page = [&](const Item& it, int x) -> int {
+            auto row_in_page = [&](const Part& it, int x) -> int {
                 const int t = it.kv0 + (x >> 1), key = w * 64 + 2 * lane;
                 return (p.tpp > 1 ? (t % p.tpp) * BN : 0) + (key & ((1 << p.box_shift) - 1));
             };
             // ... their exponent bytes (127 where there is no row), ...
-            auto exps_for = [&](const Item& it, int x, int pg) -> uint32_t {
+            auto exps_for = [&](const Part& it, int x, int pg) -> uint32_t {
                 if (pg < 0) return 0x7f7fu;
-                const int64_t* st = (x & 1) ? p.evs : p.eks;
-                const uint8_t* e = ((x & 1) ? p.ev : p.ek) + int64_t(pg) * st[0] + int64_t(it.hk) * st[1] + int64_t(row_in_page(it, x)) * st[2];
-                return uint32_t(__ldg(e)) | (uint32_t(__ldg(e + st[2])) << 8);    // (a page holds whole pairs)
+                const bool v = x & 1;      // (selected one by one: a pointer into the parameters would copy them to local memory)
+                const int64_t st = v ? p.evs[2] : p.eks[2];
+                const uint8_t* e = (v ? p.ev : p.ek) + int64_t(pg) * (v ? p.evs[0] : p.eks[0]) + int64_t(it.hk) * (v ? p.evs[1] : p.eks[1]) +
+                                   int64_t(row_in_page(it, x)) * st;
+                return uint32_t(__ldg(e)) | (uint32_t(__ldg(e + st)) << 8);    // (a page holds whole pairs)
             };
             // ... and where they lie: the address of row 2l, with the number of the two that exist in its low bits
-            auto rows_for = [&](const Item& it, int x, int pg) -> uint64_t {
-                const int64_t* st = (x & 1) ? p.cvs : p.cks;
-                const char* src = (x & 1) ? p.cv : p.ck;
+            auto rows_for = [&](const Part& it, int x, int pg) -> uint64_t {
+                const bool v = x & 1;
+                const char* src = v ? p.cv : p.ck;
                 if (pg < 0) return reinterpret_cast<uint64_t>(src);
                 const int live = min(2, it.kfin - ((it.kv0 + (x >> 1)) * BN + w * 64 + 2 * lane));
-                return reinterpret_cast<uint64_t>(src + int64_t(pg) * st[0] + int64_t(it.hk) * st[1] + int64_t(row_in_page(it, x)) * st[2]) | uint64_t(live);
+                return reinterpret_cast<uint64_t>(src + int64_t(pg) * (v ? p.cvs[0] : p.cks[0]) + int64_t(it.hk) * (v ? p.cvs[1] : p.cks[1]) +
+                                                  int64_t(row_in_page(it, x)) * (v ? p.cvs[2] : p.cks[2])) | uint64_t(live);
             };
             const int my_row = lane / kPer, my_c = lane % kPer;       // of a unit's 32 / kPer rows
             // asks for unit u (rows u * 32 / kPer ..): `rows` as rows_for gave it, `pitch` the next row's distance
@@ -477,8 +489,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + u * 512 + lane * 16), "l"(src), "r"(live ? 16 : 0)
                              : "memory");
             };
-            Item it, nx;
-            bool more = get_item(0, &it, 14), ok = true;
+            Part it, nx;
+            bool more = get_part(0, &it), ok = true;
             uint32_t seq = 0;
             int pg = -1;
             uint32_t ex = 0x7f7fu;
@@ -496,7 +508,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     // what comes after this entry
                     int nxx = x + 1;
                     if (nxx == 2 * it.n) {
-                        next_more = get_item(++seq, &nx, 14);
+                        next_more = get_part(++seq, &nx);
                         have_next = true;
                         nxx = 0;
                     }
@@ -532,30 +544,41 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     asm volatile("cp.async.wait_group 0;" ::: "memory");
                     __syncwarp();
                     const uint32_t dst = base + kSmemKV + slot * kPairBytes + ((x & 1) ? 0 : kTileBytes);
-#pragma unroll 4
-                    for (int u = 0; u < kUnits; ++u) {
-                        const int row = u * (32 / kPer) + my_row, c = my_c;
-                        const uint4 v = lds128(raw + u * 512 + lane * 16);
-                        uint32_t sc;
-                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sc) : "r"(scales + row * 4));
-                        const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-                        uint32_t o[8];
+                    // four units at a time: their loads side by side, then their conversions
+#pragma unroll 1
+                    for (int u4 = 0; u4 < kUnits; u4 += 4) {
+                        uint4 v[4];
+                        uint32_t sc[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const __half2 s2 = *reinterpret_cast<const __half2*>(&sc);
-                            uint32_t lo = e4m3x2_to_f16x2(in[i] & 0xffffu), hi = e4m3x2_to_f16x2(in[i] >> 16);
-                            const __half2 a = __hmul2(*reinterpret_cast<__half2*>(&lo), s2), bb = __hmul2(*reinterpret_cast<__half2*>(&hi), s2);
-                            o[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
-                            o[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&bb);
+                        for (int y = 0; y < 4; ++y) {
+                            v[y] = lds128(raw + (u4 + y) * 512 + lane * 16);
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sc[y]) : "r"(scales + ((u4 + y) * (32 / kPer) + my_row) * 4));
                         }
-                        if (go) fetch(rows2, pitch2, u);      // (what it will overwrite has been read)
-                        // 16 elements are two 16-byte units of a 64-element slab; odd slabs write theirs in the other
-                        // order, which keeps the eight lanes of a row on different banks
-                        const int R = w * 64 + row, odd = (c >> 2) & 1, un = (c & 3) * 2;
-                        const uint32_t rowa = dst + (c >> 2) * kChunkBytes + R * 128;
-                        const uint4 A = make_uint4(o[0], o[1], o[2], o[3]), B = make_uint4(o[4], o[5], o[6], o[7]);
-                        st_shared_v4(rowa + uint32_t(((un + odd) ^ (R & 7)) << 4), odd ? B : A);
-                        st_shared_v4(rowa + uint32_t(((un + 1 - odd) ^ (R & 7)) << 4), odd ? A : B);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const __half2 s2 = *reinterpret_cast<const __half2*>(&sc[y]);
+                            const uint32_t in[4] = {v[y].x, v[y].y, v[y].z, v[y].w};
+                            uint32_t o[8];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                uint32_t lo, hi;
+                                e4m3x4_to_f16x4(in[i], &lo, &hi);
+                                const __half2 a = __hmul2(*reinterpret_cast<__half2*>(&lo), s2), bb = __hmul2(*reinterpret_cast<__half2*>(&hi), s2);
+                                o[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+                                o[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&bb);
+                            }
+                            // 16 elements are two 16-byte units of a 64-element slab; odd slabs write theirs in the other
+                            // order, which keeps the eight lanes of a row on different banks
+                            const int R = w * 64 + (u4 + y) * (32 / kPer) + my_row, odd = (my_c >> 2) & 1, un = (my_c & 3) * 2;
+                            const uint32_t rowa = dst + (my_c >> 2) * kChunkBytes + R * 128;
+                            const uint4 A = make_uint4(o[0], o[1], o[2], o[3]), B = make_uint4(o[4], o[5], o[6], o[7]);
+                            st_shared_v4(rowa + uint32_t(((un + odd) ^ (R & 7)) << 4), odd ? B : A);
+                            st_shared_v4(rowa + uint32_t(((un + 1 - odd) ^ (R & 7)) << 4), odd ? A : B);
+                        }
+                        if (go) {      // (what they will overwrite has been read)
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) fetch(rows2, pitch2, u4 + y);
+                        }
                     }
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     fence_proxy_async_smem();

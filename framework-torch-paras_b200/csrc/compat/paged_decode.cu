@@ -40,7 +40,7 @@ template <bool E8, int HD> struct Ring {
     static constexpr int kSlab = kTileKeys * kRow;
     static constexpr int kTile = kSlabs * kSlab;
     static constexpr int kQ = 2 * kTile;                           // offset of the query rows
-    static constexpr int kExp = kQ + (HD / 64) * kRows * 128;      // offsets: K's 2^e (fp32), V's 2^e (fp16)
+    static constexpr int kExp = kQ + (HD / 64) * kRows * 128;      // K's exponent bytes, then V's
     static constexpr int kBytes = kExp + (E8 ? 1024 : 0);          // a multiple of 1024
     static constexpr int kStages = (208 * 1024) / kBytes < kMaxStages ? (208 * 1024) / kBytes : kMaxStages;
     static constexpr int kMerge = kStages * kBytes;
@@ -102,11 +102,6 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
     return r;
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 r;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
-    return r;
-}
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
     uint2 r;
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
@@ -145,7 +140,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < R::kStages; ++s) {
-            mbar_init(full(s), E8 ? 3 : 2);      // the producers
+            mbar_init(full(s), E8 ? 2 + 32 : 2);      // K's and V's producers, a lane each of the exponents'
             mbar_init(empty(s), kConsumers);
         }
         mbar_init(merge_bar, kConsumers);
@@ -193,20 +188,43 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tile = int(in - int64_t(hk) * nt);
             item0 = base0 + int64_t(hk) * nt;
         }
-        // lane i: page number of box i of the tile, -1 when it is not to be read; `prow`: the tile's first row in its page.
-        // (A number out of range is looked at where it is used: here that would wait for the load.)
-        int prow = 0;
-        auto page_of = [&]() -> int {
-            int entry = tile * p.npg + lane;
-            if (p.tpp > 1) {
-                entry = tile / p.tpp + lane;
-                prow = (tile - (entry - lane) * p.tpp) * kTileKeys;
-            }
-            if (lane >= p.npg || tile * kTileKeys + (lane << p.box_shift) >= kend) return -1;
-            return __ldg(p.table + int64_t(b) * p.table_stride + entry);
+        // Page numbers come 32 at a time, the next 32 on their way while these are used: with the ring full of loads a
+        // further one takes microseconds.  The walk over the batches runs ahead of the walk over the tiles.
+        auto entry_of = [&](int t) { return p.tpp > 1 ? t / p.tpp : t * p.npg; };    // of the tile's first box in the table
+        int lb = b, lhk = hk, lbatch = 0, lnb = 0;
+        auto load_batch = [&]() -> int {
+            const int e = lbatch * 32 + lane;
+            return lb < p.B && e < p.max_pages ? __ldg(p.table + int64_t(lb) * p.table_stride + e) : -1;
         };
+        auto next_batch = [&]() {
+            if (lb < p.B && ++lbatch == lnb) {
+                lbatch = 0;
+                if (++lhk == p.Hkv) {
+                    lhk = 0;
+                    int n = 0;
+                    while (n == 0 && ++lb < p.B) n = seq_tiles(p, paged_seq(p, lb));
+                    lnb = n > 0 ? (entry_of(n - 1) >> 5) + 1 : 0;
+                }
+            }
+        };
+        int batch = 0, cur = -1, nxt = -1;
+        if (ntiles > 0) {
+            lbatch = batch = entry_of(tile) >> 5;
+            lnb = (entry_of(nt - 1) >> 5) + 1;
+            cur = load_batch();
+            next_batch();
+            nxt = load_batch();
+        }
+        // lane i: page number of box i of the tile, -1 when it is not there or not to be read
+        auto page_of = [&]() -> int {
+            const int pg = __shfl_sync(0xffffffffu, cur, (entry_of(tile) & 31) + lane);
+            return lane < p.npg && tile * kTileKeys + (lane << p.box_shift) < kend && uint32_t(pg) < uint32_t(p.pages) ? pg : -1;
+        };
+        // on to the next tile, and to its batch of page numbers
         auto advance = [&]() {
+            bool item = false;
             if (++tile == nt) {
+                item = true;
                 tile = 0;
                 item0 += nt;
                 if (++hk == p.Hkv) {
@@ -215,115 +233,90 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     enter();
                 }
             }
-        };
-        int pg = ntiles > 0 ? page_of() : -1;
-        // lane l: exponent bytes of the tile's keys 4l .. 4l+3, 127 where there is no key
-        auto exps_of = [&](uint32_t& ek4, uint32_t& ev4) {
-            const int key = 4 * lane;
-            const int mine = __shfl_sync(0xffffffffu, pg, key >> p.box_shift);
-            const int off = prow + (key & ((1 << p.box_shift) - 1));
-            ek4 = ev4 = 0x7f7f7f7fu;
-            if (uint32_t(mine) < uint32_t(p.pages)) {
-                const uint8_t* k = p.ek + int64_t(mine) * p.eks[0] + int64_t(hk) * p.eks[1] + int64_t(off) * p.eks[2];
-                const uint8_t* v = p.ev + int64_t(mine) * p.evs[0] + int64_t(hk) * p.evs[1] + int64_t(off) * p.evs[2];
-                if (exp4) {
-                    ek4 = __ldg(reinterpret_cast<const uint32_t*>(k));
-                    ev4 = __ldg(reinterpret_cast<const uint32_t*>(v));
-                } else {
-                    ek4 = ev4 = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        ek4 |= uint32_t(k[e * p.eks[2]]) << (8 * e);
-                        ev4 |= uint32_t(v[e * p.evs[2]]) << (8 * e);
-                    }
-                }
+            const int now = entry_of(tile) >> 5;
+            if (item || now != batch) {
+                batch = now;
+                cur = nxt;
+                next_batch();
+                nxt = load_batch();
             }
         };
+        auto row_of = [&]() { return p.tpp > 1 ? (tile % p.tpp) * kTileKeys : 0; };     // the tile's first row in its page
         if (role == 2) {
-            // Exponents, two tiles ahead: a load of them is as slow as one of a whole tile.
-            uint32_t ek[2] = {0, 0}, ev[2] = {0, 0};
-            for (int i = 0; i < 2 && i < ntiles; ++i) {
-                exps_of(ek[i], ev[i]);
-                if (i + 1 < ntiles) {
-                    advance();
-                    pg = page_of();
-                }
-            }
+            // Exponent bytes: lane l brings those of the keys 4l .. 4l+3, as copies that the stage's barrier waits for; 127
+            // where no page is.
             for (int i = 0; i < ntiles; ++i) {
                 const int s = i % R::kStages;
                 if (!__all_sync(0xffffffffu, mbar_wait(empty(s), ((i / R::kStages) & 1) ^ 1u, abort_flag, 2))) break;
-                const uint32_t dst = base + s * R::kBytes;
-                // A row's exponent is within [-15, 7] (2^-15 the one subnormal in fp16); what lies past the sequence's
-                // end may be any byte, and is held within too: nothing infinite may meet the zeros there.
-                uint32_t kf[4], vh[4];
+                const uint32_t dst = base + s * R::kBytes + R::kExp + lane * 4;
+                const int key = 4 * lane, pg = page_of();
+                const int mine = __shfl_sync(0xffffffffu, pg, key >> p.box_shift);
+                const int off = row_of() + (key & ((1 << p.box_shift) - 1));
+                const int64_t page = max(mine, 0);
+                const uint8_t* k = p.ek + page * p.eks[0] + int64_t(hk) * p.eks[1] + int64_t(off) * p.eks[2];
+                const uint8_t* v = p.ev + page * p.evs[0] + int64_t(hk) * p.evs[1] + int64_t(off) * p.evs[2];
+                if (mine >= 0 && exp4) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(k) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 128), "l"(v) : "memory");
+                } else {
+                    uint32_t ek = 0x7f7f7f7fu, ev = 0x7f7f7f7fu;
+                    if (mine >= 0) {
+                        ek = ev = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    kf[e] = __float_as_uint(pow2f(max(kExpLo, min(kExpHi, int((ek[0] >> (8 * e)) & 0xffu) - 127))));
-                    const int x = max(kExpLo, min(kExpHi, int((ev[0] >> (8 * e)) & 0xffu) - 127));
-                    vh[e] = x >= -14 ? uint32_t(x + 15) << 10 : 0x200u;
+                        for (int e = 0; e < 4; ++e) {
+                            ek |= uint32_t(k[e * p.eks[2]]) << (8 * e);
+                            ev |= uint32_t(v[e * p.evs[2]]) << (8 * e);
+                        }
+                    }
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(ek) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + 128), "r"(ev) : "memory");
                 }
-                st_shared_v4(dst + R::kExp + lane * 16, make_uint4(kf[0], kf[1], kf[2], kf[3]));
-                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + R::kExp + 512 + lane * 8), "r"(vh[0] | (vh[1] << 16)),
-                             "r"(vh[2] | (vh[3] << 16)) : "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full(s));
-                ek[0] = ek[1];
-                ev[0] = ev[1];
-                if (i + 2 < ntiles) exps_of(ek[1], ev[1]);    // whose page numbers have come by now
-                if (i + 3 < ntiles) {
-                    advance();
-                    pg = page_of();
-                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(s)) : "memory");
+                if (i + 1 < ntiles) advance();
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
         bool first = true;
         for (int i = 0; role != 2 && i < ntiles; ++i) {
-            // this tile, and the way to the next one, whose page numbers are asked for
-            const int c_pg = pg, c_tile = tile, c_hk = hk, c_kend = kend, c_nt = nt, c_prow = prow;
-            const PagedSeq c_sq = sq;
-            const int64_t c_item0 = item0;
-            if (i + 1 < ntiles) {
-                advance();
-                pg = page_of();
-            }
+            const int pg = page_of(), row = row_of();
             const int s = i % R::kStages;
             if (!__all_sync(0xffffffffu, mbar_wait(empty(s), ((i / R::kStages) & 1) ^ 1u, abort_flag, 2))) break;
             const uint32_t dst = base + s * R::kBytes;
-            const bool last = c_tile + 1 == c_nt || i + 1 == ntiles;
+            const bool last = tile + 1 == nt || i + 1 == ntiles;
             // (pages outside the tensor read as zeros)
-            const bool has = uint32_t(c_pg) < uint32_t(p.pages);
-            const int page = has ? c_pg : p.pages;
+            const bool has = pg >= 0;
+            const int page = has ? pg : p.pages;
             if (role == 0) {
                 const uint32_t there = __ballot_sync(0xffffffffu, has);
                 if (lane == 0) {
                     TileMeta& m = meta[s];
-                    const int key0 = c_tile * kTileKeys;
+                    const int key0 = tile * kTileKeys;
                     // every row attends every key of the tile, and all of it is there
-                    const int all = p.causal ? min(c_kend, c_sq.pos0 + 1) : c_kend;
+                    const int all = p.causal ? min(kend, sq.pos0 + 1) : kend;
                     const bool full_tile = key0 + kTileKeys <= all && there == (1u << p.npg) - 1u;
                     int flags = (first ? 1 : 0) | (last ? 2 : 0) | (full_tile ? 0 : 8);
                     if (first || last) {
-                        const bool whole = c_item0 >= range.begin && c_item0 + c_nt <= range.end;
+                        const bool whole = item0 >= range.begin && item0 + nt <= range.end;
                         flags |= whole ? 0 : 4;
                         // the item the range begins with leaves its part in slot 2c, a later one that goes on in 2c+1
-                        const int slot = 2 * int(blockIdx.x) + (c_item0 > range.begin ? 1 : 0);
-                        m.row0 = c_sq.row0;
-                        m.nq = c_sq.nq;
-                        m.hk = c_hk;
+                        const int slot = 2 * int(blockIdx.x) + (item0 > range.begin ? 1 : 0);
+                        m.row0 = sq.row0;
+                        m.nq = sq.nq;
+                        m.hk = hk;
                         m.slot = slot;
-                        m.pos0 = c_sq.pos0;
-                        if (!whole && c_item0 >= range.begin) {
+                        m.pos0 = sq.pos0;
+                        if (!whole && item0 >= range.begin) {
                             join.first_slot = slot;
-                            join.last_cta = range.owner(c_item0 + c_nt - 1);
-                            join.row0 = c_sq.row0;
-                            join.nq = c_sq.nq;
-                            join.hk = c_hk;
+                            join.last_cta = range.owner(item0 + nt - 1);
+                            join.row0 = sq.row0;
+                            join.nq = sq.nq;
+                            join.hk = hk;
                         }
                     }
                     m.key0 = key0;
                     m.flags = flags;
                     m.pages = there;
-                    m.kend = c_kend;
+                    m.kend = kend;
                 }
             }
             const CUtensorMap* map = role ? &map_v : &map_k;
@@ -337,15 +330,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (lane == 0) {
 #pragma unroll
                     for (int c = 0; c < R::kSlabs; ++c)
-                        tma_load_4d(at + c * R::kSlab + (x << p.box_shift) * R::kRow, map, full(s), 64 * c, c_prow, c_hk, pgx);
+                        tma_load_4d(at + c * R::kSlab + (x << p.box_shift) * R::kRow, map, full(s), 64 * c, row, hk, pgx);
                 }
             }
             if (role == 0 && first && lane == 0) {
 #pragma unroll
                 for (int c = 0; c < HD / 64; ++c)
-                    tma_load_4d(dst + R::kQ + c * kRows * 128, &map_q, full(s), 64 * c, 0, c_hk, c_sq.row0);
+                    tma_load_4d(dst + R::kQ + c * kRows * 128, &map_q, full(s), 64 * c, 0, hk, sq.row0);
             }
             first = last;
+            if (i + 1 < ntiles) advance();
         }
         if (role == 0 && lane == 0) ws.join[blockIdx.x] = join;
     } else {
@@ -444,17 +438,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             // All fragments of a product are asked for before its first MMA, and V's before the softmax: with two warps
             // on a scheduler nothing else would hide the loads.
-            constexpr int kLd = R::kTile / 4096;     // ldmatrix.x4 of a warp's 16 rows
+            constexpr int kLd = R::kTile / 4096;     // ldmatrix.x4 of 16 rows
             uint32_t kf[kLd][4], vf[kLd][4];
 #pragma unroll
             for (int x = 0; x < kLd; ++x) {
-                // column n of an n-tile is any key: key n of 8, or, where four keys of V share a register, the one that
-                // leaves a thread with keys 4t, 4t+1 of the first n-tile and 4t+2, 4t+3 of the second
+                // column n of an n-tile is any key: key n of 8, or, where four keys of V share a register, the one
+                // that leaves a thread with keys 4t, 4t+1 of the first n-tile and 4t+2, 4t+3 of the second
                 const int row = krow + (E8 ? 4 * ((lane & 7) >> 1) + 2 * (x & 1) + (lane & 1) : (x & 1) * 8 + (lane & 7));
                 const int c = (x >> 1) * 4 + (lane >> 3);   // 16-byte unit of the row
                 ldsm4(kt + (E8 ? 0 : (c >> 3) * R::kSlab) + swz<R::kRow>(row, E8 ? c : c & 7), kf[x]);
             }
-            // ---- S = Q K^T for 16 keys: two n-tiles of 8 keys, even and odd steps summed apart ----
+            // ---- S = Q K^T: two n-tiles of 8 keys, even and odd steps summed apart ----
             float sc[2][4], sd[2][4];
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt)
@@ -477,22 +471,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
 #pragma unroll
             for (int x = 0; x < kLd; ++x) {
-                const int row = krow + ((lane >> 3) & 1) * 8 + (lane & 7), c = x * 2 + (lane >> 4);
+                const int row = krow + (lane & 15), c = x * 2 + (lane >> 4);
                 if constexpr (E8) ldsm2_t8(vt + swz<R::kRow>(row, c), vf[x]);
                 else ldsm4_t(vt + (c >> 3) * R::kSlab + swz<128>(row, c & 7), vf[x]);
             }
             // this thread's columns of n-tile nt: keys first + step * nt, + 1
             const int first = krow + (E8 ? 4 : 2) * t;
             constexpr int kStep = E8 ? 2 : 8;
-            uint4 ks = make_uint4(0, 0, 0, 0);
-            uint2 sv = make_uint2(0, 0);
-            if constexpr (E8) {
-                ks = lds128(kt + R::kExp + first * 4);
-                sv = lds64(kt + R::kExp + 512 + first * 2);
-            }
+            uint32_t ek = E8 ? lds32(kt + R::kExp + first) : 0u;
+            uint32_t ev = E8 ? lds32(kt + R::kExp + 128 + first) : 0u;
+            // 2^(byte - 127) of byte i (zero for a byte of 0, which no cache holds)
+            auto scale_of = [](uint32_t w, int i) { return __uint_as_float(((w >> (8 * i)) & 0xffu) << 23); };
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
-                const float k0 = E8 ? __uint_as_float(nt ? ks.z : ks.x) : 1.f, k1 = E8 ? __uint_as_float(nt ? ks.w : ks.y) : 1.f;
+                const float k0 = E8 ? scale_of(ek, 2 * nt) : 1.f, k1 = E8 ? scale_of(ek, 2 * nt + 1) : 1.f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     // x = score * scale * log2 e
@@ -504,7 +496,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const int kb = key0 + first;
             if (flags & 8) {
                 // (a page holds whole groups of 8 keys, so both of an n-tile's)
-                const uint32_t here0 = (md.pages >> (first >> p.box_shift)) & 1u, here1 = (md.pages >> ((first + kStep) >> p.box_shift)) & 1u;
+                const uint32_t here0 = (md.pages >> (first >> p.box_shift)) & 1u;
+                const uint32_t here1 = (md.pages >> ((first + kStep) >> p.box_shift)) & 1u;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -546,11 +539,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
             }
             // ---- O += P V ----
-            uint32_t pa[4];
-            pa[0] = pack16<kBfOps>(pr[0][0], pr[0][1]);
-            pa[1] = pack16<kBfOps>(pr[0][2], pr[0][3]);
-            pa[2] = pack16<kBfOps>(pr[1][0], pr[1][1]);
-            pa[3] = pack16<kBfOps>(pr[1][2], pr[1][3]);
             if (key0 + kTileKeys > kend) {
                 // past the end of the sequence the page holds anything, NaN too: 0 * NaN must not reach the sum
                 if constexpr (E8) {
@@ -560,6 +548,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     for (int x = 0; x < kLd; ++x)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) vf[x][e] &= keep;
+                    ev = (ev & keep) | (0x7f7f7f7fu & ~keep);      // (an infinite 2^e would make NaN of the zeros)
                 } else {
                     const uint32_t keep0 = (kb < kend ? 0xffffu : 0u) | (kb + 1 < kend ? 0xffff0000u : 0u);
                     const uint32_t keep1 = (kb + 8 < kend ? 0xffffu : 0u) | (kb + 9 < kend ? 0xffff0000u : 0u);
@@ -569,6 +558,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         for (int e = 0; e < 4; ++e) vf[x][e] &= (e & 1) ? keep1 : keep0;
                 }
             }
+            uint32_t pa[4];
+            pa[0] = pack16<kBfOps>(pr[0][0], pr[0][1]);
+            pa[1] = pack16<kBfOps>(pr[0][2], pr[0][3]);
+            pa[2] = pack16<kBfOps>(pr[1][0], pr[1][1]);
+            pa[3] = pack16<kBfOps>(pr[1][2], pr[1][3]);
+            // (2^-15 is subnormal in fp16, which the conversion knows)
+            const uint32_t sv01 = E8 ? pack16<false>(scale_of(ev, 0), scale_of(ev, 1)) : 0u;
+            const uint32_t sv23 = E8 ? pack16<false>(scale_of(ev, 2), scale_of(ev, 3)) : 0u;
 #pragma unroll
             for (int x = 0; x < kLd; ++x) {
                 if constexpr (!E8) {
@@ -579,7 +576,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     for (int e = 0; e < 4; ++e) {
                         uint32_t lo, hi;
                         e4m3x4_to_f16x4(vf[x][e], &lo, &hi);
-                        mma<false>(acc[4 * x + e], pa, hmul2(lo, sv.x), hmul2(hi, sv.y));
+                        mma<false>(acc[4 * x + e], pa, hmul2(lo, sv01), hmul2(hi, sv23));
                     }
                 }
             }

@@ -5,9 +5,9 @@
 //           power of two, so the only rounding is the one to e4m3.
 //   read    e4m3 * 2^e, exact in every row type.
 //
-// Sixteen lanes take a row, eight elements each at a time (16 bytes of a 16-bit row), the other half of the warp the
-// matching row of V: a 128-element head is one load a lane, the row's maximum four shuffles.  Which sequence a token
-// belongs to is found by the warp (warp_count_le) while the row's loads are in flight.
+// Sixteen lanes take a row, eight elements each (16 bytes of a 16-bit row), the other half of the warp the matching row
+// of V: a 128-element head is one load a lane, the row's maximum four shuffles.  Which sequence a token belongs to is
+// found by the warp (warp_count_le) while the row's loads are in flight.
 #include "paged_common.cuh"
 
 namespace pb {
@@ -25,13 +25,15 @@ struct KvParams {
 
 constexpr int kWarps = 4;
 
-// Position of token t in its sequence, and the page that holds it; false when the token has none.
+// Place of token t in the cache: sequence (-1: none), page and row in it; false when the token has no place there.
 template <bool WRITE>
-__device__ __forceinline__ bool locate(const KvParams& p, int t, int* page, int* off) {
+__device__ __forceinline__ bool locate(const KvParams& p, int t, int* page, int* off, int* seq) {
     const int b = warp_count_le(p.cu + 1, p.B, t);
+    *seq = -1;
     if (b >= p.B) return false;
     const int c0 = __ldg(p.cu + b);
     if (t < c0) return false;
+    *seq = b;
     int64_t pos = int64_t(t) - c0;
     if (WRITE) pos += int64_t(__ldg(p.kv_lens + b)) - (int64_t(__ldg(p.cu + b + 1)) - c0);
     if (pos < 0 || pos >= int64_t(p.max_pages) * p.page) return false;
@@ -56,127 +58,193 @@ __device__ __forceinline__ void load_row(const T* p, float (&f)[N]) {
     }
 }
 
-// N = 8 (rows whole and aligned in 16-byte units, 8 in an 8-bit cache) or 1 (anything).
-template <typename T, bool CACHE8, int N>
+// Eight elements of an 8-bit row and its 2^e as fp32.
+__device__ __forceinline__ void unpack8(uint2 w, float s, float (&f)[8]) {
+    const uint32_t ww[2] = {w.x, w.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t lo, hi;
+        e4m3x4_to_f16x4(ww[i], &lo, &hi);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        f[4 * i] = a.x * s;
+        f[4 * i + 1] = a.y * s;
+        f[4 * i + 2] = b.x * s;
+        f[4 * i + 3] = b.y * s;
+    }
+}
+__device__ __forceinline__ uint2 pack8(const float (&f)[8], float s) {
+    uint2 w;
+    w.x = pack_e4m3(f[0] * s, f[1] * s) | (pack_e4m3(f[2] * s, f[3] * s) << 16);
+    w.y = pack_e4m3(f[4] * s, f[5] * s) | (pack_e4m3(f[6] * s, f[7] * s) << 16);
+    return w;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8 / Vec16<T>::N; ++i) {
+        Vec16<T> w;
+#pragma unroll
+        for (int e = 0; e < Vec16<T>::N; ++e) w.v[e] = from_f32<T>(f[i * Vec16<T>::N + e]);
+        st16_stream(p + i * Vec16<T>::N, w);
+    }
+}
+
+// Which rows a half-warp looks after: `half` 0 is K, 1 is V; strides are selected one by one (a pointer into the
+// parameters would copy them to local memory).
+template <typename T>
+struct RowMap {
+    T* row;                  // the token's row of head 0
+    int64_t row_head;
+    char* cache;
+    int64_t cache_page, cache_head, cache_off;
+    uint8_t* exps;
+    int64_t exp_page, exp_head, exp_off;
+    __device__ __forceinline__ RowMap(const KvParams& p, int half, int t) {
+        row = reinterpret_cast<T*>(half ? p.v : p.k) + int64_t(t) * (half ? p.vs[0] : p.ks[0]);
+        row_head = half ? p.vs[1] : p.ks[1];
+        cache = half ? p.cv : p.ck;
+        cache_page = half ? p.cvs[0] : p.cks[0];
+        cache_head = half ? p.cvs[1] : p.cks[1];
+        cache_off = half ? p.cvs[2] : p.cks[2];
+        exps = half ? p.ev : p.ek;
+        exp_page = half ? p.evs[0] : p.eks[0];
+        exp_head = half ? p.evs[1] : p.eks[1];
+        exp_off = half ? p.evs[2] : p.eks[2];
+    }
+};
+
+// Rows of at most 128 elements, whole and aligned in 16-byte units (8 in an 8-bit cache): a lane holds its eight elements
+// of ROWS heads, all loaded before the token's place is looked up.
+template <typename T, bool CACHE8, int ROWS>
 __global__ void __launch_bounds__(kWarps * 32)
 paged_kv_write_kernel(const KvParams p) {
-    const int lane = threadIdx.x & 31, half = lane >> 4, l16 = lane & 15;
+    const int lane = threadIdx.x & 31, half = lane >> 4, d = (lane & 15) * 8;
     const int64_t unit = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-    if (unit >= int64_t(p.T) * p.Hkv) return;
-    const int t = int(unit / p.Hkv), h = int(unit - int64_t(t) * p.Hkv);
-    const T* row = half ? reinterpret_cast<const T*>(p.v) + int64_t(t) * p.vs[0] + int64_t(h) * p.vs[1]
-                        : reinterpret_cast<const T*>(p.k) + int64_t(t) * p.ks[0] + int64_t(h) * p.ks[1];
-    float f[N];
+    const int groups = (p.Hkv + ROWS - 1) / ROWS;
+    if (unit >= int64_t(p.T) * groups) return;
+    const int t = int(unit / groups), h0 = int(unit - int64_t(t) * groups) * ROWS;
+    const RowMap<T> m(p, half, t);
+    float f[ROWS][8];
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] = 0.f;
-    if (l16 * N < p.D) load_row<T, N>(row + l16 * N, f);
-    int page = 0, off = 0;
-    if (!locate<true>(p, t, &page, &off) || uint32_t(page) >= uint32_t(p.pages)) return;
-    // (strides are selected one by one: a pointer into the parameters would copy them to local memory)
-    const int64_t at = int64_t(page) * (half ? p.cvs[0] : p.cks[0]) + int64_t(h) * (half ? p.cvs[1] : p.cks[1]) +
-                       int64_t(off) * (half ? p.cvs[2] : p.cks[2]);
+    for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[r][e] = 0.f;
+        if (d < p.D && h0 + r < p.Hkv) load_row<T, 8>(m.row + int64_t(h0 + r) * m.row_head + d, f[r]);
+    }
+    int page = 0, off = 0, b = 0;
+    if (!locate<true>(p, t, &page, &off, &b) || uint32_t(page) >= uint32_t(p.pages)) return;
+    const int64_t at = int64_t(page) * m.cache_page + int64_t(off) * m.cache_off + d;
     if constexpr (CACHE8) {
-        float amax = 0.f;   // (fmaxf skips NaN)
+        float amax[ROWS];    // (fmaxf skips NaN)
 #pragma unroll
-        for (int e = 0; e < N; ++e) amax = fmaxf(amax, fabsf(f[e]));
-        for (int d = (l16 + 16) * N; d < p.D; d += 16 * N) {
-            float g[N];
-            load_row<T, N>(row + d, g);
+        for (int r = 0; r < ROWS; ++r) {
+            amax[r] = 0.f;
 #pragma unroll
-            for (int e = 0; e < N; ++e) amax = fmaxf(amax, fabsf(g[e]));
+            for (int e = 0; e < 8; ++e) amax[r] = fmaxf(amax[r], fabsf(f[r][e]));
         }
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const int ex = row_exponent(amax);
-        const float s = pow2f(-ex);
-        uint8_t* out = reinterpret_cast<uint8_t*>(half ? p.cv : p.ck) + at;
-        for (int d = l16 * N; d < p.D; d += 16 * N) {
-            if (d >= 16 * N) load_row<T, N>(row + d, f);
-            if constexpr (N == 8) {
-                uint2 w;
-                w.x = pack_e4m3(f[0] * s, f[1] * s) | (pack_e4m3(f[2] * s, f[3] * s) << 16);
-                w.y = pack_e4m3(f[4] * s, f[5] * s) | (pack_e4m3(f[6] * s, f[7] * s) << 16);
-                *reinterpret_cast<uint2*>(out + d) = w;
-            } else {
-                out[d] = uint8_t(pack_e4m3(f[0] * s, 0.f));
-            }
-        }
-        if (l16 == 0) {
-            (half ? p.ev : p.ek)[int64_t(page) * (half ? p.evs[0] : p.eks[0]) + int64_t(h) * (half ? p.evs[1] : p.eks[1]) +
-                                 int64_t(off) * (half ? p.evs[2] : p.eks[2])] = uint8_t(ex + 127);
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) amax[r] = fmaxf(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], o));
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const int h = h0 + r;
+            if (h >= p.Hkv) break;
+            const int ex = row_exponent(amax[r]);
+            if (d < p.D) *reinterpret_cast<uint2*>(m.cache + at + int64_t(h) * m.cache_head) = pack8(f[r], pow2f(-ex));
+            if (d == 0) m.exps[int64_t(page) * m.exp_page + int64_t(h) * m.exp_head + int64_t(off) * m.exp_off] = uint8_t(ex + 127);
         }
     } else {
-        T* out = reinterpret_cast<T*>(half ? p.cv : p.ck) + at;
-        for (int d = l16 * N; d < p.D; d += 16 * N) {
-            if (d >= 16 * N) load_row<T, N>(row + d, f);
-            if constexpr (N == 8) {
 #pragma unroll
-                for (int i = 0; i < 8 / Vec16<T>::N; ++i) {
-                    Vec16<T> w;
+        for (int r = 0; r < ROWS; ++r)
+            if (d < p.D && h0 + r < p.Hkv) store8(reinterpret_cast<T*>(m.cache) + at + int64_t(h0 + r) * m.cache_head, f[r]);
+    }
+}
+
+template <typename T, bool CACHE8, int ROWS>
+__global__ void __launch_bounds__(kWarps * 32)
+paged_kv_read_kernel(const KvParams p) {
+    const int lane = threadIdx.x & 31, half = lane >> 4, d = (lane & 15) * 8;
+    const int64_t unit = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const int groups = (p.Hkv + ROWS - 1) / ROWS;
+    if (unit >= int64_t(p.T) * groups) return;
+    const int t = int(unit / groups), h0 = int(unit - int64_t(t) * groups) * ROWS;
+    int page = 0, off = 0, b = 0;
+    const bool have = locate<false>(p, t, &page, &off, &b) && uint32_t(page) < uint32_t(p.pages);
+    if (b < 0 || d >= p.D) return;      // a row of no sequence
+    const RowMap<T> m(p, half, t);
+    const int64_t at = int64_t(page) * m.cache_page + int64_t(off) * m.cache_off + d;
+    const int64_t eat = int64_t(page) * m.exp_page + int64_t(off) * m.exp_off;
+    uint2 w[CACHE8 ? ROWS : 1];
+    float s[CACHE8 ? ROWS : 1], f[CACHE8 ? 1 : ROWS][8];
 #pragma unroll
-                    for (int e = 0; e < Vec16<T>::N; ++e) w.v[e] = from_f32<T>(f[i * Vec16<T>::N + e]);
-                    st16(out + d + i * Vec16<T>::N, w);
-                }
-            } else {
-                out[d] = from_f32<T>(f[0]);
+    for (int r = 0; r < ROWS; ++r) {
+        const bool live = have && h0 + r < p.Hkv;
+        if constexpr (CACHE8) {
+            w[r] = make_uint2(0, 0);
+            s[r] = 0.f;
+            if (live) {
+                w[r] = __ldcs(reinterpret_cast<const uint2*>(m.cache + at + int64_t(h0 + r) * m.cache_head));
+                s[r] = exp_byte(m.exps[eat + int64_t(h0 + r) * m.exp_head]);
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[r][e] = 0.f;
+            if (live) load_row<T, 8>(reinterpret_cast<const T*>(m.cache) + at + int64_t(h0 + r) * m.cache_head, f[r]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        if (h0 + r >= p.Hkv) break;
+        T* out = m.row + int64_t(h0 + r) * m.row_head + d;
+        if constexpr (CACHE8) {
+            unpack8(w[r], s[r], f[0]);
+            store8(out, f[0]);
+        } else {
+            store8(out, f[r]);
         }
     }
 }
 
-template <typename T, bool CACHE8, int N>
+// Any row length and alignment, an element at a time: 16 lanes a row as above.
+template <typename T, bool CACHE8, bool WRITE>
 __global__ void __launch_bounds__(kWarps * 32)
-paged_kv_read_kernel(const KvParams p) {
+paged_kv_any_kernel(const KvParams p) {
     const int lane = threadIdx.x & 31, half = lane >> 4, l16 = lane & 15;
     const int64_t unit = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
     if (unit >= int64_t(p.T) * p.Hkv) return;
     const int t = int(unit / p.Hkv), h = int(unit - int64_t(t) * p.Hkv);
-    int page = 0, off = 0;
-    const int b = warp_count_le(p.cu + 1, p.B, t);
-    if (b >= p.B || t < __ldg(p.cu + b)) return;   // a row of no sequence
-    const bool have = locate<false>(p, t, &page, &off) && uint32_t(page) < uint32_t(p.pages);
-    const int64_t at = have ? int64_t(page) * (half ? p.cvs[0] : p.cks[0]) + int64_t(h) * (half ? p.cvs[1] : p.cks[1]) +
-                                  int64_t(off) * (half ? p.cvs[2] : p.cks[2]) : 0;
-    T* row = half ? reinterpret_cast<T*>(p.v) + int64_t(t) * p.vs[0] + int64_t(h) * p.vs[1]
-                  : reinterpret_cast<T*>(p.k) + int64_t(t) * p.ks[0] + int64_t(h) * p.ks[1];
-    float s = 0.f;
-    if (CACHE8 && have) {
-        s = exp_byte((half ? p.ev : p.ek)[int64_t(page) * (half ? p.evs[0] : p.eks[0]) + int64_t(h) * (half ? p.evs[1] : p.eks[1]) +
-                                          int64_t(off) * (half ? p.evs[2] : p.eks[2])]);
-    }
-    for (int d = l16 * N; d < p.D; d += 16 * N) {
-        float f[N];
+    int page = 0, off = 0, b = 0;
+    const bool have = locate<WRITE>(p, t, &page, &off, &b) && uint32_t(page) < uint32_t(p.pages);
+    if (b < 0 || (WRITE && !have)) return;
+    const RowMap<T> m(p, half, t);
+    T* row = m.row + int64_t(h) * m.row_head;
+    const int64_t at = have ? int64_t(page) * m.cache_page + int64_t(h) * m.cache_head + int64_t(off) * m.cache_off : 0;
+    const int64_t eat = have && CACHE8 ? int64_t(page) * m.exp_page + int64_t(h) * m.exp_head + int64_t(off) * m.exp_off : 0;
+    if constexpr (WRITE) {
+        float s = 1.f;
+        if constexpr (CACHE8) {
+            float amax = 0.f;
+            for (int d = l16; d < p.D; d += 16) amax = fmaxf(amax, fabsf(to_f32<T>(row[d])));
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = 0.f;
-        if (have) {
-            if constexpr (CACHE8) {
-                const uint8_t* src = reinterpret_cast<const uint8_t*>(half ? p.cv : p.ck) + at + d;
-                if constexpr (N == 8) {
-                    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(src));
-                    const uint32_t ww[2] = {w.x, w.y};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 v = e4m3x2_to_f32((ww[i >> 1] >> (16 * (i & 1))) & 0xffffu);
-                        f[2 * i] = v.x * s;
-                        f[2 * i + 1] = v.y * s;
-                    }
-                } else {
-                    f[0] = e4m3_to_f32(*src) * s;
-                }
-            } else {
-                load_row<T, N>(reinterpret_cast<const T*>(half ? p.cv : p.ck) + at + d, f);
-            }
+            for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            const int ex = row_exponent(amax);
+            s = pow2f(-ex);
+            if (l16 == 0) m.exps[eat] = uint8_t(ex + 127);
         }
-        if constexpr (N == 8) {
-#pragma unroll
-            for (int i = 0; i < 8 / Vec16<T>::N; ++i) {
-                Vec16<T> w;
-#pragma unroll
-                for (int e = 0; e < Vec16<T>::N; ++e) w.v[e] = from_f32<T>(f[i * Vec16<T>::N + e]);
-                st16_stream(row + d + i * Vec16<T>::N, w);
+        for (int d = l16; d < p.D; d += 16) {
+            if constexpr (CACHE8) reinterpret_cast<uint8_t*>(m.cache)[at + d] = uint8_t(pack_e4m3(to_f32<T>(row[d]) * s, 0.f));
+            else reinterpret_cast<T*>(m.cache)[at + d] = row[d];
+        }
+    } else {
+        const float s = CACHE8 && have ? exp_byte(m.exps[eat]) : 0.f;
+        for (int d = l16; d < p.D; d += 16) {
+            float f = 0.f;
+            if (have) {
+                if constexpr (CACHE8) f = e4m3_to_f32(reinterpret_cast<const uint8_t*>(m.cache)[at + d]) * s;
+                else f = to_f32<T>(reinterpret_cast<const T*>(m.cache)[at + d]);
             }
-        } else {
-            row[d] = from_f32<T>(f[0]);
+            row[d] = from_f32<T>(f);
         }
     }
 }
@@ -188,16 +256,18 @@ bool multiples(const int64_t* s, int n, int64_t of) {
     return true;
 }
 
-template <bool WRITE, typename T>
-void launch(const KvParams& p, bool cache8, bool vec, int blocks, cudaStream_t s) {
-    auto go = [&](auto kernel) { kernel<<<blocks, kWarps * 32, 0, s>>>(p); };
-    if constexpr (WRITE) {
-        if (cache8) vec ? go(paged_kv_write_kernel<T, true, 8>) : go(paged_kv_write_kernel<T, true, 1>);
-        else vec ? go(paged_kv_write_kernel<T, false, 8>) : go(paged_kv_write_kernel<T, false, 1>);
-    } else {
-        if (cache8) vec ? go(paged_kv_read_kernel<T, true, 8>) : go(paged_kv_read_kernel<T, true, 1>);
-        else vec ? go(paged_kv_read_kernel<T, false, 8>) : go(paged_kv_read_kernel<T, false, 1>);
-    }
+template <bool WRITE, typename T, bool CACHE8>
+void launch(const KvParams& p, bool vec, int sms, cudaStream_t s) {
+    const int64_t rows = int64_t(p.T) * p.Hkv;
+    auto go = [&](auto kernel, int64_t warps) { kernel<<<unsigned((warps + kWarps - 1) / kWarps), kWarps * 32, 0, s>>>(p); };
+    if (!vec) return go(paged_kv_any_kernel<T, CACHE8, WRITE>, rows);
+    // Several heads a warp once there are rows enough for every warp slot of the GPU: the look-up of the token's place is
+    // shared and more loads are in flight; below that, a warp per row keeps the chain short.
+    constexpr int kMany = WRITE ? 4 : 8;
+    const bool many = p.Hkv > 1 && rows >= int64_t(sms) * 64 * 2;
+    const int64_t warps = many ? int64_t(p.T) * ((p.Hkv + kMany - 1) / kMany) : rows;
+    if constexpr (WRITE) many ? go(paged_kv_write_kernel<T, CACHE8, kMany>, warps) : go(paged_kv_write_kernel<T, CACHE8, 1>, warps);
+    else many ? go(paged_kv_read_kernel<T, CACHE8, kMany>, warps) : go(paged_kv_read_kernel<T, CACHE8, 1>, warps);
 }
 
 template <bool WRITE>
@@ -228,15 +298,18 @@ int run(const paras_paged_kv_args* args, const char* what) {
     const bool cache8 = c.cache_dtype == PARAS_E4M3;
     const int64_t unit = 16 / int64_t(dtype_size(a.dtype));         // elements in 16 bytes of a token row
     const int64_t cunit = cache8 ? 8 : unit;                         // elements in the cache's aligned unit
-    const bool vec = c.D % 8 == 0 && aligned(a.k, 16) && aligned(a.v, 16) && aligned(c.k, cache8 ? 8 : 16) &&
+    const bool vec = c.D % 8 == 0 && c.D <= 128 && aligned(a.k, 16) && aligned(a.v, 16) && aligned(c.k, cache8 ? 8 : 16) &&
                      aligned(c.v, cache8 ? 8 : 16) && multiples(a.k_strides, 2, unit) && multiples(a.v_strides, 2, unit) &&
                      multiples(c.k_strides, 3, cunit) && multiples(c.v_strides, 3, cunit);
-    const int blocks = int((int64_t(a.T) * c.Hkv + kWarps - 1) / kWarps);
     cudaStream_t s = pick_stream(g, a.stream);
+    auto go = [&](auto row) {
+        using T = decltype(row);
+        cache8 ? launch<WRITE, T, true>(p, vec, g->sm_count, s) : launch<WRITE, T, false>(p, vec, g->sm_count, s);
+    };
     switch (a.dtype) {
-        case PARAS_F32: launch<WRITE, float>(p, cache8, vec, blocks, s); break;
-        case PARAS_BF16: launch<WRITE, __nv_bfloat16>(p, cache8, vec, blocks, s); break;
-        default: launch<WRITE, __half>(p, cache8, vec, blocks, s); break;
+        case PARAS_F32: go(float()); break;
+        case PARAS_BF16: go(__nv_bfloat16()); break;
+        default: go(__half()); break;
     }
     PB_LAUNCH_CHECK(what);
     return PARAS_OK;

@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 
 #include "core/device_runtime.h"
+#include "ops/paged_ops.h"
 
 namespace paras {
 namespace {
@@ -182,47 +183,54 @@ Tensor rotate_half_backward(const Tensor& grad_out) {
 struct NormArgs {
     Tensor x, r, w;
     int64_t rows, H;
-    int dt, gpu;
+    int dt;
+    Place at;
 };
-NormArgs norm_args(const Tensor& x, const Tensor* residual, const Tensor& weight, const char* what) {
+NormArgs norm_args(const Tensor& x, const OptTensor& residual, const OptTensor& weight, int64_t stream, const char* what) {
     NormArgs a;
     TORCH_CHECK(x.dim() >= 1, "paras ", what, ": input must have rank >= 1");
     a.dt = checked_dtype(x, what);
-    a.gpu = Runtime::get().gpu_of(x);
+    a.at = place_of(x, stream);
     a.H = x.size(-1);
     a.rows = a.H > 0 ? x.numel() / a.H : 0;
-    if (residual) {
-        TORCH_CHECK(residual->sizes() == x.sizes(), "paras ", what, ": x and residual must have the same shape");
+    if (residual && residual->defined()) {
+        TORCH_CHECK(residual->sizes() == x.sizes(), "paras ", what, ": x and residual must have one shape");
         TORCH_CHECK(residual->scalar_type() == x.scalar_type() && residual->device() == x.device(),
-                    "paras ", what, ": x and residual must have the same dtype and device");
+                    "paras ", what, ": x and residual must have one type and device");
         a.r = residual->contiguous();
     }
-    TORCH_CHECK(weight.dim() == 1 && weight.size(0) == a.H, "paras ", what, ": weight size must match the last dimension");
-    TORCH_CHECK(weight.scalar_type() == x.scalar_type() && weight.device() == x.device(),
-                "paras ", what, ": weight dtype and device must equal the input's");
+    if (weight && weight->defined()) {
+        TORCH_CHECK(weight->dim() == 1 && weight->size(0) == a.H, "paras ", what, ": weight size must match the last dimension");
+        TORCH_CHECK(weight->scalar_type() == x.scalar_type() && weight->device() == x.device(),
+                    "paras ", what, ": weight and input must have one type and device");
+        a.w = weight->contiguous();
+    }
     a.x = x.contiguous();
-    a.w = weight.contiguous();
     return a;
 }
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-std::tuple<Tensor, Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+}  // namespace
+
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps,
+                                                bool want_rstd, int64_t stream) {
     PARAS_TRACE_OP("paras::add_rms_norm");
     c10::DeviceGuard guard(x.device());
-    const NormArgs a = norm_args(x, &residual, weight, "add_rms_norm");
-    Tensor y = at::empty_like(a.x), h = at::empty_like(a.x), rstd = at::empty({a.rows}, x.options().dtype(c10::kFloat));
-    PARAS_ABI(paras_b200_add_rmsnorm_fwd(a.gpu, a.x.data_ptr(), a.r.data_ptr(), a.w.data_ptr(), h.data_ptr(), y.data_ptr(),
-                                         a.rows ? rstd.data_ptr<float>() : nullptr, a.rows, a.H, eps, a.dt, nullptr));
+    const NormArgs a = norm_args(x, residual, weight, stream, "add_rms_norm");
+    Tensor y = at::empty_like(a.x), h = a.r.defined() ? at::empty_like(a.x) : x, rstd;
+    if (want_rstd) rstd = at::empty({a.rows}, x.options().dtype(c10::kFloat));
+    PARAS_ABI(paras_b200_add_rmsnorm_fwd(a.at.gpu, ptr(a.x), ptr(a.r), ptr(a.w), a.r.defined() ? ptr(h) : nullptr, ptr(y),
+                                         want_rstd && a.rows ? rstd.data_ptr<float>() : nullptr, a.rows, a.H, eps, a.dt, a.at.stream));
     return {y, h, rstd};
 }
 
-std::tuple<Tensor, Tensor> add_rms_norm_backward(const Tensor& grad_y, const std::optional<Tensor>& grad_h, const Tensor& h,
-                                                 const Tensor& weight, const Tensor& rstd) {
+std::tuple<Tensor, Tensor> add_rms_norm_backward(const Tensor& grad_y, const OptTensor& grad_h, const Tensor& h, const OptTensor& weight,
+                                                 const Tensor& rstd, int64_t stream) {
     PARAS_TRACE_OP("paras::add_rms_norm_backward");
     c10::DeviceGuard guard(h.device());
-    const NormArgs a = norm_args(h, &grad_y, weight, "add_rms_norm_backward");
-    const bool has_gh = grad_h.has_value() && grad_h->defined();
+    const NormArgs a = norm_args(h, grad_y, weight, stream, "add_rms_norm_backward");
     Tensor gh;
-    if (has_gh) {
+    if (grad_h && grad_h->defined()) {
         TORCH_CHECK(grad_h->sizes() == h.sizes() && grad_h->scalar_type() == h.scalar_type() && grad_h->device() == h.device(),
                     "paras add_rms_norm_backward: grad_h must match h");
         gh = grad_h->contiguous();
@@ -230,39 +238,27 @@ std::tuple<Tensor, Tensor> add_rms_norm_backward(const Tensor& grad_y, const std
     TORCH_CHECK(rstd.numel() == a.rows && rstd.scalar_type() == c10::kFloat && rstd.device() == h.device(),
                 "paras add_rms_norm_backward: rstd must be the fp32 tensor that the forward returned");
     Tensor rs = rstd.contiguous();
-    Tensor gx = at::empty_like(a.x), gw = at::empty_like(a.w);
-    PARAS_ABI(paras_b200_add_rmsnorm_bwd(a.gpu, a.r.data_ptr(), has_gh ? gh.data_ptr() : nullptr, a.x.data_ptr(), a.w.data_ptr(),
-                                         a.rows ? rs.data_ptr<float>() : nullptr, gx.data_ptr(), gw.data_ptr(), a.rows, a.H,
-                                         a.dt, nullptr));
+    Tensor gx = at::empty_like(a.x), gw = a.w.defined() ? at::empty_like(a.w) : Tensor();
+    PARAS_ABI(paras_b200_add_rmsnorm_bwd(a.at.gpu, ptr(a.r), ptr(gh), ptr(a.x), ptr(a.w), a.rows ? rs.data_ptr<float>() : nullptr,
+                                         ptr(gx), ptr(gw), a.rows, a.H, a.dt, a.at.stream));
     return {gx, gw};
 }
 
-std::tuple<Tensor, Tensor, Tensor> norm_quant(const Tensor& x, const Tensor* residual, const Tensor& weight, double eps,
-                                              int64_t group, const char* what) {
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm_quant(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps,
+                                                      int64_t group, int64_t stream) {
+    PARAS_TRACE_OP("paras::add_rms_norm_quant");
     c10::DeviceGuard guard(x.device());
-    TORCH_CHECK(group == 0 || group == 32 || group == 64 || group == 128, "paras ", what,
-                ": group must be 0 (one scale per row), 32, 64 or 128");
-    const NormArgs a = norm_args(x, residual, weight, what);
-    Tensor q = at::empty(x.sizes(), x.options().dtype(c10::kFloat8_e4m3fn)), h;
-    if (residual) h = at::empty_like(a.x);
+    TORCH_CHECK(group == 0 || group == 32 || group == 64 || group == 128,
+                "paras add_rms_norm_quant: group must be 0 (one scale per row), 32, 64 or 128");
+    const NormArgs a = norm_args(x, residual, weight, stream, "add_rms_norm_quant");
+    Tensor q = at::empty(x.sizes(), x.options().dtype(c10::kFloat8_e4m3fn)), h = a.r.defined() ? at::empty_like(a.x) : x;
     Tensor scales = at::empty({a.rows, group ? (a.H + group - 1) / group : 1}, x.options().dtype(c10::kFloat));
-    PARAS_ABI(paras_b200_add_rmsnorm_quant_fwd(a.gpu, a.x.data_ptr(), residual ? a.r.data_ptr() : nullptr, a.w.data_ptr(),
-                                               residual ? h.data_ptr() : nullptr, q.data_ptr(), scales.data_ptr<float>(), a.rows,
-                                               a.H, eps, int(group), a.dt, nullptr));
+    PARAS_ABI(paras_b200_add_rmsnorm_quant_fwd(a.at.gpu, ptr(a.x), ptr(a.r), ptr(a.w), a.r.defined() ? ptr(h) : nullptr, ptr(q),
+                                               static_cast<float*>(scales.data_ptr()), a.rows, a.H, eps, int(group), a.dt, a.at.stream));
     return {q, scales, h};
 }
 
-std::tuple<Tensor, Tensor, Tensor> add_rms_norm_quant(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps,
-                                                      int64_t group) {
-    PARAS_TRACE_OP("paras::add_rms_norm_quant");
-    return norm_quant(x, &residual, weight, eps, group, "add_rms_norm_quant");
-}
-
-std::tuple<Tensor, Tensor> rms_norm_quant(const Tensor& x, const Tensor& weight, double eps, int64_t group) {
-    PARAS_TRACE_OP("paras::rms_norm_quant");
-    auto [q, scales, h] = norm_quant(x, nullptr, weight, eps, group, "rms_norm_quant");
-    return {q, scales};
-}
+namespace {
 
 // ---- autograd for F.rms_norm on `paras` tensors -------------------------------------------
 // The reference's aten::rms_norm is a composition of at:: operators that autograd follows
@@ -338,8 +334,18 @@ TORCH_LIBRARY_IMPL(paras, PrivateUse1, m) {
     m.impl("swiglu_backward", &paras::swiglu_backward);
     m.impl("rotate_half", &paras::rotate_half);
     m.impl("rotate_half_backward", &paras::rotate_half_backward);
-    m.impl("add_rms_norm", &paras::add_rms_norm);
-    m.impl("add_rms_norm_backward", &paras::add_rms_norm_backward);
-    m.impl("add_rms_norm_quant", &paras::add_rms_norm_quant);
-    m.impl("rms_norm_quant", &paras::rms_norm_quant);
+    m.impl("add_rms_norm", [](const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, double eps) {
+        return paras::add_rms_norm(x, residual, weight, eps, true, 0);
+    });
+    m.impl("add_rms_norm_backward", [](const at::Tensor& grad_y, const std::optional<at::Tensor>& grad_h, const at::Tensor& h,
+                                       const at::Tensor& weight, const at::Tensor& rstd) {
+        return paras::add_rms_norm_backward(grad_y, grad_h, h, weight, rstd, 0);
+    });
+    m.impl("add_rms_norm_quant", [](const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, double eps, int64_t group) {
+        return paras::add_rms_norm_quant(x, residual, weight, eps, group, 0);
+    });
+    m.impl("rms_norm_quant", [](const at::Tensor& x, const at::Tensor& weight, double eps, int64_t group) {
+        auto [q, scales, h] = paras::add_rms_norm_quant(x, {}, weight, eps, group, 0);
+        return std::make_tuple(q, scales);
+    });
 }

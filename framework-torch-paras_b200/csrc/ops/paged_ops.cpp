@@ -8,15 +8,26 @@
 //
 // Caches are [pages, kv heads, page, D] of any strides with contiguous rows, in the tokens' dtype or float8_e4m3fn
 // with exponent bytes k_exp / v_exp [pages, kv heads, page].  Lengths and page numbers stay on the device.
+//
+// The functions take tensors of the `paras` device, and, for torch_paras.abi, torch.cuda ones with the stream to launch
+// on (the arguments are checked and packed in C++: in Python that costs more than the smallest kernels run).
+#include "ops/paged_ops.h"
+
 #include <torch/library.h>
 
 #include "core/device_runtime.h"
 
 namespace paras {
+
+Place place_of(const at::Tensor& t, int64_t stream) {
+    if (t.device().type() == kDevice) return {Runtime::get().gpu_of(t), nullptr};
+    TORCH_CHECK(t.is_cuda(), "paras: expected a paras or CUDA tensor, got one on ", t.device());
+    return {int(t.get_device()), reinterpret_cast<void*>(stream)};
+}
+
 namespace {
 
 using at::Tensor;
-using OptTensor = std::optional<Tensor>;
 
 void fill_cache(paras_paged_cache& c, const Tensor& k, const Tensor& v, const Tensor& table, const OptTensor& ke,
                 const OptTensor& ve, const Tensor& rows, const char* what) {
@@ -78,11 +89,13 @@ Tensor rows_of(const Tensor& t, int64_t heads, int64_t D, const char* what, cons
     return (D <= 1 || t.stride(2) == 1) ? t : t.contiguous();
 }
 
+}  // namespace
+
 void paged_kv_write(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
-                    const Tensor& kv_lens, const Tensor& cu_q, const OptTensor& k_exp, const OptTensor& v_exp) {
+                    const Tensor& kv_lens, const Tensor& cu_q, const OptTensor& k_exp, const OptTensor& v_exp, int64_t stream) {
     PARAS_TRACE_OP("paras::paged_kv_write");
     const char* what = "paged_kv_write";
-    const int gpu = Runtime::get().gpu_of(k);
+    const Place at = place_of(k, stream);
     c10::DeviceGuard guard(k.device());
     paras_paged_kv_args a{};
     fill_cache(a.cache, k_cache, v_cache, page_table, k_exp, v_exp, k, what);
@@ -99,31 +112,48 @@ void paged_kv_write(const Tensor& k, const Tensor& v, const Tensor& k_cache, con
     a.cu = index_array(cu_q, int64_t(a.cache.B) + 1, k, what, "cu_q");
     a.T = int32_t(k.size(0));
     a.dtype = dtype_code(k.scalar_type());
-    a.gpu = gpu;
+    a.gpu = at.gpu;
+    a.stream = at.stream;
     PARAS_ABI(paras_b200_paged_kv_write(&a));
 }
 
 std::tuple<Tensor, Tensor> paged_kv_read(const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
                                          const Tensor& cu_kv, int64_t total, std::optional<c10::ScalarType> dtype,
-                                         const OptTensor& k_exp, const OptTensor& v_exp) {
+                                         const OptTensor& k_exp, const OptTensor& v_exp, const OptTensor& out_k,
+                                         const OptTensor& out_v, int64_t stream) {
     PARAS_TRACE_OP("paras::paged_kv_read");
     const char* what = "paged_kv_read";
-    const int gpu = Runtime::get().gpu_of(k_cache);
+    const Place at = place_of(k_cache, stream);
     c10::DeviceGuard guard(k_cache.device());
     TORCH_CHECK(total >= 0 && total <= INT32_MAX, "paras paged_kv_read: total must be within 0 .. 2^31 - 1");
     TORCH_CHECK(k_cache.dim() == 4, "paras paged_kv_read: caches must be [pages, kv heads, page, D]");
     const auto to = dtype.value_or(k_cache.scalar_type() == c10::kFloat8_e4m3fn ? c10::kBFloat16 : k_cache.scalar_type());
     TORCH_CHECK(dtype_code(to) >= 0, "paras paged_kv_read: unsupported dtype ", to);
-    Tensor k = at::empty({total, k_cache.size(1), k_cache.size(3)}, k_cache.options().dtype(to)), v = at::empty_like(k);
+    Tensor k, v;
+    if (out_k && out_v) {
+        k = *out_k;
+        v = *out_v;
+        TORCH_CHECK(rows_of(k, k_cache.size(1), k_cache.size(3), what, "k").is_same(k) &&
+                        rows_of(v, k_cache.size(1), k_cache.size(3), what, "v").is_same(v) && k.size(0) == total && v.size(0) == total &&
+                        v.scalar_type() == k.scalar_type() && k.device() == k_cache.device() && v.device() == k.device(),
+                    "paras paged_kv_read: the two outputs must have one type, the cache's device, contiguous rows and `total` of them");
+    } else {
+        k = at::empty({total, k_cache.size(1), k_cache.size(3)}, k_cache.options().dtype(to));
+        v = at::empty_like(k);
+    }
     paras_paged_kv_args a{};
     fill_cache(a.cache, k_cache, v_cache, page_table, k_exp, v_exp, k, what);
     a.k = k.data_ptr();
     a.v = v.data_ptr();
-    for (int i = 0; i < 2; ++i) a.k_strides[i] = a.v_strides[i] = k.stride(i);
+    for (int i = 0; i < 2; ++i) {
+        a.k_strides[i] = k.stride(i);
+        a.v_strides[i] = v.stride(i);
+    }
     a.cu = index_array(cu_kv, int64_t(a.cache.B) + 1, k, what, "cu_kv");
     a.T = int32_t(total);
-    a.dtype = dtype_code(to);
-    a.gpu = gpu;
+    a.dtype = dtype_code(k.scalar_type());
+    a.gpu = at.gpu;
+    a.stream = at.stream;
     PARAS_ABI(paras_b200_paged_kv_read(&a));
     return {k, v};
 }
@@ -131,20 +161,28 @@ std::tuple<Tensor, Tensor> paged_kv_read(const Tensor& k_cache, const Tensor& v_
 std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
                                            const Tensor& page_table, const Tensor& kv_lens, const Tensor& cu_q, int64_t max_q,
                                            bool is_causal, std::optional<double> scale, const OptTensor& k_exp,
-                                           const OptTensor& v_exp) {
+                                           const OptTensor& v_exp, const OptTensor& out_given, bool want_lse,
+                                           const OptTensor& workspace, int64_t stream, size_t* workspace_bytes) {
     PARAS_TRACE_OP("paras::paged_attention");
     const char* what = "paged_attention";
-    const int gpu = Runtime::get().gpu_of(q);
+    const Place at = place_of(q, stream);
     c10::DeviceGuard guard(q.device());
     paras_paged_attn_args a{};
     fill_cache(a.cache, k_cache, v_cache, page_table, k_exp, v_exp, q, what);
-    Tensor qr = rows_of(q, -1, a.cache.D, what, "q");
+    Tensor qr = rows_of(q, -1, a.cache.D, what, "q"), out, lse;
     TORCH_CHECK(max_q >= 0, "paras paged_attention: max_q is negative");
-    Tensor out = at::empty(q.sizes(), q.options());
-    Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(c10::kFloat));
+    if (out_given && out_given->defined()) {
+        out = *out_given;
+        TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() &&
+                        (a.cache.D <= 1 || out.stride(2) == 1),
+                    "paras paged_attention: out must have q's shape, type and device and contiguous rows");
+    } else {
+        out = workspace_bytes ? q : at::empty(q.sizes(), q.options());
+    }
+    if (want_lse) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(c10::kFloat));
     a.q = qr.data_ptr();
     a.out = out.data_ptr();
-    a.lse = static_cast<float*>(lse.data_ptr());
+    a.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
     for (int i = 0; i < 2; ++i) {
         a.q_strides[i] = qr.stride(i);
         a.o_strides[i] = out.stride(i);
@@ -156,13 +194,23 @@ std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor& k_cach
     a.max_q = int32_t(std::min<int64_t>(max_q, q.size(0)));
     a.dtype = dtype_code(q.scalar_type());
     a.causal = is_causal;
-    a.gpu = gpu;
+    a.gpu = at.gpu;
+    a.stream = at.stream;
     a.scale = scale ? *scale : 1.0 / std::sqrt(double(a.cache.D));
-    PARAS_ABI(paras_b200_paged_attn(&a));
+    if (workspace && workspace->defined()) {
+        TORCH_CHECK(workspace->device() == q.device() && workspace->is_contiguous(),
+                    "paras paged_attention: workspace must be contiguous and on q's device");
+        a.workspace = workspace->data_ptr();
+        a.workspace_bytes = workspace->nbytes();
+    }
+    if (workspace_bytes) {
+        PARAS_ABI(paras_b200_paged_attn_workspace_bytes(&a, workspace_bytes));
+    } else {
+        PARAS_ABI(paras_b200_paged_attn(&a));
+    }
     return {out, lse};
 }
 
-}  // namespace
 }  // namespace paras
 
 TORCH_LIBRARY_FRAGMENT(paras, m) {
@@ -175,7 +223,20 @@ TORCH_LIBRARY_FRAGMENT(paras, m) {
 }
 
 TORCH_LIBRARY_IMPL(paras, PrivateUse1, m) {
-    m.impl("paged_kv_write", &paras::paged_kv_write);
-    m.impl("paged_kv_read", &paras::paged_kv_read);
-    m.impl("paged_attention", &paras::paged_attention);
+    using paras::OptTensor;
+    m.impl("paged_kv_write", [](const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                const at::Tensor& page_table, const at::Tensor& kv_lens, const at::Tensor& cu_q, const OptTensor& k_exp,
+                                const OptTensor& v_exp) {
+        paras::paged_kv_write(k, v, k_cache, v_cache, page_table, kv_lens, cu_q, k_exp, v_exp, 0);
+    });
+    m.impl("paged_kv_read", [](const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& page_table, const at::Tensor& cu_kv,
+                               int64_t total, std::optional<c10::ScalarType> dtype, const OptTensor& k_exp, const OptTensor& v_exp) {
+        return paras::paged_kv_read(k_cache, v_cache, page_table, cu_kv, total, dtype, k_exp, v_exp, {}, {}, 0);
+    });
+    m.impl("paged_attention", [](const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& page_table,
+                                 const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t max_q, bool is_causal, std::optional<double> scale,
+                                 const OptTensor& k_exp, const OptTensor& v_exp) {
+        return paras::paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, is_causal, scale, k_exp, v_exp, {}, true, {},
+                                      0, nullptr);
+    });
 }

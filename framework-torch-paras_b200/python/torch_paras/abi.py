@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-import struct
 
 import torch
 
@@ -216,7 +215,7 @@ def _stream_of(t: torch.Tensor, stream) -> int:
 def _gpu_of(t: torch.Tensor) -> int:
     if not t.is_cuda:
         raise RuntimeError("paras abi: expected a CUDA tensor (raw device memory)")
-    return t.device.index if t.device.index is not None else torch.cuda.current_device()
+    return t.get_device()
 
 
 def sdpa_args(q, k, v, out, *, causal=False, scale=None, mask=None, lse=None, flags=0,
@@ -568,109 +567,35 @@ def rotate_half(x, *, backward=False, stream=None):
     return out
 
 
-# ---- paged key / value cache -----------------------------------------------------------------
-# The argument blocks are packed in one go: filling some fifty ctypes fields one by one costs several microseconds,
-# more than the smallest of these kernels runs.  The layouts are those of PagedCache, PagedKvArgs and PagedAttnArgs.
-_PACK_CACHE = "4Q12qQq8i"
-_PACK_KV = struct.Struct("=" + _PACK_CACHE + "2Q4q2Q4iQ")
-_PACK_ATTN = struct.Struct("=" + _PACK_CACHE + "3Q4q2Q6id2QQ")
-_ZERO6 = (0,) * 6
+# ---- paged key / value cache, residual addition and RMSNorm --------------------------------------
+# These calls check and pack their arguments in C++ (`_C`, the same functions that the `paras` operators run): filling
+# some fifty ctypes fields and comparing shapes in Python costs 10 to 20 microseconds, more than the smallest of the
+# kernels runs.  They therefore always run the library that `_C` is linked to.
+def _c():
+    global _C
+    if _C is None:
+        from . import _C as module
+        _C = module
+    return _C
 
 
-def _index_array(t, dev, n, what):
-    if t.dtype != torch.int32 or t.shape != (n,) or t.device != dev or not t.is_contiguous():
-        raise RuntimeError(f"paras abi: {what} must be a contiguous int32 vector of {n} entries on the tensors' device")
-    return t.data_ptr()
-
-
-def _paged_cache(k_cache, v_cache, page_table, k_exp, v_exp, dev):
-    """The values of a ``paras_paged_cache``, after the checks that the C side cannot make (shapes, devices, types)."""
-    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
-    dtype = k_cache.dtype
-    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != dtype:
-        raise RuntimeError("paras abi: caches must be two [pages, kv heads, page, D] tensors of one type")
-    if shape[3] > 1 and (ks[3] != 1 or vs[3] != 1):
-        raise RuntimeError("paras abi: cache rows must be contiguous")
-    ts = page_table.shape
-    if page_table.dtype != torch.int32 or len(ts) != 2 or (ts[1] > 1 and page_table.stride(1) != 1):
-        raise RuntimeError("paras abi: page_table must be int32 [sequences, pages] with contiguous rows")
-    if k_cache.device != dev or v_cache.device != dev or page_table.device != dev:
-        raise RuntimeError("paras abi: tensors are on different devices")
-    if dtype == torch.float8_e4m3fn:
-        for e in (k_exp, v_exp):
-            if e is None or e.shape != shape[:3] or e.element_size() != 1 or e.device != dev:
-                raise RuntimeError("paras abi: an 8-bit cache needs k_exp and v_exp, bytes of shape [pages, kv heads, page]")
-        code, kp, vp, es = E4M3, k_exp.data_ptr(), v_exp.data_ptr(), k_exp.stride() + v_exp.stride()
-    elif k_exp is not None or v_exp is not None:
-        raise RuntimeError("paras abi: k_exp and v_exp belong to an 8-bit cache")
-    else:
-        code, kp, vp, es = dtype_code(k_cache), 0, 0, _ZERO6
-    return (k_cache.data_ptr(), v_cache.data_ptr(), kp, vp, *ks[:3], *vs[:3], *es, page_table.data_ptr(), page_table.stride(0),
-            code, shape[0], shape[2], shape[1], shape[3], ts[0], ts[1], 0)
-
-
-def _token_rows(t, shape, what):
-    """Strides of {token, head} rows [tokens, heads, D]; `shape` is the cache's."""
-    s, st = t.shape, t.stride()
-    if len(s) != 3 or (what != "q" and s[1] != shape[1]) or s[2] != shape[3] or (s[2] > 1 and st[2] != 1):
-        raise RuntimeError(f"paras abi: {what} must be [tokens, heads, D] with contiguous rows that fit the cache")
-    return st[0], st[1]
+_C = None
 
 
 def paged_kv_write(k, v, k_cache, v_cache, page_table, kv_lens, cu_q, *, k_exp=None, v_exp=None, stream=None):
     """Writes new tokens' rows k, v [tokens, kv heads, D] into the paged cache in place (rounded to e4m3 with one
     exponent byte per row when the cache is ``float8_e4m3fn``): row ``cu_q[b] + i`` is position
     ``kv_lens[b] - (cu_q[b+1] - cu_q[b]) + i`` of sequence b."""
-    dev, shape = k.device, k_cache.shape
-    cache = _paged_cache(k_cache, v_cache, page_table, k_exp, v_exp, dev)
-    ks, vs = _token_rows(k, shape, "k"), _token_rows(v, shape, "v")
-    if v.dtype != k.dtype or v.shape != k.shape or v.device != dev:
-        raise RuntimeError("paras abi: k and v must have one type, shape and device")
-    n = page_table.shape[0]
-    check(lib().paras_b200_paged_kv_write(_PACK_KV.pack(
-        *cache, k.data_ptr(), v.data_ptr(), *ks, *vs, _index_array(kv_lens, dev, n, "kv_lens"),
-        _index_array(cu_q, dev, n + 1, "cu_q"), k.shape[0], dtype_code(k), _gpu_of(k), 0, _stream_of(k, stream))))
+    (_C or _c()).paged_kv_write(k, v, k_cache, v_cache, page_table, kv_lens, cu_q, k_exp, v_exp, _stream_of(k, stream))
 
 
 def paged_kv_read(k_cache, v_cache, page_table, cu_kv, total, *, dtype=None, k_exp=None, v_exp=None, out=None, stream=None):
     """(k, v) [total, kv heads, D]: the first ``cu_kv[b+1] - cu_kv[b]`` positions of every sequence, one after the
     other.  ``dtype`` is the result's type (the cache's, or bfloat16 for an 8-bit one, when omitted); rows behind the
-    last sequence keep what ``out`` held."""
-    dev, shape = k_cache.device, k_cache.shape
-    cache = _paged_cache(k_cache, v_cache, page_table, k_exp, v_exp, dev)
-    if out is None:
-        if dtype is None:
-            dtype = torch.bfloat16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
-        out = torch.empty((2, total, shape[1], shape[3]), dtype=dtype, device=dev).unbind(0)
-    k, v = out
-    ks, vs = _token_rows(k, shape, "k"), _token_rows(v, shape, "v")
-    if v.dtype != k.dtype or v.shape != k.shape or k.shape[0] != total or v.device != dev or k.device != dev:
-        raise RuntimeError("paras abi: the two outputs must have one type, the cache's device and `total` rows")
-    check(lib().paras_b200_paged_kv_read(_PACK_KV.pack(
-        *cache, k.data_ptr(), v.data_ptr(), *ks, *vs, 0, _index_array(cu_kv, dev, page_table.shape[0] + 1, "cu_kv"), total,
-        dtype_code(k), _gpu_of(k), 0, _stream_of(k, stream))))
-    return k, v
-
-
-def paged_attn_args(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, out, *, causal=True, scale=None, k_exp=None,
-                    v_exp=None, lse=None, workspace=None, stream=None) -> bytes:
-    """A ``paras_paged_attn_args`` as bytes."""
-    dev, shape = q.device, k_cache.shape
-    cache = _paged_cache(k_cache, v_cache, page_table, k_exp, v_exp, dev)
-    qs = _token_rows(q, shape, "q")
-    if out is q:
-        os_ = qs
-    else:
-        os_ = _token_rows(out, shape, "q")
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
-            raise RuntimeError("paras abi: out must have q's shape, type and device and contiguous rows")
-    n = page_table.shape[0]
-    return _PACK_ATTN.pack(
-        *cache, q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else 0, *qs, *os_,
-        _index_array(kv_lens, dev, n, "kv_lens"), _index_array(cu_q, dev, n + 1, "cu_q"), q.shape[0], q.shape[1], max_q,
-        dtype_code(q), 1 if causal else 0, _gpu_of(q), shape[3] ** -0.5 if scale is None else scale,
-        workspace.data_ptr() if workspace is not None else 0,
-        workspace.numel() * workspace.element_size() if workspace is not None else 0, _stream_of(q, stream))
+    last sequence keep what ``out`` = (k, v) held."""
+    k, v = out if out is not None else (None, None)
+    return (_C or _c()).paged_kv_read(k_cache, v_cache, page_table, cu_kv, total, dtype, k_exp, v_exp, k, v,
+                                      _stream_of(k_cache, stream))
 
 
 def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, *, causal=True, scale=None, k_exp=None,
@@ -678,81 +603,34 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, *, ca
     """Attention of the new tokens q [tokens, heads, D] over a paged cache that holds their keys and values already.
     Row ``cu_q[b] + i`` is the query at position ``kv_lens[b] - (cu_q[b+1] - cu_q[b]) + i`` of sequence b and attends
     the positions up to its own (all of them with ``causal=False``).  ``max_q`` bounds a sequence's new tokens."""
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    check(lib().paras_b200_paged_attn(paged_attn_args(
-        q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, out, causal=causal, scale=scale, k_exp=k_exp, v_exp=v_exp,
-        lse=lse, workspace=workspace, stream=stream)))
-    return (out, lse) if return_lse else out
+    res = (_C or _c()).paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, causal, scale, k_exp, v_exp, out,
+                                       return_lse, workspace, _stream_of(q, stream))
+    return res if return_lse else res[0]
 
 
 def paged_attn_workspace_bytes(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, *, causal=True, k_exp=None,
                                v_exp=None) -> int:
-    n = C.c_size_t(0)
-    check(lib().paras_b200_paged_attn_workspace_bytes(
-        paged_attn_args(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, q, causal=causal, k_exp=k_exp, v_exp=v_exp),
-        C.byref(n)))
-    return int(n.value)
+    return _c().paged_attn_workspace_bytes(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, causal, k_exp, v_exp)
 
 
 def paged_attn_last_kernel() -> str:
     return lib().paras_b200_paged_attn_last_kernel().decode()
 
 
-# ---- residual addition and RMSNorm -------------------------------------------------------------
-def _norm_operands(x, residual, weight):
-    h = x.shape[-1]
-    dtype, dev = x.dtype, x.device
-    for t in (residual, weight):
-        if t is not None and (t.dtype != dtype or t.device != dev or not t.is_contiguous()):
-            raise RuntimeError("paras abi: norm operands must be contiguous, of one type and on one device")
-    if not x.is_contiguous() or (residual is not None and residual.shape != x.shape) or \
-            (weight is not None and weight.shape != (h,)):
-        raise RuntimeError("paras abi: x and residual must be contiguous and of one shape, weight [its last dimension]")
-    return h, x.numel() // h if h else 0
-
-
 def add_rmsnorm_fwd(x, residual, weight, eps=1e-6, *, return_rstd=False, stream=None):
     """(y, h[, rstd]): h = x + residual in x's type, y = RMSNorm(h) * weight.  ``residual=None`` normalises x itself
     (h is x); ``weight=None`` stands for ones."""
-    width, rows = _norm_operands(x, residual, weight)
-    y = torch.empty_like(x)
-    h = torch.empty_like(x) if residual is not None else x
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if return_rstd else None
-    check(lib().paras_b200_add_rmsnorm_fwd(
-        _gpu_of(x), x.data_ptr(), residual.data_ptr() if residual is not None else None,
-        weight.data_ptr() if weight is not None else None, h.data_ptr(), y.data_ptr(),
-        rstd.data_ptr() if return_rstd and rows else None, rows, width, float(eps), dtype_code(x), _stream_of(x, stream)))
-    return (y, h, rstd) if return_rstd else (y, h)
+    res = (_C or _c()).add_rms_norm(x, residual, weight, eps, return_rstd, _stream_of(x, stream))
+    return res if return_rstd else res[:2]
 
 
 def add_rmsnorm_quant(x, residual, weight, eps=1e-6, *, group=0, stream=None):
     """(q, scales, h): the same norm in 8 bits, y ~ q * scales, q ``float8_e4m3fn``; one fp32 scale per row
     (``group=0``: scales [rows, 1]) or per ``group`` = 32, 64 or 128 columns (scales [rows, ceil(width / group)])."""
-    width, rows = _norm_operands(x, residual, weight)
-    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
-    h = torch.empty_like(x) if residual is not None else x
-    scales = torch.empty((rows, -(-width // group) if group > 0 else 1), dtype=torch.float32, device=x.device)
-    check(lib().paras_b200_add_rmsnorm_quant_fwd(
-        _gpu_of(x), x.data_ptr(), residual.data_ptr() if residual is not None else None,
-        weight.data_ptr() if weight is not None else None, h.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, width,
-        float(eps), group, dtype_code(x), _stream_of(x, stream)))
-    return q, scales, h
+    return (_C or _c()).add_rms_norm_quant(x, residual, weight, eps, group, _stream_of(x, stream))
 
 
 def add_rmsnorm_bwd(grad_y, grad_h, h, weight, rstd, *, stream=None):
     """(grad_x, grad_weight) of ``add_rmsnorm_fwd`` from the gradients that reach y and h (``grad_h=None``: none);
     grad_x is the gradient of x and of residual alike."""
-    width, rows = _norm_operands(h, grad_y, weight)
-    if grad_h is not None:
-        _norm_operands(h, grad_h, None)
-    if rstd.dtype != torch.float32 or rstd.numel() != rows or not rstd.is_contiguous() or rstd.device != h.device:
-        raise RuntimeError("paras abi: rstd must be the fp32 [rows] that the forward returned")
-    gx = torch.empty_like(h)
-    gw = torch.empty_like(weight) if weight is not None else None
-    check(lib().paras_b200_add_rmsnorm_bwd(
-        _gpu_of(h), grad_y.data_ptr(), grad_h.data_ptr() if grad_h is not None else None, h.data_ptr(),
-        weight.data_ptr() if weight is not None else None, rstd.data_ptr(), gx.data_ptr(),
-        gw.data_ptr() if gw is not None else None, rows, width, dtype_code(h), _stream_of(h, stream)))
-    return gx, gw
+    return (_C or _c()).add_rms_norm_backward(grad_y, grad_h, h, weight, rstd, _stream_of(h, stream))

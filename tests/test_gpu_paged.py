@@ -453,7 +453,7 @@ def test_refusals_on_the_device():
         abi.paged_attention(q.half(), *c.cache, c.table, c.kv_lens, cu, 1)
     with pytest.raises(RuntimeError, match="int32"):
         abi.paged_attention(q, *c.cache, c.table, c.kv_lens.long(), cu, 1)
-    with pytest.raises(RuntimeError, match="3 entries|2 entries"):
+    with pytest.raises(RuntimeError, match="2 entries"):
         abi.paged_attention(q, *c.cache, c.table, c.kv_lens, torch.zeros(3, dtype=torch.int32, device=DEV), 1)
     with pytest.raises(RuntimeError, match="scale is not finite"):
         abi.paged_attention(q, *c.cache, c.table, c.kv_lens, cu, 1, scale=float("nan"))

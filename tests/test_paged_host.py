@@ -79,20 +79,6 @@ def test_no_gpu_is_said_so():
         torch_paras.nn.add_rms_norm(torch.zeros(2, 8, device="paras:0"), torch.zeros(2, 8, device="paras:0"), torch.zeros(8, device="paras:0"))
 
 
-def test_packed_arguments_are_the_structs():
-    assert abi._PACK_KV.size == ctypes.sizeof(abi.PagedKvArgs) and abi._PACK_ATTN.size == ctypes.sizeof(abi.PagedAttnArgs)
-    for pack, cls in ((abi._PACK_KV, abi.PagedKvArgs), (abi._PACK_ATTN, abi.PagedAttnArgs)):
-        n = len(pack.unpack(bytes(pack.size)))
-        a = cls.from_buffer_copy(pack.pack(*range(1, n + 1)))
-        flat = []
-        for obj in (a.cache, a):
-            for name, _ in obj._fields_:
-                x = getattr(obj, name)
-                if name != "cache":
-                    flat += list(x) if hasattr(x, "__len__") else [x]
-        assert flat == list(range(1, n + 1))
-
-
 def test_struct_sizes_match_the_header():
     assert ctypes.sizeof(abi.PagedCache) == 4 * 8 + 4 * 24 + 16 + 8 * 4
     assert ctypes.sizeof(abi.PagedKvArgs) == ctypes.sizeof(abi.PagedCache) + 16 + 32 + 16 + 16 + 8

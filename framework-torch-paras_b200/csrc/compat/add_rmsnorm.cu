@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "paged_common.cuh"
+#include "tc_prims.cuh"
 
 namespace pb {
 namespace {
@@ -29,14 +30,67 @@ struct NormParams {
     double eps;
 };
 
+// A row in 32-bit words of E elements: conversions and roundings work on whole words (element by element they, not the
+// memory, bound the 16-bit kernels: 4.6 of 6.5 TB/s).
+template <typename T> struct Word;
+template <> struct Word<float> {
+    static constexpr int E = 1;
+    static __device__ __forceinline__ void get(uint32_t w, float (&f)[1]) { f[0] = __uint_as_float(w); }
+    static __device__ __forceinline__ uint32_t put(const float (&f)[1]) { return __float_as_uint(f[0]); }
+    static __device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }
+    static constexpr uint32_t kOnes = 0x3f800000u;
+};
+template <> struct Word<__nv_bfloat16> {
+    static constexpr int E = 2;
+    static __device__ __forceinline__ void get(uint32_t w, float (&f)[2]) {
+        f[0] = __uint_as_float(w << 16);
+        f[1] = __uint_as_float(w & 0xffff0000u);
+    }
+    static __device__ __forceinline__ uint32_t put(const float (&f)[2]) { return tc::pack16<true>(f[0], f[1]); }
+    static __device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) {
+        const __nv_bfloat162 r = __hadd2_rn(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    static constexpr uint32_t kOnes = 0x3f803f80u;
+};
+template <> struct Word<__half> {
+    static constexpr int E = 2;
+    static __device__ __forceinline__ void get(uint32_t w, float (&f)[2]) {
+        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        f[0] = r.x;
+        f[1] = r.y;
+    }
+    static __device__ __forceinline__ uint32_t put(const float (&f)[2]) { return tc::pack16<false>(f[0], f[1]); }
+    static __device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) {
+        const __half2 r = __hadd2_rn(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    static constexpr uint32_t kOnes = 0x3c003c00u;
+};
+struct Quad { uint32_t w[4]; };     // 16 bytes of a row
+__device__ __forceinline__ Quad load_quad(const void* p, int64_t i) {
+    Quad q;
+    *reinterpret_cast<uint4*>(&q) = __ldcs(static_cast<const uint4*>(p) + i);
+    return q;
+}
+__device__ __forceinline__ Quad load_quad_kept(const void* p, int64_t i) {
+    Quad q;
+    *reinterpret_cast<uint4*>(&q) = __ldg(static_cast<const uint4*>(p) + i);
+    return q;
+}
+__device__ __forceinline__ void store_quad(void* p, int64_t i, const Quad& q) {
+    __stcs(static_cast<uint4*>(p) + i, *reinterpret_cast<const uint4*>(&q));
+}
+
 constexpr float kScaleMin = 1.1754943508222875e-38f;   // 2^-126
 __device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax * (1.0f / 448.0f), kScaleMin); }
 
 // TPR threads hold a row in registers, V vectors of 16 bytes each (rows whole and aligned in such vectors).
 template <typename T, int TPR, int V, bool QUANT>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR <= 128 ? 8 : 1024 / TPR)
 add_rmsnorm_rows_kernel(const NormParams p) {
-    constexpr int N = Vec16<T>::N;
+    using W = Word<T>;
+    constexpr int E = W::E, N = 4 * E;
     constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
     constexpr int kW = TPR / 32;
     static_assert(TPR % 32 == 0, "a row takes whole warps");
@@ -46,41 +100,45 @@ add_rmsnorm_rows_kernel(const NormParams p) {
     const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / TPR;
     if (row >= p.rows) return;      // (whole warps leave: with several rows a block, a row is one warp)
     const int nvec = int(p.H / N);
-    const T* x = static_cast<const T*>(p.x) + row * p.H;
-    const T* r = static_cast<const T*>(p.r) + row * p.H;
-    const T* w = static_cast<const T*>(p.w);
-    T* hrow = static_cast<T*>(p.h) + row * p.H;
-    Vec16<T> hv[V], rv[V], wv[V];
+    const int64_t at = row * nvec + tid;
+    Quad hv[V], wv[V];
+    {
+        Quad rv[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int c = i * TPR + tid;
-        if (c < nvec) {
-            hv[i] = ld16_stream(x + int64_t(c) * N);
-            if (p.r) rv[i] = ld16_stream(r + int64_t(c) * N);
+        for (int i = 0; i < V; ++i) {
+            if (i * TPR + tid < nvec) {
+                hv[i] = load_quad(p.x, at + i * TPR);
+                if (p.r) rv[i] = load_quad(p.r, at + i * TPR);
+            }
         }
-    }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int c = i * TPR + tid;
-        if (c < nvec && w) wv[i] = ld16(w + int64_t(c) * N);
+        for (int i = 0; i < V; ++i) {
+            const int c = i * TPR + tid;
+            if (p.w && c < nvec) wv[i] = load_quad_kept(p.w, c);
+            else wv[i] = Quad{{W::kOnes, W::kOnes, W::kOnes, W::kOnes}};
+        }
+        if (p.r) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i * TPR + tid < nvec) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) hv[i].w[k] = W::add(hv[i].w[k], rv[i].w[k]);
+                    store_quad(p.h, at + i * TPR, hv[i]);
+                }
+        }
     }
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int c = i * TPR + tid;
-        if (c < nvec) {
-            if (p.r) {
+    for (int i = 0; i < V; ++i)
+        if (i * TPR + tid < nvec) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) hv[i].v[e] = from_f32<T>(to_f32<T>(hv[i].v[e]) + to_f32<T>(rv[i].v[e]));
-                st16_stream(hrow + int64_t(c) * N, hv[i]);
-            }
+            for (int k = 0; k < 4; ++k) {
+                float f[E];
+                W::get(hv[i].w[k], f);
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float f = to_f32<T>(hv[i].v[e]);
-                ss = fmaf(f, f, ss);
+                for (int e = 0; e < E; ++e) ss = fmaf(f[e], f[e], ss);
             }
         }
-    }
     double total = warp_sum(double(ss));
     if constexpr (kW > 1) {
         if (lane == 0) red[warp] = total;
@@ -91,30 +149,41 @@ add_rmsnorm_rows_kernel(const NormParams p) {
     }
     const float rstd = float(1.0 / sqrt(total / double(p.H) + p.eps));
     if (p.rstd && tid == 0) p.rstd[row] = rstd;
+    // y of word k of vector i.  (The 8-bit form needs it twice, for the maxima and for the result: keeping it would cost 32
+    // registers and with them loads in flight.)
+    auto yv = [&](int i, int k, float (&y)[E]) {
+        float f[E], w[E];
+        W::get(hv[i].w[k], f);
+        W::get(wv[i].w[k], w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = f[e] * rstd * w[e];
+    };
     if constexpr (!QUANT) {
-        T* y = static_cast<T*>(p.y) + row * p.H;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = i * TPR + tid;
-            if (c < nvec) {
-                Vec16<T> o;
+        for (int i = 0; i < V; ++i)
+            if (i * TPR + tid < nvec) {
+                Quad o;
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    o.v[e] = from_f32<T>(to_f32<T>(hv[i].v[e]) * rstd * (w ? to_f32<T>(wv[i].v[e]) : 1.0f));
-                st16_stream(y + int64_t(c) * N, o);
+                for (int k = 0; k < 4; ++k) {
+                    float y[E];
+                    yv(i, k, y);
+                    o.w[k] = W::put(y);
+                }
+                store_quad(p.y, at + i * TPR, o);
             }
-        }
     } else {
-        uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.H;
-        float f[V][N], amax[V];
+        float amax[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int c = i * TPR + tid;
             amax[i] = 0.f;
+            if (i * TPR + tid < nvec) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                f[i][e] = c < nvec ? to_f32<T>(hv[i].v[e]) * rstd * (w ? to_f32<T>(wv[i].v[e]) : 1.0f) : 0.f;
-                amax[i] = fmaxf(amax[i], fabsf(f[i][e]));
+                for (int k = 0; k < 4; ++k) {
+                    float y[E];
+                    yv(i, k, y);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) amax[i] = fmaxf(amax[i], fabsf(y[e]));
+                }
             }
         }
         if (p.group == 0) {
@@ -134,30 +203,140 @@ add_rmsnorm_rows_kernel(const NormParams p) {
             if (tid == 0) p.scales[row] = scale_of(m);
         } else {
             const int gl = p.group / N;    // lanes of a group: 4 .. 32, a power of two
+            const int sh = 31 - __clz(gl);
+            for (int o = gl >> 1; o > 0; o >>= 1) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
+            }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                for (int o = gl >> 1; o > 0; o >>= 1) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
                 const int c = i * TPR + tid;
-                if (c < nvec && (c & (gl - 1)) == 0) p.scales[row * p.groups + c / gl] = scale_of(amax[i]);
+                if (c < nvec && (c & (gl - 1)) == 0) p.scales[row * p.groups + (c >> sh)] = scale_of(amax[i]);
             }
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int c = i * TPR + tid;
-            if (c >= nvec) continue;
+            if (i * TPR + tid >= nvec) continue;
             const float inv = 1.0f / scale_of(amax[i]);
-            uint32_t b[N / 4];
+            uint32_t b[E];
 #pragma unroll
-            for (int e = 0; e < N / 4; ++e)
-                b[e] = pack_e4m3(f[i][4 * e] * inv, f[i][4 * e + 1] * inv) |
-                       (pack_e4m3(f[i][4 * e + 2] * inv, f[i][4 * e + 3] * inv) << 16);
-            if constexpr (N == 8) __stcs(reinterpret_cast<uint2*>(q + int64_t(c) * 8), make_uint2(b[0], b[1]));
-            else __stcs(reinterpret_cast<uint32_t*>(q + int64_t(c) * 4), b[0]);
+            for (int x = 0; x < E; ++x) {       // four elements: 4 / E words
+                float f[4];
+#pragma unroll
+                for (int k = 0; k < 4 / E; ++k) {
+                    float y[E];
+                    yv(i, x * (4 / E) + k, y);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) f[k * E + e] = y[e] * inv;
+                }
+                b[x] = pack_e4m3(f[0], f[1]) | (pack_e4m3(f[2], f[3]) << 16);
+            }
+            if constexpr (E == 2) __stcs(static_cast<uint2*>(p.y) + at + i * TPR, make_uint2(b[0], b[1]));
+            else __stcs(static_cast<uint32_t*>(p.y) + at + i * TPR, b[0]);
         }
     }
 }
 
-// Any row length and alignment: a CTA per row, h kept in memory between the passes (L2 holds it).
+// Rows that are not whole 16-byte vectors, or not aligned: TPR threads hold a row in registers as single columns, thread t
+// columns t, t + TPR, ...  Loads and stores of two bytes a lane, 64 a warp, are half as fast as vectors; rows need not
+// start anywhere in particular.
+template <typename T, int TPR, int V, bool QUANT>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+add_rmsnorm_cols_kernel(const NormParams p) {
+    constexpr int kW = TPR / 32, kRows = TPR < 128 ? 128 / TPR : 1;
+    static_assert(kRows == 1 || kW == 1, "several rows a block: a warp each");
+    __shared__ double red[kW];
+    __shared__ float redm[QUANT ? kRows : 1][QUANT ? V : 1][kW], inv[QUANT ? kRows : 1][QUANT ? V : 1][kW];
+    const int sub = threadIdx.x / TPR, tid = threadIdx.x % TPR, lane = tid & 31, warp = tid >> 5, H = int(p.H);
+    const int64_t row = int64_t(blockIdx.x) * kRows + sub, at = row * p.H;
+    if (row >= p.rows) return;      // (whole warps, that no barrier waits for)
+    auto sync = [] {
+        if constexpr (kW == 1) __syncwarp();
+        else __syncthreads();
+    };
+    const T *x = static_cast<const T*>(p.x) + at, *r = static_cast<const T*>(p.r) + at, *w = static_cast<const T*>(p.w);
+    T hv[V], rv[V], wv[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int j = i * TPR + tid;
+        if (j < H) {
+            hv[i] = x[j];
+            if (p.r) rv[i] = r[j];
+            wv[i] = w ? w[j] : from_f32<T>(1.0f);
+        } else {
+            hv[i] = wv[i] = from_f32<T>(0.0f);
+        }
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int j = i * TPR + tid;
+        if (p.r && j < H) {
+            hv[i] = from_f32<T>(to_f32<T>(hv[i]) + to_f32<T>(rv[i]));
+            static_cast<T*>(p.h)[at + j] = hv[i];
+        }
+        const float f = to_f32<T>(hv[i]);
+        ss = fmaf(f, f, ss);
+    }
+    double total = warp_sum(double(ss));
+    if constexpr (kW > 1) {
+        if (lane == 0) red[warp] = total;
+        __syncthreads();
+        total = 0.0;
+#pragma unroll
+        for (int i = 0; i < kW; ++i) total += red[i];
+    }
+    const float rstd = float(1.0 / sqrt(total / double(p.H) + p.eps));
+    if (p.rstd && tid == 0) p.rstd[row] = rstd;
+    auto yv = [&](int i) { return to_f32<T>(hv[i]) * rstd * to_f32<T>(wv[i]); };
+    if constexpr (!QUANT) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i * TPR + tid < H) static_cast<T*>(p.y)[at + i * TPR + tid] = from_f32<T>(yv(i));
+    } else {
+        float row_inv = 0.f;
+        if (p.group == 0) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) m = fmaxf(m, fabsf(yv(i)));
+            m = warp_max(m);
+            if constexpr (kW > 1) {
+                if (lane == 0) redm[0][0][warp] = m;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kW; ++i) m = fmaxf(m, redm[0][0][i]);
+            }
+            if (tid == 0) p.scales[row] = scale_of(m);
+            row_inv = 1.0f / scale_of(m);
+        } else {
+            // A warp's 32 columns of step i are a group of 32 or a piece of a larger one, whose other pieces are the
+            // neighbouring warps', or, where a warp has the row, its neighbouring steps.  A scale is formed once per piece.
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float m = warp_max(fabsf(yv(i)));
+                if (lane == 0) redm[sub][i][warp] = m;
+            }
+            sync();
+            const int per = p.group / 32;
+            for (int e = tid; e < V * kW; e += TPR) {
+                const int first = e & ~(per - 1);
+                float m = 0.f;
+                for (int k = first; k < min(first + per, V * kW); ++k) m = fmaxf(m, redm[sub][k / kW][k % kW]);
+                inv[sub][e / kW][e % kW] = 1.0f / scale_of(m);
+                if (e == first && int64_t(e) * 32 < p.H) p.scales[row * p.groups + e / per] = scale_of(m);
+            }
+            sync();
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int j = i * TPR + tid;
+            const float f = p.group ? inv[sub][i][warp] : row_inv;
+            if (j < H) static_cast<uint8_t*>(p.y)[at + j] = uint8_t(pack_e4m3(yv(i) * f, 0.f));
+        }
+    }
+}
+
+// Rows too long for registers: a CTA per row, h kept in memory between the passes (L2 holds it).
 template <typename T, bool QUANT>
 __global__ void __launch_bounds__(256)
 add_rmsnorm_any_kernel(const NormParams p) {
@@ -252,6 +431,17 @@ void launch_fwd(const NormParams& p, bool vec, cudaStream_t s) {
     } else if (vec && nvec <= 1024 * 4) {
         if (nvec <= 2048) go(add_rmsnorm_rows_kernel<T, 512, 4, QUANT>, 512);
         else go(add_rmsnorm_rows_kernel<T, 1024, 4, QUANT>, 1024);
+    } else if (p.H <= 256 * 4) {
+        // (a warp to 256 columns, 128 threads to 1024)
+        if (p.H <= 128) go(add_rmsnorm_cols_kernel<T, 32, 4, QUANT>, 32);
+        else if (p.H <= 256) go(add_rmsnorm_cols_kernel<T, 32, 8, QUANT>, 32);
+        else if (p.H <= 512) add_rmsnorm_cols_kernel<T, 128, 4, QUANT><<<unsigned(p.rows), 128, 0, s>>>(p);
+        else add_rmsnorm_cols_kernel<T, 128, 8, QUANT><<<unsigned(p.rows), 128, 0, s>>>(p);
+    } else if (p.H <= 1024 * 16) {
+        if (p.H <= 256 * 8) add_rmsnorm_cols_kernel<T, 256, 8, QUANT><<<unsigned(p.rows), 256, 0, s>>>(p);
+        else if (p.H <= 256 * 16) add_rmsnorm_cols_kernel<T, 256, 16, QUANT><<<unsigned(p.rows), 256, 0, s>>>(p);
+        else if (p.H <= 512 * 16) add_rmsnorm_cols_kernel<T, 512, 16, QUANT><<<unsigned(p.rows), 512, 0, s>>>(p);
+        else add_rmsnorm_cols_kernel<T, 1024, 16, QUANT><<<unsigned(p.rows), 1024, 0, s>>>(p);
     } else {
         const int64_t blocks = std::min<int64_t>(p.rows, 148 * 8);
         add_rmsnorm_any_kernel<T, QUANT><<<int(blocks), 256, 0, s>>>(p);
@@ -284,7 +474,8 @@ struct BwdParams {
 template <typename T, int THREADS, int V>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS)
 add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
-    constexpr int N = Vec16<T>::N;
+    using W = Word<T>;
+    constexpr int E = W::E, N = 4 * E;
     constexpr int kStages = bwd_stages(THREADS, V);
     constexpr uint32_t kOne = THREADS * V * 16, kStage = 3 * kOne;
     extern __shared__ __align__(16) unsigned char ring_raw[];
@@ -292,7 +483,7 @@ add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(ring_raw));
     const int nvec = int(p.H / N);
-    const T *gy = static_cast<const T*>(p.gy), *gh = static_cast<const T*>(p.gh), *h = static_cast<const T*>(p.h);
+    const uint4 *gy = static_cast<const uint4*>(p.gy), *gh = static_cast<const uint4*>(p.gh), *h = static_cast<const uint4*>(p.h);
     auto issue = [&](int64_t row, int stage) {
         if (row < p.rows) {
 #pragma unroll
@@ -300,7 +491,7 @@ add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
                 const int c = i * THREADS + tid;
                 if (c < nvec) {
                     const uint32_t dst = ring + stage * kStage + uint32_t(c) * 16;
-                    const int64_t at = row * p.H + int64_t(c) * N;
+                    const int64_t at = row * nvec + c;
                     copy16(dst, gy + at);
                     copy16(dst + kOne, h + at);
                     if (gh) copy16(dst + 2 * kOne, gh + at);
@@ -309,18 +500,16 @@ add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
         }
         copy_commit();
     };
-    Vec16<T> wv[V];
+    Quad wv[V];
     float dw[V * N];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = i * THREADS + tid;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            wv[i].v[e] = from_f32<T>(1.0f);
-            dw[i * N + e] = 0.f;
-        }
-        if (p.w && c < nvec) wv[i] = ld16(static_cast<const T*>(p.w) + int64_t(c) * N);
+        if (p.w && c < nvec) wv[i] = load_quad_kept(p.w, c);
+        else wv[i] = Quad{{W::kOnes, W::kOnes, W::kOnes, W::kOnes}};
     }
+#pragma unroll
+    for (int i = 0; i < V * N; ++i) dw[i] = 0.f;
     const float inv_h = 1.0f / float(p.H);
 #pragma unroll
     for (int st = 0; st < kStages - 1; ++st) issue(int64_t(blockIdx.x) + int64_t(st) * gridDim.x, st);
@@ -331,19 +520,25 @@ add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
         const float rr = rr_next;
         rr_next = p.rstd[min(row + int64_t(gridDim.x), p.rows - 1)];
         copy_wait<kStages - 1>();
-        const unsigned char* buf = ring_raw + stage * kStage;
+        const uint4* buf = reinterpret_cast<const uint4*>(ring_raw + stage * kStage);
         stage = stage + 1 == kStages ? 0 : stage + 1;
-        Vec16<T> g[V], x[V];
+        Quad g[V], x[V];
         float dot = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = i * THREADS + tid;
             if (c < nvec) {
-                g[i] = *reinterpret_cast<const Vec16<T>*>(buf + c * 16);
-                x[i] = *reinterpret_cast<const Vec16<T>*>(buf + kOne + c * 16);
+                *reinterpret_cast<uint4*>(&g[i]) = buf[c];
+                *reinterpret_cast<uint4*>(&x[i]) = buf[kOne / 16 + c];
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    dot = fmaf(to_f32<T>(g[i].v[e]) * to_f32<T>(wv[i].v[e]), to_f32<T>(x[i].v[e]), dot);
+                for (int k = 0; k < 4; ++k) {
+                    float ge[E], xe[E], we[E];
+                    W::get(g[i].w[k], ge);
+                    W::get(x[i].w[k], xe);
+                    W::get(wv[i].w[k], we);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) dot = fmaf(ge[e] * we[e], xe[e], dot);
+                }
             }
         }
         dot = warp_sum(dot);
@@ -353,20 +548,27 @@ add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
 #pragma unroll
         for (int i = 0; i < THREADS / 32; ++i) dot += red[flip][i];
         const float coef = rr * rr * (inv_h * dot) * rr;
-        T* out = static_cast<T*>(p.gx) + row * p.H;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = i * THREADS + tid;
             if (c < nvec) {
-                Vec16<T> o, a;
-                if (gh) a = *reinterpret_cast<const Vec16<T>*>(buf + 2 * kOne + c * 16);
+                Quad o, a{};
+                if (gh) *reinterpret_cast<uint4*>(&a) = buf[2 * (kOne / 16) + c];
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const float ge = to_f32<T>(g[i].v[e]), xe = to_f32<T>(x[i].v[e]);
-                    o.v[e] = from_f32<T>(fmaf(ge * to_f32<T>(wv[i].v[e]), rr, -coef * xe) + (gh ? to_f32<T>(a.v[e]) : 0.f));
-                    dw[i * N + e] = fmaf(ge * xe, rr, dw[i * N + e]);
+                for (int k = 0; k < 4; ++k) {
+                    float ge[E], xe[E], we[E], ae[E], oe[E];
+                    W::get(g[i].w[k], ge);
+                    W::get(x[i].w[k], xe);
+                    W::get(wv[i].w[k], we);
+                    W::get(a.w[k], ae);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        oe[e] = fmaf(ge[e] * we[e], rr, fmaf(-coef, xe[e], ae[e]));
+                        dw[i * N + k * E + e] = fmaf(ge[e] * xe[e], rr, dw[i * N + k * E + e]);
+                    }
+                    o.w[k] = W::put(oe);
                 }
-                st16_stream(out + int64_t(c) * N, o);
+                store_quad(p.gx, row * nvec + c, o);
             }
         }
     }
@@ -385,7 +587,83 @@ add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
     }
 }
 
-// Any row length and alignment: grad_x, a CTA per row.
+// The same for rows that are not whole aligned vectors, a column at a time as in the forward: the next row's values are in
+// flight, in registers, while a row is reduced and written.
+template <typename T, int THREADS, int V>
+__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS)
+add_rmsnorm_bwd_cols_kernel(const BwdParams p) {
+    // below 128 threads a block is several walkers, a warp each, that share nothing
+    constexpr int kSubs = THREADS < 128 ? 128 / THREADS : 1;
+    static_assert(kSubs == 1 || THREADS == 32, "a walker is a warp or the block");
+    __shared__ float red[2][THREADS / 32];
+    const int64_t walker = int64_t(blockIdx.x) * kSubs + threadIdx.x / THREADS, walkers = int64_t(gridDim.x) * kSubs;
+    const int tid = threadIdx.x % THREADS, lane = tid & 31, warp = tid >> 5, H = int(p.H);
+    const T *gy = static_cast<const T*>(p.gy), *gh = static_cast<const T*>(p.gh), *h = static_cast<const T*>(p.h), *w = static_cast<const T*>(p.w);
+    const T zero = from_f32<T>(0.f);
+    T wv[V], g[V], x[V], a[V], g2[V], x2[V], a2[V];
+    float dw[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int j = i * THREADS + tid;
+        wv[i] = w && j < H ? w[j] : from_f32<T>(1.0f);
+        dw[i] = 0.f;
+        g[i] = x[i] = a[i] = zero;
+    }
+    auto fetch = [&](int64_t row, T (&fg)[V], T (&fx)[V], T (&fa)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int j = i * THREADS + tid;
+            const bool live = j < H && row < p.rows;
+            const int64_t at = row * p.H + j;
+            fg[i] = live ? gy[at] : zero;
+            fx[i] = live ? h[at] : zero;
+            fa[i] = live && gh ? gh[at] : zero;
+        }
+    };
+    const float inv_h = 1.0f / float(p.H);
+    int flip = 0;
+    auto step = [&](int64_t row, const T (&fg)[V], const T (&fx)[V], const T (&fa)[V]) {
+        const float rr = p.rstd[row];
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) dot = fmaf(to_f32<T>(fg[i]) * to_f32<T>(wv[i]), to_f32<T>(fx[i]), dot);
+        dot = warp_sum(dot);
+        if constexpr (kSubs == 1) {
+            if (lane == 0) red[flip][warp] = dot;
+            __syncthreads();
+            dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < THREADS / 32; ++i) dot += red[flip][i];
+            flip ^= 1;
+        }
+        const float coef = rr * rr * (inv_h * dot) * rr;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int j = i * THREADS + tid;
+            const float ge = to_f32<T>(fg[i]), xe = to_f32<T>(fx[i]);
+            if (j < H) static_cast<T*>(p.gx)[row * p.H + j] = from_f32<T>(fmaf(ge * to_f32<T>(wv[i]), rr, fmaf(-coef, xe, to_f32<T>(fa[i]))));
+            dw[i] = fmaf(ge * xe, rr, dw[i]);
+        }
+    };
+    fetch(walker, g, x, a);
+    for (int64_t row = walker; row < p.rows; row += 2 * walkers) {
+        const int64_t next = row + walkers;
+        fetch(next, g2, x2, a2);
+        step(row, g, x, a);
+        if (next >= p.rows) break;       // (the same for the whole walker)
+        fetch(next + walkers, g, x, a);
+        step(next, g2, x2, a2);
+    }
+    if (p.part) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int j = i * THREADS + tid;
+            if (j < H) p.part[walker * p.H + j] = dw[i];
+        }
+    }
+}
+
+// Rows too long for registers: grad_x, a CTA per row.
 template <typename T>
 __global__ void __launch_bounds__(256)
 add_rmsnorm_bwd_dx_kernel(const BwdParams p) {
@@ -461,15 +739,18 @@ int launch_bwd(Gpu* g, BwdParams p, void* gw, bool vec, cudaStream_t s) {
     const int64_t nvec = p.H / N;
     const int sms = g->sm_count > 0 ? g->sm_count : 148;
     const unsigned dwblocks = unsigned((p.H + 31) / 32);
-    if (vec && nvec <= 512 * 4) {
+    const bool cols = !(vec && nvec <= 512 * 4) && p.H <= 1024 * 8;
+    if (cols || (vec && nvec <= 512 * 4)) {
         // 128, 256 or 512 threads a row, at most 4 vectors each; the ring (2 or 3 stages of 3 inputs) takes at most
         // 72 / 144 / 216 KB a CTA; 4 / 2 / 1 CTAs share an SM as registers and shared memory allow
-        const int threads = nvec <= 128 * 4 ? 128 : nvec <= 256 * 4 ? 256 : 512;
-        const int v = int((nvec + threads - 1) / threads);
-        const size_t ring = size_t(bwd_stages(threads, v)) * 3 * threads * v * 16;
-        int per_sm = 512 / threads;
+        // (columns: 32 to 1024 threads, at most 8 columns each)
+        const int threads = cols ? (p.H <= 256 ? 32 : p.H <= 1024 ? 128 : p.H <= 2048 ? 256 : p.H <= 4096 ? 512 : 1024) : nvec <= 128 * 4 ? 128 : nvec <= 256 * 4 ? 256 : 512;
+        const int v = cols ? 8 : int((nvec + threads - 1) / threads);
+        const size_t ring = cols ? 0 : size_t(bwd_stages(threads, v)) * 3 * threads * v * 16;
+        int per_sm = std::max(1, (cols ? 1024 : 512) / threads);
         while (per_sm > 1 && (ring + 1024) * per_sm > 220 * 1024) --per_sm;
-        const int parts = int(std::min<int64_t>(p.rows, int64_t(sms) * per_sm));
+        const int parts = threads == 32 ? int((std::min<int64_t>(p.rows, int64_t(sms) * 32) + 3) / 4 * 4)
+                                        : int(std::min<int64_t>(p.rows, int64_t(sms) * per_sm));
         void* scratch = nullptr;
         if (gw) {
             const int st = paras_b200_malloc_async(g->ordinal, size_t(parts) * size_t(p.H) * sizeof(float), s, &scratch);
@@ -488,7 +769,14 @@ int launch_bwd(Gpu* g, BwdParams p, void* gw, bool vec, cudaStream_t s) {
             else if (v == 3) go(add_rmsnorm_bwd_rows_kernel<T, TH, 3>);
             else go(add_rmsnorm_bwd_rows_kernel<T, TH, 4>);
         };
-        if (threads == 128) by_v(std::integral_constant<int, 128>());
+        auto plain = [&](auto kernel) { kernel<<<parts, threads, 0, s>>>(p); };
+        if (cols) {
+            if (threads == 32) add_rmsnorm_bwd_cols_kernel<T, 32, 8><<<parts / 4, 128, 0, s>>>(p);
+            else if (threads == 128) plain(add_rmsnorm_bwd_cols_kernel<T, 128, 8>);
+            else if (threads == 256) plain(add_rmsnorm_bwd_cols_kernel<T, 256, 8>);
+            else if (threads == 512) plain(add_rmsnorm_bwd_cols_kernel<T, 512, 8>);
+            else plain(add_rmsnorm_bwd_cols_kernel<T, 1024, 8>);
+        } else if (threads == 128) by_v(std::integral_constant<int, 128>());
         else if (threads == 256) by_v(std::integral_constant<int, 256>());
         else by_v(std::integral_constant<int, 512>());
         if (err == cudaSuccess && gw)

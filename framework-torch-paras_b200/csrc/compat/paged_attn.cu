@@ -104,11 +104,29 @@ int check(const paras_paged_attn_args* args, const char* what) {
 
 // At most 16 query rows per kv head stream through mma.sync tiles, more go to the tensor-core tiles of 128 rows; fp32,
 // other head dims than 64 and 128, pages that no tile of 128 positions is made of, and unaligned tensors to CUDA cores.
-enum class Route { kSimt, kDecode, kTc };
-Route pick_route(const Gpu* g, const paras_paged_attn_args& a) {
-    return paged_decode_supported(g, a) ? Route::kDecode : paged_tc_supported(g, a) ? Route::kTc : Route::kSimt;
+// A call for chunks whose sequences besides the longest average less than twice 16 rows is taken to mix both, and makes a
+// launch for each: single tokens in 128-row tiles cost their CTA a whole softmax tile per step (12 sequences, one of 700
+// tokens, 8-bit cache: 93 us in one launch).  The rule goes by counts the host knows; where it is wrong, one of the launches
+// finds nothing to do and costs about 3 us.
+struct Routes {
+    bool decode, tc;
+    int small;      // tokens a sequence may have for the first of the two
+};
+Routes pick_routes(const Gpu* g, const paras_paged_attn_args& a) {
+    Routes r{};
+    const int group = a.Hq / a.cache.Hkv;
+    r.small = 16 / group;
+    const bool dec = paged_decode_supported(g, a);
+    if (dec && a.max_q <= r.small) {
+        r.decode = true;
+    } else if (paged_tc_supported(g, a)) {
+        r.tc = true;
+        const int64_t others = a.cache.B - 1, left = int64_t(a.T) - a.max_q;
+        r.decode = dec && others > 0 && left < others * 2 * r.small;
+    }
+    return r;
 }
-int route_rows(Route r) { return r == Route::kDecode ? paged_decode_rows() : paged_tc_rows(); }
+size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
 int stream_ctas(const Gpu* g) { return g->sm_count > 0 ? g->sm_count : 148; }   // persistent, one per SM
 
 PagedParams make_params(const Gpu* g, const paras_paged_attn_args& a) {
@@ -129,6 +147,8 @@ PagedParams make_params(const Gpu* g, const paras_paged_attn_args& a) {
     p.causal = a.causal;
     p.scale = float(a.scale);
     p.scale_log2 = p.scale * 1.4426950408889634f;
+    p.q_min = 1;
+    p.q_max = p.qbox = p.max_q;
     p.status = g->status_dev;
     const int box = c.page < kTileKeys ? c.page : kTileKeys;
     p.box_shift = 0;
@@ -172,10 +192,11 @@ int paras_b200_paged_attn(const paras_paged_attn_args* args) {
     if (!a.q || !a.out || !a.kv_lens || !a.cu) return fail(PARAS_E_INVALID, "%s: null pointer", what);
     const pb::PagedParams p = pb::make_params(g, a);
     cudaStream_t s = pb::pick_stream(g, a.stream);
-    const pb::Route r = pb::pick_route(g, a);
-    if (r == pb::Route::kSimt) return pb::paged_simt_launch(p, a.dtype, a.cache.cache_dtype == PARAS_E4M3, s);
-    const int G = pb::stream_ctas(g), rows = pb::route_rows(r);
-    const size_t need = pb::paged_workspace_bytes(G, rows, p.D);
+    const pb::Routes r = pb::pick_routes(g, a);
+    if (!r.decode && !r.tc) return pb::paged_simt_launch(p, a.dtype, a.cache.cache_dtype == PARAS_E4M3, s);
+    const int G = pb::stream_ctas(g);
+    const size_t dec_bytes = r.decode ? pb::round16(pb::paged_workspace_bytes(G, pb::paged_decode_rows(), p.D)) : 0;
+    const size_t need = dec_bytes + (r.tc ? pb::paged_workspace_bytes(G, pb::paged_tc_rows(), p.D) : 0);
     void* scratch = a.workspace;
     if (scratch) {
         if (a.workspace_bytes < need)
@@ -184,9 +205,26 @@ int paras_b200_paged_attn(const paras_paged_attn_args* args) {
     } else if ((st = paras_b200_malloc_async(a.gpu, need, s, &scratch)) != PARAS_OK) {
         return st;
     }
-    const pb::PagedWorkspace ws = pb::paged_carve(scratch, G, rows);
-    st = r == pb::Route::kDecode ? pb::paged_decode_launch(g, a, p, ws, G, s) : pb::paged_tc_launch(g, a, p, ws, G, s);
-    if (st == PARAS_OK) pb::tl_paged_kernel = r == pb::Route::kDecode ? "paged_decode" : "paged_tcgen05";
+    pb::PagedWorkspace ws[2];
+    int rows[2], count = 0;
+    if (r.tc) {
+        pb::PagedParams pt = p;
+        if (r.decode) pt.q_min = r.small + 1;
+        rows[count] = pb::paged_tc_rows();
+        ws[count] = pb::paged_carve(static_cast<char*>(scratch) + dec_bytes, G, rows[count]);
+        st = pb::paged_tc_launch(g, a, pt, ws[count++], G, s);
+    }
+    if (st == PARAS_OK && r.decode) {
+        pb::PagedParams pd = p;
+        pd.q_max = r.small < p.max_q ? r.small : p.max_q;
+        pd.qbox = pd.q_max;
+        pd.wait_late = r.tc;
+        rows[count] = pb::paged_decode_rows();
+        ws[count] = pb::paged_carve(scratch, G, rows[count]);
+        st = pb::paged_decode_launch(g, a, pd, ws[count++], G, s);
+    }
+    if (st == PARAS_OK) st = pb::paged_join_launch(p, ws, rows, count, G, a.dtype, s);
+    if (st == PARAS_OK) pb::tl_paged_kernel = r.tc ? (r.decode ? "paged_tcgen05+paged_decode" : "paged_tcgen05") : "paged_decode";
     if (!a.workspace) {
         const int st2 = paras_b200_free_async(a.gpu, scratch, s);
         if (st == PARAS_OK) st = st2;
@@ -202,8 +240,10 @@ int paras_b200_paged_attn_workspace_bytes(const paras_paged_attn_args* args, siz
     pb::DeviceRestore restore;
     pb::Gpu* g = pb::use_gpu(args->gpu, &st);
     if (!g) return st;
-    const pb::Route r = pb::pick_route(g, *args);
-    if (r != pb::Route::kSimt) *bytes = pb::paged_workspace_bytes(pb::stream_ctas(g), pb::route_rows(r), args->cache.D);
+    const pb::Routes r = pb::pick_routes(g, *args);
+    const int G = pb::stream_ctas(g), D = args->cache.D;
+    if (r.decode) *bytes += pb::round16(pb::paged_workspace_bytes(G, pb::paged_decode_rows(), D));
+    if (r.tc) *bytes += pb::paged_workspace_bytes(G, pb::paged_tc_rows(), D);
     return PARAS_OK;
 }
 

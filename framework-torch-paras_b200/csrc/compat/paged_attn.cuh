@@ -21,6 +21,10 @@ struct PagedParams {
     int64_t qs[2], os[2];
     int64_t cks[3], cvs[3], eks[3], evs[3];
     int T, Hq, Hkv, group, D, B, max_pages, pages, page, max_q;
+    // A launch takes the sequences of q_min to q_max new tokens (a call that mixes single tokens with chunks makes one
+    // launch for each); qbox: tokens that a TMA box on q covers in the launch for few.
+    int q_min, q_max, qbox;
+    int wait_late;       // the launch depends on the one before it only for the order of what comes after
     int cap;             // positions the page table can name
     int causal;
     float scale, scale_log2;
@@ -44,6 +48,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
     const int end = max(s.row0, min(c1, p.T));
     const int count = end - s.row0;
     s.nq = min(count, p.max_q);
+    if (s.nq < p.q_min || s.nq > p.q_max) s.nq = 0;
     s.kv = max(0, min(kv, p.cap));
     s.pos0 = int(max(int64_t(-(1 << 30)), min(int64_t(kv) - count, int64_t(1 << 30))));
     return s;
@@ -179,8 +184,26 @@ cudaError_t paged_allow_smem(int gpu, int bytes) {
     return e;
 }
 
-// Joins the partial results of cut items: a launch of G blocks after the streaming kernel on the same stream.
-int paged_join_launch(const PagedParams& p, const PagedWorkspace& ws, int G, int rows, int dtype, cudaStream_t s);
+// Joins the partial results that up to two streaming launches (of G CTAs, items of rows[i] query rows) left of their cut
+// items: one launch after them on the same stream.
+int paged_join_launch(const PagedParams& p, const PagedWorkspace* ws, const int* rows, int count, int G, int dtype, cudaStream_t s);
+
+// Launches `kernel` so that its start may overlap the end of the kernel before it, for whose memory it waits itself
+// (griddepcontrol.wait).
+template <typename... Params, typename... Args>
+cudaError_t paged_launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(unsigned(threads), 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
 
 bool paged_decode_supported(const Gpu* g, const paras_paged_attn_args& a);
 int paged_decode_rows();     // query rows of an item in the workspace
@@ -192,9 +215,10 @@ int paged_tc_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p
 
 // Can the cache be read by TMA in tiles of 128 positions (page size, alignment, strides)?
 bool paged_tma_ok(const paras_paged_cache& c);
-// Map of the cache's K (which = 0) or V: {D, position, head, page}, box of one page's (at most 128) rows by 128 bytes (the
-// row, where it is shorter).  16-bit rows: slabs of 64 elements; 8-bit rows: the whole row.
-int paged_cache_map(CUtensorMap_st* map, const paras_paged_cache& c, int which);
+// Map of the cache's K (which = 0) or V, a box of one page's (at most 128) rows by 128 bytes (the row, where it is
+// shorter): {D, position, head, page}, 16-bit rows in slabs of 64 elements that are loaded one by one; or, with `whole`,
+// {64, position, slab, head, page} and all slabs in one box, slab after slab.
+int paged_cache_map(CUtensorMap_st* map, const paras_paged_cache& c, int which, bool whole);
 // Map of q seen as {D, group, kv head, token}: box {64, group, 1, tokens}.
 bool paged_q_tma_ok(const paras_paged_attn_args& a);
 int paged_q_map(CUtensorMap_st* map, const paras_paged_attn_args& a, int tokens);

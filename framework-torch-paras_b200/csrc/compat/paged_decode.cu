@@ -108,6 +108,14 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
     return r;
 }
 
+// 5-D tiled load global -> shared, completion on an mbarrier.
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+        : "memory");
+}
+
 // Byte offset of 16-byte unit c of row r in a tile that TMA wrote with the 128- or 64-byte swizzle.
 template <int ROW>
 __device__ __forceinline__ uint32_t swz(int r, int c) {
@@ -148,6 +156,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         mbar_fence_init();
         fence_proxy_async_smem();
     }
+    if (!p.wait_late) asm volatile("griddepcontrol.wait;" ::: "memory");
     int b0;
     int64_t base0;
     const PagedRange range = paged_range(p.B, reinterpret_cast<int64_t*>(gen + R::kSums),
@@ -322,16 +331,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const CUtensorMap* map = role ? &map_v : &map_k;
             const uint32_t at = dst + (role ? R::kTile : 0);
             if (lane == 0)
-                mbar_arrive_expect_tx(full(s), R::kTile + (role == 0 && first ? (HD / 64) * p.max_q * p.group * 128 : 0));
+                mbar_arrive_expect_tx(full(s), R::kTile + (role == 0 && first ? (HD / 64) * p.qbox * p.group * 128 : 0));
             __syncwarp();
             // one lane issues: a box per lane would be issued one after the other too, with a loop around it
             for (int x = 0; x < p.npg; ++x) {
                 const int pgx = __shfl_sync(0xffffffffu, page, x);
-                if (lane == 0) {
-#pragma unroll
-                    for (int c = 0; c < R::kSlabs; ++c)
-                        tma_load_4d(at + c * R::kSlab + (x << p.box_shift) * R::kRow, map, full(s), 64 * c, row, hk, pgx);
-                }
+                if (lane == 0) tma_load_5d(at + (x << p.box_shift) * R::kSlabs * R::kRow, map, full(s), 0, row, 0, hk, pgx);
             }
             if (role == 0 && first && lane == 0) {
 #pragma unroll
@@ -346,6 +351,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         // ------------------------------ consumers ------------------------------
         const int r0 = lane >> 2, t = lane & 3;
         const int krow = warp * 16;             // this warp's keys in a tile
+        // A tile is boxes of 2^box_shift keys, each with its slabs of 128-byte rows one after the other: where row r's
+        // first slab begins, and how far the next one is.
+        auto row_at = [&](int r) {
+            return uint32_t(((r >> p.box_shift) << p.box_shift) * R::kSlabs + (r & ((1 << p.box_shift) - 1))) * uint32_t(R::kRow);
+        };
+        const uint32_t slab_step = uint32_t(R::kRow) << p.box_shift;
+        // of K, column n of an n-tile is any key: key n of 8, or, where four keys of V share a register, the one that leaves a
+        // thread with keys 4t, 4t+1 of the first n-tile and 4t+2, 4t+3 of the second
+        int krows[2];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) krows[nt] = krow + (E8 ? 4 * ((lane & 7) >> 1) + 2 * nt + (lane & 1) : nt * 8 + (lane & 7));
+        const uint32_t k_at[2] = {row_at(krows[0]), row_at(krows[1])}, v_at = row_at(krow + (lane & 15));
+        // 16-byte unit c of row r of a slab, swizzled
+        auto unit = [](int r, int c) { return swz<R::kRow>(r, c) - uint32_t(r * R::kRow); };
         float* merge = reinterpret_cast<float*>(gen + R::kMerge);
         float* m_sm = reinterpret_cast<float*>(gen + R::kMl);
         float* l_sm = m_sm + kConsumers * kRows;
@@ -442,11 +461,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             uint32_t kf[kLd][4], vf[kLd][4];
 #pragma unroll
             for (int x = 0; x < kLd; ++x) {
-                // column n of an n-tile is any key: key n of 8, or, where four keys of V share a register, the one
-                // that leaves a thread with keys 4t, 4t+1 of the first n-tile and 4t+2, 4t+3 of the second
-                const int row = krow + (E8 ? 4 * ((lane & 7) >> 1) + 2 * (x & 1) + (lane & 1) : (x & 1) * 8 + (lane & 7));
                 const int c = (x >> 1) * 4 + (lane >> 3);   // 16-byte unit of the row
-                ldsm4(kt + (E8 ? 0 : (c >> 3) * R::kSlab) + swz<R::kRow>(row, E8 ? c : c & 7), kf[x]);
+                ldsm4(kt + k_at[x & 1] + (E8 ? unit(krows[x & 1], c) : (c >> 3) * slab_step + unit(krows[x & 1], c & 7)), kf[x]);
             }
             // ---- S = Q K^T: two n-tiles of 8 keys, even and odd steps summed apart ----
             float sc[2][4], sd[2][4];
@@ -472,8 +488,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
             for (int x = 0; x < kLd; ++x) {
                 const int row = krow + (lane & 15), c = x * 2 + (lane >> 4);
-                if constexpr (E8) ldsm2_t8(vt + swz<R::kRow>(row, c), vf[x]);
-                else ldsm4_t(vt + (c >> 3) * R::kSlab + swz<128>(row, c & 7), vf[x]);
+                if constexpr (E8) ldsm2_t8(vt + v_at + unit(row, c), vf[x]);
+                else ldsm4_t(vt + v_at + (c >> 3) * slab_step + unit(row, c & 7), vf[x]);
             }
             // this thread's columns of n-tile nt: keys first + step * nt, + 1
             const int first = krow + (E8 ? 4 : 2) * t;
@@ -664,6 +680,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
         }
     }
+    // (launched beside the kernel for chunks, whose inputs are complete: only what follows must find both done)
+    if (p.wait_late) asm volatile("griddepcontrol.wait;" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) {
         *p.status = *abort_flag;
@@ -676,8 +694,7 @@ int launch(int gpu, int G, cudaStream_t s, const CUtensorMap& mq, const CUtensor
            const PagedWorkspace& ws) {
     constexpr int bytes = Ring<E8, HD>::kLaunch;
     PB_CUDA((paged_allow_smem<paged_decode_kernel<BF16, E8, HD>>(gpu, bytes)));
-    paged_decode_kernel<BF16, E8, HD><<<G, Ring<E8, HD>::kThreads, bytes, s>>>(mq, mk, mv, p, ws);
-    PB_LAUNCH_CHECK("paged_decode_kernel");
+    PB_CUDA(paged_launch(paged_decode_kernel<BF16, E8, HD>, dim3(unsigned(G)), Ring<E8, HD>::kThreads, bytes, s, mq, mk, mv, p, ws));
     return PARAS_OK;
 }
 
@@ -687,23 +704,22 @@ int paged_decode_rows() { return kRows; }
 
 bool paged_decode_supported(const Gpu* g, const paras_paged_attn_args& a) {
     return g->cc_major >= 9 && a.dtype != PARAS_F32 && paged_tma_ok(a.cache) && paged_q_tma_ok(a) &&
-           int64_t(a.max_q) * (a.Hq / a.cache.Hkv) <= kRows && g->smem_optin >= 227 * 1024;
+           a.Hq / a.cache.Hkv <= kRows && g->smem_optin >= 227 * 1024;
 }
 
 int paged_decode_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p, const PagedWorkspace& ws, int G, cudaStream_t s) {
     int st = check_status_word(g);
     if (st != PARAS_OK) return st;
     CUtensorMap mq, mk, mv;
-    if ((st = paged_q_map(&mq, a, p.max_q)) != PARAS_OK) return st;
-    if ((st = paged_cache_map(&mk, a.cache, 0)) != PARAS_OK) return st;
-    if ((st = paged_cache_map(&mv, a.cache, 1)) != PARAS_OK) return st;
+    if ((st = paged_q_map(&mq, a, p.qbox)) != PARAS_OK) return st;
+    if ((st = paged_cache_map(&mk, a.cache, 0, true)) != PARAS_OK) return st;
+    if ((st = paged_cache_map(&mv, a.cache, 1, true)) != PARAS_OK) return st;
     const bool bf = a.dtype == PARAS_BF16, e8 = a.cache.cache_dtype == PARAS_E4M3;
 #define PB_GO(B, E, H) launch<B, E, H>(g->ordinal, G, s, mq, mk, mv, p, ws)
     if (p.D == 128) st = bf ? (e8 ? PB_GO(true, true, 128) : PB_GO(true, false, 128)) : (e8 ? PB_GO(false, true, 128) : PB_GO(false, false, 128));
     else st = bf ? (e8 ? PB_GO(true, true, 64) : PB_GO(true, false, 64)) : (e8 ? PB_GO(false, true, 64) : PB_GO(false, false, 64));
 #undef PB_GO
-    if (st != PARAS_OK) return st;
-    return paged_join_launch(p, ws, G, kRows, a.dtype, s);
+    return st;
 }
 
 }  // namespace pb

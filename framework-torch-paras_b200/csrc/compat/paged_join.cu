@@ -9,39 +9,74 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 
+struct JoinSet {
+    PagedWorkspace ws[2];
+    int rows[2];
+};
+
 // out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the parts s of an item, in the order of the CTAs: a warp per
-// row, the head dim over its lanes.  The parts were written a moment ago and lie in L2; few items are cut, so the
-// launch itself is most of its cost: it is launched early and waits for the streaming kernel's memory.
+// row, the head dim over its lanes.  The parts were written a moment ago and lie in L2, and few items are cut, so latency
+// is all of its cost: it is launched early and waits for the streaming kernel's memory, and the first four parts' outputs
+// are asked for together with the maxima that weigh them.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-paged_join_kernel(const PagedParams p, const PagedWorkspace ws, int rows_per_slot) {
+paged_join_kernel(const PagedParams p, const JoinSet set) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const PagedWorkspace& ws = set.ws[blockIdx.z];
+    const int slot_rows = set.rows[blockIdx.z];
     const PagedJoin j = ws.join[blockIdx.x];
     if (j.first_slot < 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows = j.nq * p.group, parts = j.last_cta - int(blockIdx.x) + 1;
-    constexpr int E = D / 32;
+    constexpr int E = D / 32, kAhead = 4;
     auto slot = [&](int i) { return i == 0 ? j.first_slot : 2 * (int(blockIdx.x) + i); };
     for (int r = blockIdx.y * (kJoinThreads / 32) + warp; r < rows; r += gridDim.y * (kJoinThreads / 32)) {
+        auto outputs = [&](int i, float (&o)[E]) {
+            const float* src = ws.o + (size_t(slot(i)) * slot_rows + r) * D + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(src + e));
+                o[e] = v.x;
+                o[e + 1] = v.y;
+            }
+        };
+        float ahead[kAhead][E];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (i < parts) outputs(i, ahead[i]);
+        // lane i looks at parts i, i + 32, ...
         float M = -INFINITY;
-        for (int i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(&ws.ml[size_t(slot(i)) * rows_per_slot + r]).x);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < parts) ml = __ldcg(&ws.ml[size_t(slot(lane)) * slot_rows + r]);
+        M = ml.x;
+        for (int i = lane + 32; i < parts; i += 32) M = fmaxf(M, __ldcg(&ws.ml[size_t(slot(i)) * slot_rows + r]).x);
         M = warp_max(M);
         float l = 0.f, acc[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = 0.f;
         if (M != -INFINITY) {
-#pragma unroll 4
+            float w = 0.f;      // of part i0 + lane; 0 for one that saw no key, whose outputs may not have been written
             for (int i = 0; i < parts; ++i) {
-                const size_t at = size_t(slot(i)) * rows_per_slot + r;
-                const float2 ml = __ldcg(&ws.ml[at]);
-                if (ml.x == -INFINITY) continue;      // a part that saw no key: its outputs may not have been written
-                const float w = tc::ex2_approx(ml.x - M);
-                l = fmaf(w, ml.y, l);
+                if ((i & 31) == 0) {
+                    if (i > 0) ml = i + lane < parts ? __ldcg(&ws.ml[size_t(slot(i + lane)) * slot_rows + r]) : make_float2(-INFINITY, 0.f);
+                    w = ml.x == -INFINITY ? 0.f : tc::ex2_approx(ml.x - M);
+                    l += warp_sum(w * ml.y);
+                }
+                const float wi = __shfl_sync(0xffffffffu, w, i & 31);
+                float o[E];
+                if (i < kAhead) {
 #pragma unroll
-                for (int e = 0; e < E; e += 2) {
-                    const float2 o = __ldcg(reinterpret_cast<const float2*>(ws.o + at * D + lane * E + e));
-                    acc[e] = fmaf(w, o.x, acc[e]);
-                    acc[e + 1] = fmaf(w, o.y, acc[e + 1]);
+                    for (int k = 0; k < kAhead; ++k)
+                        if (k == i) {
+#pragma unroll
+                            for (int e = 0; e < E; ++e) o[e] = ahead[k][e];
+                        }
+                } else {
+                    outputs(i, o);
+                }
+                if (wi != 0.f) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] = fmaf(wi, o[e], acc[e]);
                 }
             }
         }
@@ -59,24 +94,23 @@ bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
 
-int paged_join_launch(const PagedParams& p, const PagedWorkspace& ws, int G, int rows, int dtype, cudaStream_t s) {
-    cudaLaunchConfig_t cfg{};
+int paged_join_launch(const PagedParams& p, const PagedWorkspace* ws, const int* rows, int count, int G, int dtype, cudaStream_t s) {
+    JoinSet set{};
+    int most = 0;
+    for (int i = 0; i < count; ++i) {
+        set.ws[i] = ws[i];
+        set.rows[i] = rows[i];
+        most = rows[i] > most ? rows[i] : most;
+    }
     // an item of many rows is shared by several blocks
-    cfg.gridDim = dim3(unsigned(G), unsigned(rows > 16 ? 8 : 1), 1);
-    cfg.blockDim = dim3(kJoinThreads, 1, 1);
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    const dim3 grid(unsigned(G), unsigned(most > 16 ? 16 : 2), unsigned(count));
     cudaError_t e;
     if (dtype == PARAS_BF16)
-        e = p.D == 128 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<__nv_bfloat16, 128>, p, ws, rows)
-                       : cudaLaunchKernelEx(&cfg, paged_join_kernel<__nv_bfloat16, 64>, p, ws, rows);
+        e = p.D == 128 ? paged_launch(paged_join_kernel<__nv_bfloat16, 128>, grid, kJoinThreads, 0, s, p, set)
+                       : paged_launch(paged_join_kernel<__nv_bfloat16, 64>, grid, kJoinThreads, 0, s, p, set);
     else
-        e = p.D == 128 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<__half, 128>, p, ws, rows)
-                       : cudaLaunchKernelEx(&cfg, paged_join_kernel<__half, 64>, p, ws, rows);
+        e = p.D == 128 ? paged_launch(paged_join_kernel<__half, 128>, grid, kJoinThreads, 0, s, p, set)
+                       : paged_launch(paged_join_kernel<__half, 64>, grid, kJoinThreads, 0, s, p, set);
     if (e != cudaSuccess) return fail(PARAS_E_CUDA, "paras paged_attention: launch of paged_join_kernel failed: %s", cudaGetErrorString(e));
     return PARAS_OK;
 }
@@ -96,23 +130,34 @@ bool paged_tma_ok(const paras_paged_cache& c) {
     return true;
 }
 
-int paged_cache_map(CUtensorMap* map, const paras_paged_cache& c, int which) {
+int paged_cache_map(CUtensorMap* map, const paras_paged_cache& c, int which, bool whole) {
     TensorMapEncodeFn fn = tensor_map_encode_fn();
     if (!fn) return fail(PARAS_E_CUDA, "paras_b200: cuTensorMapEncodeTiled is unavailable");
     const bool e8 = c.cache_dtype == PARAS_E4M3;
     const int64_t es = e8 ? 1 : 2;
     const int64_t* st = which ? c.v_strides : c.k_strides;
-    const cuuint64_t dims[4] = {cuuint64_t(c.D), cuuint64_t(c.page), cuuint64_t(c.Hkv), cuuint64_t(c.pages)};
     // the stride of a size-1 dim is never used for addressing; keep it a legal multiple of 16 bytes
     const int64_t s2 = c.page > 1 ? st[2] : c.D, s1 = c.Hkv > 1 ? st[1] : s2 * c.page, s0 = c.pages > 1 ? st[0] : s1 * c.Hkv;
-    const cuuint64_t strides[3] = {cuuint64_t(s2 * es), cuuint64_t(s1 * es), cuuint64_t(s0 * es)};
-    const cuuint32_t box[4] = {cuuint32_t(e8 ? c.D : 64), cuuint32_t(c.page < kTileKeys ? c.page : kTileKeys), 1, 1};
-    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const cuuint32_t rows = cuuint32_t(c.page < kTileKeys ? c.page : kTileKeys), inner = cuuint32_t(e8 ? c.D : 64), slabs = cuuint32_t(c.D) / inner;
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
     const CUtensorMapDataType dt = e8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                       : c.cache_dtype == PARAS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const CUresult r = fn(map, dt, 4, which ? c.v : c.k, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          e8 && c.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapSwizzle swizzle = e8 && c.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    void* base = which ? c.v : c.k;
+    CUresult r;
+    if (whole) {
+        const cuuint64_t dims[5] = {inner, cuuint64_t(c.page), slabs, cuuint64_t(c.Hkv), cuuint64_t(c.pages)};
+        const cuuint64_t strides[4] = {cuuint64_t(s2 * es), 128, cuuint64_t(s1 * es), cuuint64_t(s0 * es)};
+        const cuuint32_t box[5] = {inner, rows, slabs, 1, 1};
+        r = fn(map, dt, 5, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    } else {
+        const cuuint64_t dims[4] = {cuuint64_t(c.D), cuuint64_t(c.page), cuuint64_t(c.Hkv), cuuint64_t(c.pages)};
+        const cuuint64_t strides[3] = {cuuint64_t(s2 * es), cuuint64_t(s1 * es), cuuint64_t(s0 * es)};
+        const cuuint32_t box[4] = {inner, rows, 1, 1};
+        r = fn(map, dt, 4, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    }
     if (r != CUDA_SUCCESS) return fail(PARAS_E_CUDA, "paras_b200: cuTensorMapEncodeTiled failed with code %d", int(r));
     return PARAS_OK;
 }

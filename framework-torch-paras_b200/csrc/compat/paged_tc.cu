@@ -145,6 +145,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         tma_prefetch_desc(&map_v);
     }
     tc_fence_before_sync();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     int b0;
     int64_t base0;
     const PagedRange range = paged_range(p.B, reinterpret_cast<int64_t*>(gen + L::kSums),
@@ -853,8 +854,7 @@ int launch(int gpu, int G, cudaStream_t s, const CUtensorMap& mq, const CUtensor
            const PagedWorkspace& ws) {
     constexpr int bytes = Layout<E8>::kLaunch;
     PB_CUDA((paged_allow_smem<paged_tc_kernel<BF16, E8, HD>>(gpu, bytes)));
-    paged_tc_kernel<BF16, E8, HD><<<G, kThreads, bytes, s>>>(mq, mk, mv, p, ws);
-    PB_LAUNCH_CHECK("paged_tc_kernel");
+    PB_CUDA(paged_launch(paged_tc_kernel<BF16, E8, HD>, dim3(unsigned(G)), kThreads, bytes, s, mq, mk, mv, p, ws));
     return PARAS_OK;
 }
 
@@ -874,15 +874,14 @@ int paged_tc_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p
     if (st != PARAS_OK) return st;
     CUtensorMap mq, mk, mv;
     if ((st = paged_q_map(&mq, a, BM / p.group)) != PARAS_OK) return st;
-    if ((st = paged_cache_map(&mk, a.cache, 0)) != PARAS_OK) return st;
-    if ((st = paged_cache_map(&mv, a.cache, 1)) != PARAS_OK) return st;
+    if ((st = paged_cache_map(&mk, a.cache, 0, false)) != PARAS_OK) return st;
+    if ((st = paged_cache_map(&mv, a.cache, 1, false)) != PARAS_OK) return st;
     const bool bf = a.dtype == PARAS_BF16, e8 = a.cache.cache_dtype == PARAS_E4M3;
 #define PB_GO(B, E, H) launch<B, E, H>(g->ordinal, G, s, mq, mk, mv, p, ws)
     if (p.D == 128) st = bf ? (e8 ? PB_GO(true, true, 128) : PB_GO(true, false, 128)) : (e8 ? PB_GO(false, true, 128) : PB_GO(false, false, 128));
     else st = bf ? (e8 ? PB_GO(true, true, 64) : PB_GO(true, false, 64)) : (e8 ? PB_GO(false, true, 64) : PB_GO(false, false, 64));
 #undef PB_GO
-    if (st != PARAS_OK) return st;
-    return paged_join_launch(p, ws, G, 256, a.dtype, s);
+    return st;
 }
 
 }  // namespace pb

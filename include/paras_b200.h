@@ -458,7 +458,8 @@ typedef struct paras_paged_attn_args {
 } paras_paged_attn_args;
 int paras_b200_paged_attn(const paras_paged_attn_args* args);
 int paras_b200_paged_attn_workspace_bytes(const paras_paged_attn_args* args, size_t* bytes);
-/* Route of this thread's last successful paras_b200_paged_attn: "paged_simt", "paged_decode", "paged_tcgen05". */
+/* Route of this thread's last successful paras_b200_paged_attn: "paged_simt", "paged_decode" (few query rows per kv
+ * head), "paged_tcgen05", "paged_tcgen05+paged_decode" (a call that mixes chunks with single tokens). */
 const char* paras_b200_paged_attn_last_kernel(void);
 
 /* ---- residual addition and RMSNorm in one pass ----

@@ -29,7 +29,6 @@ using namespace tc;
 constexpr int kConsumers = 8;
 constexpr int threads_of(bool e8) { return (kConsumers + (e8 ? 3 : 2)) * 32; }
 constexpr int kRows = 16;
-constexpr int kMergeBytes = 16 * 1024;
 constexpr int kMaxStages = 8;
 constexpr int kMetaBytes = 48;
 
@@ -42,7 +41,11 @@ template <bool E8, int HD> struct Ring {
     static constexpr int kQ = 2 * kTile;                           // offset of the query rows
     static constexpr int kExp = kQ + (HD / 64) * kRows * 128;      // K's exponent bytes, then V's
     static constexpr int kBytes = kExp + (E8 ? 1024 : 0);          // a multiple of 1024
-    static constexpr int kStages = (208 * 1024) / kBytes < kMaxStages ? (208 * 1024) / kBytes : kMaxStages;
+    // Columns of the outputs that are merged at a time: 64, in 32 KB, or half that where three whole stages leave no more.
+    static constexpr int kMergeCols = E8 || HD == 64 ? 64 : 32;
+    static constexpr int kMergeBytes = kConsumers * kRows * kMergeCols * 4;
+    static constexpr int kFit = (224 * 1024 - kMergeBytes) / kBytes;
+    static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
     static constexpr int kMerge = kStages * kBytes;
     static constexpr int kMl = kMerge + kMergeBytes;               // [8][16] maxima, [8][16] sums
     static constexpr int kMeta = kMl + 2 * kConsumers * kRows * 4;
@@ -370,13 +373,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         float* l_sm = m_sm + kConsumers * kRows;
         uint32_t qf[HD / 16][4];
         float acc[HD / 8][4];
-        float m_run[2], l_run[2], c2[2];
+        float m_run[2], l_run[2];       // reference (in units of S) and sum of a row
+        float c2[2], lag[2];            // S * c2 is the exponent of 2; 2^8 in units of S
         int lim[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             m_run[h] = -INFINITY;
             l_run[h] = 0.f;
             c2[h] = p.scale_log2;
+            lag[h] = 8.f / p.scale_log2;
             lim[h] = 0;
         }
 #pragma unroll
@@ -441,6 +446,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             const int ex = max(-120, min(120, int(__float_as_uint(amax) >> 23) - 127));
                             const float f = pow2f(-ex);
                             c2[h] = p.scale_log2 * pow2f(ex);
+                            lag[h] = 8.f / c2[h];
 #pragma unroll
                             for (int ks = 0; ks < HD / 16; ++ks) {
                                 const float2 x = pair16_to_f32<true>(qf[ks][h]), y = pair16_to_f32<true>(qf[ks][2 + h]);
@@ -464,24 +470,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const int c = (x >> 1) * 4 + (lane >> 3);   // 16-byte unit of the row
                 ldsm4(kt + k_at[x & 1] + (E8 ? unit(krows[x & 1], c) : (c >> 3) * slab_step + unit(krows[x & 1], c & 7)), kf[x]);
             }
-            // ---- S = Q K^T: two n-tiles of 8 keys, even and odd steps summed apart ----
-            float sc[2][4], sd[2][4];
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sc[nt][e] = sd[nt][e] = 0.f;
+            // ---- S = Q K^T: two n-tiles of 8 keys ----
+            float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int x = 0; x < kLd; ++x) {
                 const int nt = x & 1, k = x >> 1;
                 if constexpr (!E8) {
                     mma<kBfOps>(sc[nt], qf[2 * k], kf[x][0], kf[x][1]);
-                    mma<kBfOps>(sd[nt], qf[2 * k + 1], kf[x][2], kf[x][3]);
+                    mma<kBfOps>(sc[nt], qf[2 * k + 1], kf[x][2], kf[x][3]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         uint32_t lo, hi;
                         e4m3x4_to_f16x4(kf[x][e], &lo, &hi);
-                        mma<false>((e & 1) ? sd[nt] : sc[nt], qf[4 * k + e], lo, hi);
+                        mma<false>(sc[nt], qf[4 * k + e], lo, hi);
                     }
                 }
             }
@@ -498,14 +500,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             uint32_t ev = E8 ? lds32(kt + R::kExp + 128 + first) : 0u;
             // 2^(byte - 127) of byte i (zero for a byte of 0, which no cache holds)
             auto scale_of = [](uint32_t w, int i) { return __uint_as_float(((w >> (8 * i)) & 0xffu) << 23); };
+            if constexpr (E8) {
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                const float k0 = E8 ? scale_of(ek, 2 * nt) : 1.f, k1 = E8 ? scale_of(ek, 2 * nt + 1) : 1.f;
+                for (int nt = 0; nt < 2; ++nt) {
+                    const float k0 = scale_of(ek, 2 * nt), k1 = scale_of(ek, 2 * nt + 1);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    // x = score * scale * log2 e
-                    sc[nt][2 * h] = (sc[nt][2 * h] + sd[nt][2 * h]) * (k0 * c2[h]);
-                    sc[nt][2 * h + 1] = (sc[nt][2 * h + 1] + sd[nt][2 * h + 1]) * (k1 * c2[h]);
+                    for (int h = 0; h < 2; ++h) {
+                        sc[nt][2 * h] *= k0;
+                        sc[nt][2 * h + 1] *= k1;
+                    }
                 }
             }
             // ---- mask, online softmax ----
@@ -522,30 +525,22 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         for (int e = 0; e < 2; ++e)
                             if (kb + nt * kStep + e >= lim[h] || !(nt ? here1 : here0)) sc[nt][2 * h + e] = -INFINITY;
             }
-            float pr[2][4], alpha[2];
-            bool moved = false;
+            // The reference m of a row lags behind its maximum: it moves when a score has outgrown it by 2^8 (P stays far
+            // inside 16 bits), which after an item's first tiles is rare, so that a tile usually needs no exchange between lanes.
+            float mx[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float m_new = fmaxf(m_run[h], mx);
-                alpha[h] = m_new == m_run[h] ? 1.f : ex2_approx(m_run[h] - m_new);
-                moved |= m_new != m_run[h];
-                const float ref = m_new == -INFINITY ? 0.f : m_new;
-                float sum = 0.f;
+            for (int h = 0; h < 2; ++h) mx[h] = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+            if (__any_sync(0xffffffffu, mx[0] > m_run[0] + lag[0] || mx[1] > m_run[1] + lag[1])) {
+                float alpha[2];
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float pv = ex2_approx(sc[nt][2 * h + e] - ref);
-                        pr[nt][2 * h + e] = pv;
-                        sum += pv;
-                    }
-                l_run[h] = l_run[h] * alpha[h] + sum;     // this thread's keys; the quad is added up at the end of the item
-                m_run[h] = m_new;
-            }
-            if (__any_sync(0xffffffffu, moved)) {
+                for (int h = 0; h < 2; ++h) {
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                    const float m_new = fmaxf(m_run[h], mx[h]);
+                    alpha[h] = m_new == m_run[h] ? 1.f : ex2_approx((m_run[h] - m_new) * c2[h]);
+                    l_run[h] *= alpha[h];
+                    m_run[h] = m_new;
+                }
 #pragma unroll
                 for (int x = 0; x < HD / 8; ++x) {
                     acc[x][0] *= alpha[0];
@@ -553,6 +548,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     acc[x][2] *= alpha[1];
                     acc[x][3] *= alpha[1];
                 }
+            }
+            float pr[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float neg = m_run[h] == -INFINITY ? 0.f : -m_run[h] * c2[h];     // (no key yet: every P is 0)
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float pv = ex2_approx(fmaf(sc[nt][2 * h + e], c2[h], neg));
+                        pr[nt][2 * h + e] = pv;
+                        l_run[h] += pv;      // of this thread's keys; the quad is added up at the end of the item
+                    }
             }
             // ---- O += P V ----
             if (key0 + kTileKeys > kend) {
@@ -617,7 +625,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (t == 0) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        m_sm[warp * kRows + r0 + 8 * h] = m_run[h];
+                        m_sm[warp * kRows + r0 + 8 * h] = m_run[h] * c2[h];      // (exponents of 2 from here on)
                         l_sm[warp * kRows + r0 + 8 * h] = l_run[h];
                     }
                 }
@@ -628,52 +636,67 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     float M = -INFINITY;
 #pragma unroll
                     for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, m_sm[w * kRows + r0 + 8 * h]);
-                    f[h] = m_run[h] == -INFINITY ? 0.f : ex2_approx(m_run[h] - M);
+                    f[h] = m_run[h] == -INFINITY ? 0.f : ex2_approx(m_run[h] * c2[h] - M);
                 }
-                // 32 columns at a time: [warp][row][32] fp32
+                // Sixteen threads finish a row; its maximum and sum are found once.
+                constexpr int kCols = R::kMergeCols, kMine = kCols / 16;
+                const int r = threadIdx.x >> 4, cp = threadIdx.x & 15;
+                float M = -INFINITY, l = 0.f;
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
+                for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, m_sm[w * kRows + r]);
+#pragma unroll
+                for (int w = 0; w < kConsumers; ++w) {
+                    const float mw = m_sm[w * kRows + r];
+                    if (mw != -INFINITY) l = fmaf(l_sm[w * kRows + r], ex2_approx(mw - M), l);
+                }
+                const float inv = M == -INFINITY ? 0.f : 1.0f / l;
+                const int tok = row_tok + r / p.group, hq = hk * p.group + r % p.group;
+                const size_t at = size_t(slot) * kRows + r;
+                uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.os[0] + int64_t(hq) * p.os[1];
+                if (r < rows && cp == 0) {
+                    if (flags & 4) ws.ml[at] = make_float2(M, l);
+                    else if (p.lse) p.lse[int64_t(tok) * p.Hq + hq] = M == -INFINITY ? -INFINITY : M * 0.6931471805599453f + logf(l);
+                }
+                // [warp][row][kCols] fp32, groups of 8 columns exchanged by row so that the rows lie on different banks
+#pragma unroll
+                for (int c = 0; c < HD / kCols; ++c) {
                     if (c > 0) merge_sync();
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int r = r0 + 8 * h;
-                        if (r < rows) {
-                            float* dst = merge + (warp * kRows + r) * 32;
+                        const int rr = r0 + 8 * h;
+                        if (rr < rows) {
+                            float* dst = merge + (warp * kRows + rr) * kCols;
 #pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                *reinterpret_cast<float2*>(dst + 8 * x + 2 * t) =
-                                    make_float2(acc[4 * c + x][2 * h] * f[h], acc[4 * c + x][2 * h + 1] * f[h]);
+                            for (int x = 0; x < kCols / 8; ++x)
+                                *reinterpret_cast<float2*>(dst + 8 * (x ^ (rr & (kCols / 8 - 1))) + 2 * t) =
+                                    make_float2(acc[c * (kCols / 8) + x][2 * h] * f[h], acc[c * (kCols / 8) + x][2 * h + 1] * f[h]);
                         }
                     }
                     merge_sync();
-                    // 16 rows x 16 column pairs: a pair per thread
-                    const int r = threadIdx.x >> 4, cp = threadIdx.x & 15;
                     if (r < rows) {
-                        float M = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+                        float o[kMine];
 #pragma unroll
-                        for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, m_sm[w * kRows + r]);
+                        for (int e = 0; e < kMine; ++e) o[e] = 0.f;
+                        const int col = kMine * cp;
+                        const float* src = merge + r * kCols + 8 * ((col >> 3) ^ (r & (kCols / 8 - 1))) + (col & 7);
 #pragma unroll
-                        for (int w = 0; w < kConsumers; ++w) {
-                            const float mw = m_sm[w * kRows + r];
-                            if (mw != -INFINITY) l = fmaf(l_sm[w * kRows + r], ex2_approx(mw - M), l);
-                            const float2 v = *reinterpret_cast<const float2*>(merge + (w * kRows + r) * 32 + 2 * cp);
-                            o0 += v.x;
-                            o1 += v.y;
-                        }
-                        const int d = 32 * c + 2 * cp;
-                        if (flags & 4) {
-                            const size_t at = size_t(slot) * kRows + r;
-                            *reinterpret_cast<float2*>(ws.o + at * HD + d) = make_float2(o0, o1);
-                            if (d == 0) ws.ml[at] = make_float2(M, l);
-                        } else {
-                            const int tok = row_tok + r / p.group, h = hk * p.group + r % p.group;
-                            const float inv = M == -INFINITY ? 0.f : 1.0f / l;
-                            uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.os[0] + int64_t(h) * p.os[1] + d;
-                            const uint32_t w = pack16<BF16>(o0 * inv, o1 * inv);
-                            out[0] = uint16_t(w);
-                            out[1] = uint16_t(w >> 16);
-                            if (p.lse && d == 0)
-                                p.lse[int64_t(tok) * p.Hq + h] = M == -INFINITY ? -INFINITY : M * 0.6931471805599453f + logf(l);
+                        for (int w = 0; w < kConsumers; ++w)
+#pragma unroll
+                            for (int e = 0; e < kMine; e += 2) {
+                                const float2 v = *reinterpret_cast<const float2*>(src + w * kRows * kCols + e);
+                                o[e] += v.x;
+                                o[e + 1] += v.y;
+                            }
+#pragma unroll
+                        for (int e = 0; e < kMine; e += 2) {
+                            const int d = c * kCols + col + e;
+                            if (flags & 4) {
+                                *reinterpret_cast<float2*>(ws.o + at * HD + d) = make_float2(o[e], o[e + 1]);
+                            } else {
+                                const uint32_t w = pack16<BF16>(o[e] * inv, o[e + 1] * inv);
+                                out[d] = uint16_t(w);
+                                out[d + 1] = uint16_t(w >> 16);
+                            }
                         }
                     }
                 }
@@ -704,7 +727,7 @@ int paged_decode_rows() { return kRows; }
 
 bool paged_decode_supported(const Gpu* g, const paras_paged_attn_args& a) {
     return g->cc_major >= 9 && a.dtype != PARAS_F32 && paged_tma_ok(a.cache) && paged_q_tma_ok(a) &&
-           a.Hq / a.cache.Hkv <= kRows && g->smem_optin >= 227 * 1024;
+           a.Hq / a.cache.Hkv <= kRows && a.scale > 0.0 && g->smem_optin >= 227 * 1024;
 }
 
 int paged_decode_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p, const PagedWorkspace& ws, int G, cudaStream_t s) {

@@ -223,7 +223,7 @@ int paras_b200_paged_attn(const paras_paged_attn_args* args) {
         ws[count] = pb::paged_carve(scratch, G, rows[count]);
         st = pb::paged_decode_launch(g, a, pd, ws[count++], G, s);
     }
-    if (st == PARAS_OK) st = pb::paged_join_launch(p, ws, rows, count, G, a.dtype, s);
+    if (st == PARAS_OK) st = pb::paged_join_launch(g, p, ws, rows, count, G, a.dtype, s);
     if (st == PARAS_OK) pb::tl_paged_kernel = r.tc ? (r.decode ? "paged_tcgen05+paged_decode" : "paged_tcgen05") : "paged_decode";
     if (!a.workspace) {
         const int st2 = paras_b200_free_async(a.gpu, scratch, s);

@@ -186,7 +186,8 @@ cudaError_t paged_allow_smem(int gpu, int bytes) {
 
 // Joins the partial results that up to two streaming launches (of G CTAs, items of rows[i] query rows) left of their cut
 // items: one launch after them on the same stream.
-int paged_join_launch(const PagedParams& p, const PagedWorkspace* ws, const int* rows, int count, int G, int dtype, cudaStream_t s);
+int paged_join_launch(const Gpu* g, const PagedParams& p, const PagedWorkspace* ws, const int* rows, int count, int G, int dtype,
+                      cudaStream_t s);
 
 // Launches `kernel` so that its start may overlap the end of the kernel before it, for whose memory it waits itself
 // (griddepcontrol.wait).

@@ -8,6 +8,10 @@
 // Sixteen lanes take a row, eight elements each (16 bytes of a 16-bit row), the other half of the warp the matching row
 // of V: a 128-element head is one load a lane, the row's maximum four shuffles.  Which sequence a token belongs to is
 // found by the warp (warp_count_le) while the row's loads are in flight.
+//
+// Measured (8 kv heads of 128, pages of 64): write of 4 x 4096 tokens 21.1 us as bf16 (5.9 TB/s), 19.1 us into 8 bits
+// (4.9 TB/s; bound by instructions before the rows stayed in pairs of 16 bits: 25.3 us); one token for each of 64
+// sequences 2.6 us; read of 16 sequences of up to 8192 from 8 bits 61.4 us (5.8 TB/s), of one of 1500 as bf16 5.0 us.
 #include "paged_common.cuh"
 
 namespace pb {
@@ -72,11 +76,112 @@ __device__ __forceinline__ void unpack8(uint2 w, float s, float (&f)[8]) {
         f[4 * i + 3] = b.y * s;
     }
 }
-__device__ __forceinline__ uint2 pack8(const float (&f)[8], float s) {
-    uint2 w;
-    w.x = pack_e4m3(f[0] * s, f[1] * s) | (pack_e4m3(f[2] * s, f[3] * s) << 16);
-    w.y = pack_e4m3(f[4] * s, f[5] * s) | (pack_e4m3(f[6] * s, f[7] * s) << 16);
-    return w;
+// Eight elements of a row as the writer holds them: their largest magnitude and their 8-bit form.  16-bit elements stay in
+// pairs: magnitudes and maxima are taken two at a time, and the product by a power of two is exact there too (an fp16 value
+// that becomes subnormal is far below half of e4m3's smallest and rounds to zero by either way).
+template <typename T>
+struct Lane8 {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const T* p) { *reinterpret_cast<uint4*>(w) = __ldcs(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0u; }
+    __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(w)); }
+};
+template <>
+struct Lane8<float> {
+    float f[8];
+    __device__ __forceinline__ void load(const float* p) { load_row<float, 8>(p, f); }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = 0.f;
+    }
+    __device__ __forceinline__ void store(float* p) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) __stcs(reinterpret_cast<float4*>(p) + i, make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]));
+    }
+};
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+    using V = __half2;
+    static __device__ __forceinline__ float value(uint32_t h) { return __half2float(__ushort_as_half(uint16_t(h))); }
+    static __device__ __forceinline__ uint32_t scaled(uint32_t w, int e) {       // two e4m3 of w * 2^e, -7 <= e <= 15
+        const uint32_t s = uint32_t(e + 15) * 0x04000400u;
+        const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&s));
+        uint16_t r;
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
+        return r;
+    }
+};
+template <> struct Pair<__nv_bfloat16> {
+    using V = __nv_bfloat162;
+    static __device__ __forceinline__ float value(uint32_t h) { return __uint_as_float(h << 16); }
+    static __device__ __forceinline__ uint32_t scaled(uint32_t w, int e) {
+        const uint32_t s = uint32_t(e + 127) * 0x00800080u;
+        const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&s));
+        const uint32_t b = *reinterpret_cast<const uint32_t*>(&v);
+        return pack_e4m3(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
+    }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    using V = typename Pair<T>::V;
+    const V r = __hmax2(*reinterpret_cast<const V*>(&a), *reinterpret_cast<const V*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <typename T>
+__device__ __forceinline__ uint2 pack8(const Lane8<T>& v, int e) {
+    uint2 r;
+    if constexpr (sizeof(T) == 4) {
+        const float s = pow2f(e);
+        r.x = pack_e4m3(v.f[0] * s, v.f[1] * s) | (pack_e4m3(v.f[2] * s, v.f[3] * s) << 16);
+        r.y = pack_e4m3(v.f[4] * s, v.f[5] * s) | (pack_e4m3(v.f[6] * s, v.f[7] * s) << 16);
+    } else {
+        r.x = __byte_perm(Pair<T>::scaled(v.w[0], e), Pair<T>::scaled(v.w[1], e), 0x5410);
+        r.y = __byte_perm(Pair<T>::scaled(v.w[2], e), Pair<T>::scaled(v.w[3], e), 0x5410);
+    }
+    return r;
+}
+// The exponent of row (lane mod ROWS) of the half-warp's ROWS rows.  Maxima skip NaN.
+template <typename T, int ROWS>
+__device__ __forceinline__ int row_exponents(const Lane8<T> (&v)[ROWS]) {
+    const int lane = int(threadIdx.x) & 31;
+    float mine = 0.f;
+    if constexpr (sizeof(T) == 4) {
+        float amax[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            amax[r] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax[r] = fmaxf(amax[r], fabsf(v[r].f[e]));
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) amax[r] = fmaxf(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], o));
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) mine = (lane & (ROWS - 1)) == r ? amax[r] : mine;
+    } else {
+        constexpr int kPairs = (ROWS + 1) / 2;
+        constexpr uint32_t kAbs = 0x7fff7fffu;
+        uint32_t m[2 * kPairs], both[kPairs];        // two rows' maxima in a word
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            m[r] = max2<T>(max2<T>(v[r].w[0] & kAbs, v[r].w[1] & kAbs), max2<T>(v[r].w[2] & kAbs, v[r].w[3] & kAbs));
+        if constexpr (ROWS & 1) m[ROWS] = m[ROWS - 1];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            both[i] = max2<T>(__byte_perm(m[2 * i], m[2 * i + 1], 0x5410), __byte_perm(m[2 * i], m[2 * i + 1], 0x7632));
+            both[i] = max2<T>(both[i], 0u);          // nothing but NaN counts as zeros
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) both[i] = max2<T>(both[i], __shfl_xor_sync(0xffffffffu, both[i], o));
+        uint32_t w = both[0];
+#pragma unroll
+        for (int i = 1; i < kPairs; ++i) w = (lane & (ROWS - 1)) >> 1 == i ? both[i] : w;
+        mine = Pair<T>::value(lane & 1 ? w >> 16 : w & 0xffffu);
+    }
+    return row_exponent(mine);
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
@@ -124,40 +229,37 @@ paged_kv_write_kernel(const KvParams p) {
     if (unit >= int64_t(p.T) * groups) return;
     const int t = int(unit / groups), h0 = int(unit - int64_t(t) * groups) * ROWS;
     const RowMap<T> m(p, half, t);
-    float f[ROWS][8];
+    const int heads = min(ROWS, p.Hkv - h0);
+    Lane8<T> v[ROWS];
+    const T* row = m.row + int64_t(h0) * m.row_head + d;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[r][e] = 0.f;
-        if (d < p.D && h0 + r < p.Hkv) load_row<T, 8>(m.row + int64_t(h0 + r) * m.row_head + d, f[r]);
+        v[r].clear();
+        if (d < p.D && r < heads) v[r].load(row);
+        row += m.row_head;
     }
     int page = 0, off = 0, b = 0;
     if (!locate<true>(p, t, &page, &off, &b) || uint32_t(page) >= uint32_t(p.pages)) return;
-    const int64_t at = int64_t(page) * m.cache_page + int64_t(off) * m.cache_off + d;
+    const int64_t at = int64_t(page) * m.cache_page + int64_t(off) * m.cache_off + int64_t(h0) * m.cache_head + d;
     if constexpr (CACHE8) {
-        float amax[ROWS];    // (fmaxf skips NaN)
+        static_assert((ROWS & (ROWS - 1)) == 0 && ROWS <= 16, "a lane per row's exponent");
+        const int ex = row_exponents<T, ROWS>(v), r = lane & 15;
+        if (r < ROWS && r < heads)
+            m.exps[int64_t(page) * m.exp_page + int64_t(h0 + r) * m.exp_head + int64_t(off) * m.exp_off] = uint8_t(ex + 127);
+        char* to = m.cache + at;
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            amax[r] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) amax[r] = fmaxf(amax[r], fabsf(f[r][e]));
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1)
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) amax[r] = fmaxf(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], o));
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            const int h = h0 + r;
-            if (h >= p.Hkv) break;
-            const int ex = row_exponent(amax[r]);
-            if (d < p.D) *reinterpret_cast<uint2*>(m.cache + at + int64_t(h) * m.cache_head) = pack8(f[r], pow2f(-ex));
-            if (d == 0) m.exps[int64_t(page) * m.exp_page + int64_t(h) * m.exp_head + int64_t(off) * m.exp_off] = uint8_t(ex + 127);
+        for (int i = 0; i < ROWS; ++i) {
+            const int e = __shfl_sync(0xffffffffu, ex, i, 16);
+            if (d < p.D && i < heads) *reinterpret_cast<uint2*>(to) = pack8<T>(v[i], -e);
+            to += m.cache_head;
         }
     } else {
+        T* to = reinterpret_cast<T*>(m.cache) + at;
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-            if (d < p.D && h0 + r < p.Hkv) store8(reinterpret_cast<T*>(m.cache) + at + int64_t(h0 + r) * m.cache_head, f[r]);
+        for (int r = 0; r < ROWS; ++r) {
+            if (d < p.D && r < heads) v[r].store(to);
+            to += m.cache_head;
+        }
     }
 }
 
@@ -262,7 +364,9 @@ void launch(const KvParams& p, bool vec, int sms, cudaStream_t s) {
     auto go = [&](auto kernel, int64_t warps) { kernel<<<unsigned((warps + kWarps - 1) / kWarps), kWarps * 32, 0, s>>>(p); };
     if (!vec) return go(paged_kv_any_kernel<T, CACHE8, WRITE>, rows);
     // Several heads a warp once there are rows enough for every warp slot of the GPU: the look-up of the token's place is
-    // shared and more loads are in flight; below that, a warp per row keeps the chain short.
+    // shared and more loads are in flight; below that, a warp per row keeps the chain short.  4 x 4096 bf16 tokens of 8 heads
+    // into an 8-bit cache: 19.1 us with four heads a warp, 26.0 with two, 19.0 with eight (which costs short rows more:
+    // 4 x 2048 of 4 heads of 64 take 6.0, 8.0, 7.2 us).
     constexpr int kMany = WRITE ? 4 : 8;
     const bool many = p.Hkv > 1 && rows >= int64_t(sms) * 64 * 2;
     const int64_t warps = many ? int64_t(p.T) * ((p.Hkv + kMany - 1) / kMany) : rows;

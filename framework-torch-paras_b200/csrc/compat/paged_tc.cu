@@ -6,9 +6,11 @@
 //   warps 0-3, 4-7  softmax of query tile 0 / 1, a thread per row, the whole S row in registers
 //   warp  8         one lane issues every tcgen05.mma
 //   warp  9         finds the items, loads Q (TMA), and K / V of a 16-bit cache: a TMA box per page
-//   warps 10-11     16-bit cache: zero what a page holds past the end of its sequence (0 * NaN must not reach O);
-//                   8-bit cache: bring e4m3 rows to fp16 (cp.async into a staging tile, exact conversion, 2^e of the row
-//                   multiplied in), a tile ahead of the MMAs
+//   warps 10-11     16-bit cache: zero what a page holds past the end of its sequence (0 * NaN must not reach O)
+//   warps 10-13     8-bit cache: bring e4m3 rows to fp16 (cp.async into a staging tile, exact conversion, 2^e of the row
+//                   multiplied in), a tile ahead of the MMAs; with two warps for this, 2 x 2048 tokens over 6000-8192
+//                   positions took 594 us, with four 553 (430 and 369 with heads of 64), and 330 from a 16-bit cache:
+//                   the conversion shares the issue slots with the softmax.  (14 and 15 only fill their warpgroup.)
 // What differs: the query heads of a GQA group always share a tile (rows = (token, head), floor(128 / group) tokens of a
 // tile, by a 4-D box on q), so that K and V are read once per group whatever the lengths; tiles are shared out over the
 // CTAs as paged_attn.cuh describes, cut items leaving fp32 partial outputs; the lengths are read on the device, and the
@@ -35,7 +37,6 @@ constexpr int kChunkBytes = 64 * 2 * 128;    // 64 elements x 128 rows
 constexpr int kTileBytes = 2 * kChunkBytes;
 constexpr int kPairBytes = 2 * kTileBytes;   // V_j, then K_j+1
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kHelpWarp = 10;
-constexpr int kThreads = 384;
 constexpr int kItems = 4;                     // descriptors in flight
 constexpr float kRescaleSum = 256.0f, kRedoSum = 32768.0f;
 constexpr int kColS = 0, kColO = 256;
@@ -48,20 +49,24 @@ constexpr int kBarQFull = 0, kBarQEmpty = 2, kBarKVFull = 4, kBarKVEmpty = 6, kB
               kNumBars = kBarItemEmpty + kItems;
 
 template <bool E8> struct Layout {
+    static constexpr int kConv = E8 ? 4 : 0;                           // warps that convert, a quarter of a tile's rows each
+    static constexpr int kThreads = E8 ? 512 : 384;
+    static constexpr int kAtLaunch = E8 ? 128 : 168;                   // registers per thread
     static constexpr int kORow = E8 ? 64 : 128;                        // bytes a row of the output staging holds
     static constexpr int kOStage = 32 * kORow;
-    static constexpr int kRaw = kSmemO + 8 * kOStage;                  // 8-bit: a tile of e4m3 rows, 64 rows per warp
-    static constexpr int kScale = kRaw + (E8 ? 16 * 1024 : 0);         // 8-bit: 2^e of the rows, fp16 twice, [2 warps][64]
+    static constexpr int kRaw = kSmemO + 8 * kOStage;                  // 8-bit: a tile of e4m3 rows
+    static constexpr int kScale = kRaw + (E8 ? 16 * 1024 : 0);         // 8-bit: 2^e of the rows, fp16 twice
     static constexpr int kItem = kScale + (E8 ? 512 : 0);
     static constexpr int kBits = kItem + kItems * 64;                  // pages that are there, of the last four tiles
     static constexpr int kSums = kBits + 16;
     static constexpr int kBars = kSums + (kThreads / 32 + 3) * 8 + 8;
     static constexpr int kMisc = kBars + kNumBars * 8;
     static constexpr int kLaunch = kMisc + 16 + 1024;
-    // Registers per thread after setmaxnreg, of 168 at launch: their sum, 256 * 200 + 128 * 96 = 63488, stays below what
-    // the CTA was launched with, 384 * 168 = 64512.  (A softmax thread with 192 spills a third of its row.)
-    static constexpr int kRegsSoftmax = 200, kRegsOther = 96;
-    static_assert(256 * kRegsSoftmax + 128 * kRegsOther < 384 * 168, "register split");
+    // Registers per thread after setmaxnreg, which come to no more than what the CTA was launched with: 256 * 200 + 128 * 96
+    // = 63488 of 384 * 168 = 64512; 8-bit: 256 * 200 + 256 * 56 = 65536 of 512 * 128.  (A softmax thread with 192 spills a
+    // third of its row.)
+    static constexpr int kRegsSoftmax = 200, kRegsOther = E8 ? 56 : 96;
+    static_assert(256 * kRegsSoftmax + (kThreads - 256) * kRegsOther <= kThreads * kAtLaunch, "register split");
     static_assert(kLaunch <= 227 * 1024, "shared memory of a CTA");
     static_assert(kItem % 16 == 0 && kSums % 8 == 0 && kBars % 8 == 0, "alignment");
 };
@@ -104,7 +109,7 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 }
 
 template <bool BF16, bool E8, int HD>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Layout<E8>::kThreads, 1)
 paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const PagedParams p, const PagedWorkspace ws) {
     using L = Layout<E8>;
@@ -124,16 +129,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNumBars; ++i) {
             int n = 1;                                                                   // a commit, a TMA, the loading warp
-            if (i >= kBarKVFull && i < kBarKVFull + 2) n = E8 ? 4 : 2;                   // entries of a pair (by two warps)
+            if (i >= kBarKVFull && i < kBarKVFull + 2) n = E8 ? 2 * L::kConv : 2;        // entries of a pair (by four warps)
             else if ((i >= kBarPFull && i < kBarPFull + 2) || i == kBarQConv || i == kBarQConv + 1) n = 4;   // softmax warps
-            else if (i >= kBarItemEmpty) n = 11;                                         // MMA, softmax and helping warps
+            else if (i >= kBarItemEmpty) n = 1 + 8 + (E8 ? L::kConv : 2);                // MMA, softmax, converting or helping warps
             mbar_init(bar(i), n);
         }
         *abort_flag = 0;
         mbar_fence_init();
     }
     // rows that no token fills (128 is not a multiple of the group) stay zero
-    for (int i = threadIdx.x; i < 2 * kTileBytes / 16; i += kThreads) st_shared_v4(base + kSmemQ + i * 16, make_uint4(0, 0, 0, 0));
+    for (int i = threadIdx.x; i < 2 * kTileBytes / 16; i += L::kThreads) st_shared_v4(base + kSmemQ + i * 16, make_uint4(0, 0, 0, 0));
     fence_proxy_async_smem();
     if (warp == kMmaWarp) {
         tmem_alloc(base + L::kMisc, 512);
@@ -433,13 +438,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(kBarKVFull + slot));
             }
-        } else {
+        } else if (warp < kHelpWarp + L::kConv) {
             // ------------------------------ e4m3 rows to fp16 ------------------------------
-            // Each of the two warps brings 64 of a tile's rows; HD / 16 lanes take a row, 16 bytes each.  The rows of the
+            // Each of the four warps brings 32 of a tile's rows; HD / 16 lanes take a row, 16 bytes each.  The rows of the
             // next entry are on their way into the staging tile while this one is converted, unit by unit in the same place.
-            constexpr int kPer = HD / 16, kUnits = 64 * kPer / 32;    // lanes of a row, units of a lane
+            constexpr int kPer = HD / 16, kUnits = kPer;              // lanes of a row, units of a lane (32 / kPer rows each)
             const int w = warp - kHelpWarp;
-            const uint32_t raw = base + L::kRaw + w * 8192, scales = base + L::kScale + w * 256;
+            const uint32_t raw = base + L::kRaw + w * 4096, scales = base + L::kScale + w * 128;
             int r = 0;
             // Entry x of an item: K_0, then V_j (odd x), K_j+1 (even x): kv tile x / 2.
             struct Part { int b, hk, kv0, n, kfin; };      // what this role needs of an item
@@ -451,42 +456,38 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 drop_item(i);
                 return true;
             };
-            // lane l looks after the warp's rows 2l and 2l+1: their page, ...
+            // lane l looks after the warp's row l: its page, ...
             auto page_for = [&](const Part& it, int x) -> int {
-                const int t = it.kv0 + (x >> 1), key = w * 64 + 2 * lane;
+                const int t = it.kv0 + (x >> 1), key = w * 32 + lane;
                 if (t * BN + key >= it.kfin) return -1;
                 const int pg = __ldg(p.table + int64_t(it.b) * p.table_stride + (p.tpp > 1 ? t / p.tpp : t * npg + (key >> p.box_shift)));
                 return uint32_t(pg) < uint32_t(p.pages) ? pg : -1;
             };
             auto row_in_page = [&](const Part& it, int x) -> int {
-                const int t = it.kv0 + (x >> 1), key = w * 64 + 2 * lane;
+                const int t = it.kv0 + (x >> 1), key = w * 32 + lane;
                 return (p.tpp > 1 ? (t % p.tpp) * BN : 0) + (key & ((1 << p.box_shift) - 1));
             };
-            // ... their exponent bytes (127 where there is no row), ...
+            // ... its exponent byte (127 where there is no row), ...
             auto exps_for = [&](const Part& it, int x, int pg) -> uint32_t {
-                if (pg < 0) return 0x7f7fu;
+                if (pg < 0) return 127u;
                 const bool v = x & 1;      // (selected one by one: a pointer into the parameters would copy them to local memory)
-                const int64_t st = v ? p.evs[2] : p.eks[2];
-                const uint8_t* e = (v ? p.ev : p.ek) + int64_t(pg) * (v ? p.evs[0] : p.eks[0]) + int64_t(it.hk) * (v ? p.evs[1] : p.eks[1]) +
-                                   int64_t(row_in_page(it, x)) * st;
-                return uint32_t(__ldg(e)) | (uint32_t(__ldg(e + st)) << 8);    // (a page holds whole pairs)
+                return __ldg((v ? p.ev : p.ek) + int64_t(pg) * (v ? p.evs[0] : p.eks[0]) + int64_t(it.hk) * (v ? p.evs[1] : p.eks[1]) +
+                             int64_t(row_in_page(it, x)) * (v ? p.evs[2] : p.eks[2]));
             };
-            // ... and where they lie: the address of row 2l, with the number of the two that exist in its low bits
+            // ... and where it lies; the low bit says that there is such a row
             auto rows_for = [&](const Part& it, int x, int pg) -> uint64_t {
                 const bool v = x & 1;
                 const char* src = v ? p.cv : p.ck;
                 if (pg < 0) return reinterpret_cast<uint64_t>(src);
-                const int live = min(2, it.kfin - ((it.kv0 + (x >> 1)) * BN + w * 64 + 2 * lane));
                 return reinterpret_cast<uint64_t>(src + int64_t(pg) * (v ? p.cvs[0] : p.cks[0]) + int64_t(it.hk) * (v ? p.cvs[1] : p.cks[1]) +
-                                                  int64_t(row_in_page(it, x)) * (v ? p.cvs[2] : p.cks[2])) | uint64_t(live);
+                                                  int64_t(row_in_page(it, x)) * (v ? p.cvs[2] : p.cks[2])) | 1u;
             };
             const int my_row = lane / kPer, my_c = lane % kPer;       // of a unit's 32 / kPer rows
-            // asks for unit u (rows u * 32 / kPer ..): `rows` as rows_for gave it, `pitch` the next row's distance
-            auto fetch = [&](uint64_t rows, int64_t pitch, int u) {
-                const int row = u * (32 / kPer) + my_row;
-                const uint64_t at = __shfl_sync(0xffffffffu, rows, row >> 1);
-                const bool live = (row & 1) < int(at & 3);
-                const uint64_t src = (at & ~uint64_t(15)) + (live ? uint64_t((row & 1) * pitch + my_c * 16) : 0);
+            // asks for unit u (rows u * 32 / kPer ..): `rows` as rows_for gave it
+            auto fetch = [&](uint64_t rows, int u) {
+                const uint64_t at = __shfl_sync(0xffffffffu, rows, u * (32 / kPer) + my_row);
+                const bool live = at & 1u;
+                const uint64_t src = (at & ~uint64_t(15)) + (live ? my_c * 16 : 0);
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + u * 512 + lane * 16), "l"(src), "r"(live ? 16 : 0)
                              : "memory");
             };
@@ -494,12 +495,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             bool more = get_part(0, &it), ok = true;
             uint32_t seq = 0;
             int pg = -1;
-            uint32_t ex = 0x7f7fu;
+            uint32_t ex = 127u;
             if (more) {
                 pg = page_for(it, 0);
                 ex = exps_for(it, 0, pg);
                 const uint64_t rows = rows_for(it, 0, pg);
-                for (int u = 0; u < kUnits; ++u) fetch(rows, p.cks[2], u);
+                for (int u = 0; u < kUnits; ++u) fetch(rows, u);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             while (ok && more) {
@@ -515,9 +516,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     }
                     const bool go = !have_next || next_more;
                     int pg2 = -1;
-                    uint32_t ex2 = 0x7f7fu;
+                    uint32_t ex2 = 127u;
                     uint64_t rows2 = 0;
-                    const int64_t pitch2 = (nxx & 1) ? p.cvs[2] : p.cks[2];
                     if (go) {
                         pg2 = (nxx & 1) ? pg : page_for(nx, nxx);      // V_j lies where K_j does
                         rows2 = rows_for(nx, nxx, pg2);
@@ -530,33 +530,32 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         if (r == 0 && lane == 0) mbar_arrive(bar(kBarKVFull + slot));
                     }
                     if (!(x & 1)) {
-                        // bit i: page i of the tile is there, from both warps' rows
-                        const int mine = __shfl_sync(0xffffffffu, pg, ((lane << p.box_shift) >> 1) & 31);
-                        const uint32_t there = __ballot_sync(0xffffffffu, lane < max(1, 64 >> p.box_shift) && mine >= 0);
-                        if (lane == 0) reinterpret_cast<volatile uint16_t*>(gen + L::kBits)[2 * (g & 3) + w] = uint16_t(there);
+                        // bit i: page i of the tile is there, from the warp that has its first row
+                        const int key = lane << p.box_shift, mine = __shfl_sync(0xffffffffu, pg, key & 31);
+                        const uint32_t there = __ballot_sync(0xffffffffu, lane < npg && key >> 5 == w && mine >= 0);
+                        if (lane == 0) reinterpret_cast<volatile uint8_t*>(gen + L::kBits)[4 * (g & 3) + w] = uint8_t(there >> ((w * 32) >> p.box_shift));
                     }
-                    // 2^e of this lane's two rows, fp16 twice
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int e = max(kExpLo, min(kExpHi, int((ex >> (8 * h)) & 0xffu) - 127));
+                    // 2^e of this lane's row, fp16 twice
+                    {
+                        const int e = max(kExpLo, min(kExpHi, int(ex) - 127));
                         const uint32_t f = e >= -14 ? uint32_t(e + 15) << 10 : 0x200u;
-                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(scales + (2 * lane + h) * 4), "r"(f | (f << 16)) : "memory");
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(scales + lane * 4), "r"(f | (f << 16)) : "memory");
                     }
                     asm volatile("cp.async.wait_group 0;" ::: "memory");
                     __syncwarp();
                     const uint32_t dst = base + kSmemKV + slot * kPairBytes + ((x & 1) ? 0 : kTileBytes);
-                    // four units at a time: their loads side by side, then their conversions
+                    // two units at a time: their loads side by side, then their conversions
 #pragma unroll 1
-                    for (int u4 = 0; u4 < kUnits; u4 += 4) {
-                        uint4 v[4];
-                        uint32_t sc[4];
+                    for (int u2 = 0; u2 < kUnits; u2 += 2) {
+                        uint4 v[2];
+                        uint32_t sc[2];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            v[y] = lds128(raw + (u4 + y) * 512 + lane * 16);
-                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sc[y]) : "r"(scales + ((u4 + y) * (32 / kPer) + my_row) * 4));
+                        for (int y = 0; y < 2; ++y) {
+                            v[y] = lds128(raw + (u2 + y) * 512 + lane * 16);
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sc[y]) : "r"(scales + ((u2 + y) * (32 / kPer) + my_row) * 4));
                         }
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
+                        for (int y = 0; y < 2; ++y) {
                             const __half2 s2 = *reinterpret_cast<const __half2*>(&sc[y]);
                             const uint32_t in[4] = {v[y].x, v[y].y, v[y].z, v[y].w};
                             uint32_t o[8];
@@ -570,7 +569,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                             }
                             // 16 elements are two 16-byte units of a 64-element slab; odd slabs write theirs in the other
                             // order, which keeps the eight lanes of a row on different banks
-                            const int R = w * 64 + (u4 + y) * (32 / kPer) + my_row, odd = (my_c >> 2) & 1, un = (my_c & 3) * 2;
+                            const int R = w * 32 + (u2 + y) * (32 / kPer) + my_row, odd = (my_c >> 2) & 1, un = (my_c & 3) * 2;
                             const uint32_t rowa = dst + (my_c >> 2) * kChunkBytes + R * 128;
                             const uint4 A = make_uint4(o[0], o[1], o[2], o[3]), B = make_uint4(o[4], o[5], o[6], o[7]);
                             st_shared_v4(rowa + uint32_t(((un + odd) ^ (R & 7)) << 4), odd ? B : A);
@@ -578,7 +577,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         }
                         if (go) {      // (what they will overwrite has been read)
 #pragma unroll
-                            for (int y = 0; y < 4; ++y) fetch(rows2, pitch2, u4 + y);
+                            for (int y = 0; y < 2; ++y) fetch(rows2, u2 + y);
                         }
                     }
                     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -685,7 +684,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     m = m_next;
                 }
                 uint32_t there = bits[g & 3];
-                if (E8) there = npg > 1 ? (there & 0xffffu) | ((there >> 16) << (64 >> p.box_shift)) : there & 0xffffu;   // (a half per warp)
+                if constexpr (E8) {                              // (a byte per converting warp)
+                    const uint32_t of = there;
+                    there = 0u;
+#pragma unroll
+                    for (int w = 0; w < L::kConv; ++w) there |= ((of >> (8 * w)) & 0xffu) << ((w * 32) >> p.box_shift);
+                }
                 uint32_t pk[BN / 2];
                 float l_tile;
                 bool bad = false;
@@ -854,7 +858,7 @@ int launch(int gpu, int G, cudaStream_t s, const CUtensorMap& mq, const CUtensor
            const PagedWorkspace& ws) {
     constexpr int bytes = Layout<E8>::kLaunch;
     PB_CUDA((paged_allow_smem<paged_tc_kernel<BF16, E8, HD>>(gpu, bytes)));
-    PB_CUDA(paged_launch(paged_tc_kernel<BF16, E8, HD>, dim3(unsigned(G)), kThreads, bytes, s, mq, mk, mv, p, ws));
+    PB_CUDA(paged_launch(paged_tc_kernel<BF16, E8, HD>, dim3(unsigned(G)), Layout<E8>::kThreads, bytes, s, mq, mk, mv, p, ws));
     return PARAS_OK;
 }
 

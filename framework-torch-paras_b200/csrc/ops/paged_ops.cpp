@@ -177,15 +177,16 @@ std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor& k_cach
                         (a.cache.D <= 1 || out.stride(2) == 1),
                     "paras paged_attention: out must have q's shape, type and device and contiguous rows");
     } else {
-        out = workspace_bytes ? q : at::empty(q.sizes(), q.options());
+        out = workspace_bytes ? Tensor() : at::empty(q.sizes(), q.options());
     }
     if (want_lse) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(c10::kFloat));
     a.q = qr.data_ptr();
-    a.out = out.data_ptr();
+    a.out = out.defined() ? out.data_ptr() : nullptr;
     a.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
     for (int i = 0; i < 2; ++i) {
         a.q_strides[i] = qr.stride(i);
-        a.o_strides[i] = out.stride(i);
+        // (a workspace is measured for contiguous rows: other ones never need more)
+        a.o_strides[i] = out.defined() ? out.stride(i) : (i == 0 ? q.size(1) : 1) * q.size(2);
     }
     a.kv_lens = index_array(kv_lens, a.cache.B, q, what, "kv_lens");
     a.cu = index_array(cu_q, int64_t(a.cache.B) + 1, q, what, "cu_q");

@@ -582,10 +582,20 @@ def _c():
 _C = None
 
 
+def _rows_in_place(stream, *tensors, whole=False):
+    """On a stream of the caller's the arguments have to be as the kernels read them: a copy that these calls make of rows
+    that are not (contiguous in the last dim, or ``whole``) is ordered with torch's current stream."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None and not (t.is_contiguous() if whole else t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1):
+                raise RuntimeError("paras abi: tensors must have contiguous rows when a stream is given")
+
+
 def paged_kv_write(k, v, k_cache, v_cache, page_table, kv_lens, cu_q, *, k_exp=None, v_exp=None, stream=None):
     """Writes new tokens' rows k, v [tokens, kv heads, D] into the paged cache in place (rounded to e4m3 with one
     exponent byte per row when the cache is ``float8_e4m3fn``): row ``cu_q[b] + i`` is position
     ``kv_lens[b] - (cu_q[b+1] - cu_q[b]) + i`` of sequence b."""
+    _rows_in_place(stream, k, v)
     (_C or _c()).paged_kv_write(k, v, k_cache, v_cache, page_table, kv_lens, cu_q, k_exp, v_exp, _stream_of(k, stream))
 
 
@@ -602,7 +612,9 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, *, ca
                     v_exp=None, out=None, return_lse=False, workspace=None, stream=None):
     """Attention of the new tokens q [tokens, heads, D] over a paged cache that holds their keys and values already.
     Row ``cu_q[b] + i`` is the query at position ``kv_lens[b] - (cu_q[b+1] - cu_q[b]) + i`` of sequence b and attends
-    the positions up to its own (all of them with ``causal=False``).  ``max_q`` bounds a sequence's new tokens."""
+    the positions up to its own (all of them with ``causal=False``).  ``max_q`` bounds a sequence's new tokens.  Rows of
+    ``out`` that belong to no sequence, or lie past ``max_q``, keep what they held (in a new tensor: anything)."""
+    _rows_in_place(stream, q)
     res = (_C or _c()).paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, causal, scale, k_exp, v_exp, out,
                                        return_lse, workspace, _stream_of(q, stream))
     return res if return_lse else res[0]
@@ -620,6 +632,7 @@ def paged_attn_last_kernel() -> str:
 def add_rmsnorm_fwd(x, residual, weight, eps=1e-6, *, return_rstd=False, stream=None):
     """(y, h[, rstd]): h = x + residual in x's type, y = RMSNorm(h) * weight.  ``residual=None`` normalises x itself
     (h is x); ``weight=None`` stands for ones."""
+    _rows_in_place(stream, x, residual, weight, whole=True)
     res = (_C or _c()).add_rms_norm(x, residual, weight, eps, return_rstd, _stream_of(x, stream))
     return res if return_rstd else res[:2]
 
@@ -627,10 +640,12 @@ def add_rmsnorm_fwd(x, residual, weight, eps=1e-6, *, return_rstd=False, stream=
 def add_rmsnorm_quant(x, residual, weight, eps=1e-6, *, group=0, stream=None):
     """(q, scales, h): the same norm in 8 bits, y ~ q * scales, q ``float8_e4m3fn``; one fp32 scale per row
     (``group=0``: scales [rows, 1]) or per ``group`` = 32, 64 or 128 columns (scales [rows, ceil(width / group)])."""
+    _rows_in_place(stream, x, residual, weight, whole=True)
     return (_C or _c()).add_rms_norm_quant(x, residual, weight, eps, group, _stream_of(x, stream))
 
 
 def add_rmsnorm_bwd(grad_y, grad_h, h, weight, rstd, *, stream=None):
     """(grad_x, grad_weight) of ``add_rmsnorm_fwd`` from the gradients that reach y and h (``grad_h=None``: none);
     grad_x is the gradient of x and of residual alike."""
+    _rows_in_place(stream, grad_y, grad_h, h, weight, rstd, whole=True)
     return (_C or _c()).add_rms_norm_backward(grad_y, grad_h, h, weight, rstd, _stream_of(h, stream))

@@ -37,6 +37,7 @@ class _AddRMSNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_h):
         h, weight, rstd = ctx.saved_tensors
         if grad_y is None:      # only h was used: the sum passes its gradient on
@@ -129,9 +130,10 @@ def paged_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                     k_exp: torch.Tensor = None, v_exp: torch.Tensor = None, return_lse: bool = False):
     """Attention of new tokens over a paged cache that already holds their own keys and values (``paged_kv_write``); the
     arguments are laid out as there.  ``query``: ``[tokens, heads, D]``, one token, a few or a chunk per sequence, mixed
-    freely; ``max_q`` bounds a sequence's count.  A token attends the positions up to its own (``is_causal=False``: all of
-    its sequence).  Forward only.  Returns ``[tokens, heads, D]`` and, with ``return_lse``, the fp32 log-sum-exp
-    ``[tokens, heads]``; a token that attends nothing gives zeros and ``-inf``."""
+    freely; ``max_q`` bounds a sequence's count (rows past it, and rows of no sequence, are left unset).  A token attends
+    the positions up to its own (``is_causal=False``: all of its sequence).  Forward only.  Returns
+    ``[tokens, heads, D]`` and, with ``return_lse``, the fp32 log-sum-exp ``[tokens, heads]``; a token that attends nothing
+    gives zeros and ``-inf``."""
     out, lse = torch.ops.paras.paged_attention(query, k_cache, v_cache, page_table, kv_lens, cu_q, max_q, is_causal, scale,
                                                k_exp, v_exp)
     return (out, lse) if return_lse else out

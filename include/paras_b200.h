@@ -385,7 +385,8 @@ int paras_b200_scale_columns(int gpu, const void* weight, const void* scale, voi
  * position of one kv head) in k_exp / v_exp, [pages, Hkv, page] bytes with strides *_exp_strides[3]; an element is
  * worth  e4m3 * 2^(byte - 127).  The byte is the smallest exponent that keeps the row's largest magnitude within
  * e4m3's 448, held between 2^-15 and 2^7, so that what a cache holds is exact in fp32, bf16 and fp16 alike; magnitudes
- * above 57344, infinities among them, are stored as 57344, NaN stays NaN.
+ * above 57344, infinities among them, are stored as 57344, NaN stays NaN.  Bytes outside 112 .. 134, which no writer
+ * here leaves, give unspecified finite or infinite values.
  *
  * The sequences, all on the device, so that a captured launch follows them: page_table[b][i] (row stride
  * table_stride) is the page of positions i*page .. of sequence b, max_pages entries a row.  An entry outside
@@ -470,7 +471,8 @@ const char* paras_b200_paged_attn_last_kernel(void);
  * _fwd writes y rounded once to `dtype`, h, and rstd (optional, fp32 [rows]).
  * _quant_fwd writes y in 8 bits instead, y ~ e4m3 * scale: one fp32 scale per row (group = 0) or per `group` = 32, 64
  * or 128 consecutive columns (the last group of a row may be shorter), scales [rows, ceil(H / group)] contiguous,
- * scale = max |y| / 448, at least 2^-126; y is not rounded to 16 bits in between.
+ * scale = max |y| / 448, at least 2^-126; y is not rounded to 16 bits in between.  The maximum skips NaN, which stays NaN.
+ * h may be the memory of x or of residual; no other two tensors may overlap.
  * _bwd: the gradients of _fwd from grad_y and grad_h (the gradient that arrives at h, NULL: none): grad_x is the
  * gradient of x and of residual alike, grad_weight [H] in `dtype` (NULL with weight NULL). */
 int paras_b200_add_rmsnorm_fwd(int gpu, const void* x, const void* residual, const void* weight, void* h, void* y,

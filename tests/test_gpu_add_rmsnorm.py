@@ -187,3 +187,51 @@ def test_in_place_streams_capture_and_refusals():
     assert y.shape == (0, 4096)
     gx, gw = abi.add_rmsnorm_bwd(x[:0], None, x[:0], w, torch.empty(0, device=DEV))
     assert bool((gw == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("width", [7, 577, 4096, 5001, 16384, 33000, 40961])
+def test_the_sum_over_either_of_its_terms(width, dtype):
+    # through the C entries: h is the memory of x or of residual, on every kernel
+    code = abi.BF16 if dtype == BF else abi.F32
+    x, r, w = data(9, width, dtype, 1), data(9, width, dtype, 2), data(1, width, dtype, 3)[0]
+    ref, quant = abi.add_rmsnorm_fwd(x, r, w), abi.add_rmsnorm_quant(x, r, w, group=64)
+    stream = torch.cuda.current_stream().cuda_stream or 1
+    for over in (0, 1):
+        a, b, y = x.clone(), r.clone(), torch.empty_like(x)
+        h = b if over else a
+        abi.check(abi.lib().paras_b200_add_rmsnorm_fwd(0, a.data_ptr(), b.data_ptr(), w.data_ptr(), h.data_ptr(), y.data_ptr(), None,
+                                                       9, width, 1e-6, code, stream))
+        assert torch.equal(h, ref[1]) and torch.equal(y, ref[0])
+        a, b = x.clone(), r.clone()
+        h, q, s = b if over else a, torch.empty_like(quant[0]), torch.empty_like(quant[1])
+        abi.check(abi.lib().paras_b200_add_rmsnorm_quant_fwd(0, a.data_ptr(), b.data_ptr(), w.data_ptr(), h.data_ptr(), q.data_ptr(),
+                                                             s.data_ptr(), 9, width, 1e-6, 64, code, stream))
+        assert torch.equal(h, ref[1]) and torch.equal(s, quant[1]) and torch.equal(q.view(torch.uint8), quant[0].view(torch.uint8))
+
+
+def test_a_given_stream_takes_no_copies():
+    x, w = data(8, 512, BF, 1), data(1, 512, BF, 3)[0]
+    wide = data(8, 1024, BF, 2)[:, ::2]
+    want = abi.add_rmsnorm_fwd(x, wide, w)
+    assert torch.equal(want[1], (x.float() + wide.float()).to(BF))
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = abi.add_rmsnorm_fwd(x, wide.contiguous(), w, stream=torch.cuda.current_stream().cuda_stream or 1)
+    assert torch.equal(got[0], want[0])
+    for call in (lambda: abi.add_rmsnorm_fwd(x, wide, w, stream=s.cuda_stream),
+                 lambda: abi.add_rmsnorm_quant(wide, x, w, stream=s.cuda_stream),
+                 lambda: abi.add_rmsnorm_bwd(wide, None, x, w, torch.ones(8, device=DEV), stream=s.cuda_stream)):
+        with pytest.raises(RuntimeError, match="contiguous rows"):
+            call()
+
+
+def test_a_second_derivative_is_refused():
+    from torch_paras import nn
+    x, r, w = (torch.randn(n, 16, dtype=torch.float32).squeeze(0).to("paras:1").requires_grad_() for n in (3, 3, 1))
+    ones = torch.ones(3, 16).to("paras:1")
+    for grad_y, text in ((ones, "does not require grad"), (ones.clone().requires_grad_(), "once_differentiable")):
+        y, h = nn.add_rms_norm(x, r, w)
+        g = torch.autograd.grad(y, x, grad_y, create_graph=True)[0]
+        with pytest.raises(RuntimeError, match=text):
+            g.backward(ones)

@@ -274,6 +274,160 @@ def test_a_cache_past_2_31_elements():
         del big, kw, table, a, b
 
 
+def test_routes():
+    def route(q_lens, Hq, Hkv, D, page, dtype, cache8=False, kv=300, **kw):
+        check_attention(q_lens, [kv] * len(q_lens), Hq, Hkv, D, page, dtype, cache8, **kw)
+        return abi.paged_attn_last_kernel()
+
+    for cache8 in (False, True):
+        for dtype in (BF, HF):
+            assert route([1, 1], 8, 2, 128, 16, dtype, cache8) == "paged_decode"
+            assert route([4, 1], 8, 2, 64, 256, dtype, cache8) == "paged_decode"
+            assert route([9, 9], 8, 2, 128, 16, dtype, cache8) == "paged_tcgen05"
+            assert route([1, 1], 34, 2, 64, 8, dtype, cache8) == "paged_tcgen05"
+            assert route([60, 1, 1, 1], 8, 2, 128, 16, dtype, cache8) == "paged_tcgen05+paged_decode"
+            assert route([60, 30, 1, 1], 8, 2, 128, 16, dtype, cache8) == "paged_tcgen05"
+        assert route([3], 8, 2, 128, 16, FP, cache8) == "paged_simt"
+        assert route([3], 8, 2, 96, 16, BF, cache8) == "paged_simt"
+        assert route([3], 8, 2, 128, 24, BF, cache8) == "paged_simt"
+        assert route([3], 130, 1, 64, 16, BF, cache8) == "paged_simt"
+        assert route([30], 8, 2, 128, 16, BF, cache8, scale=0.0) == "paged_simt"
+
+
+MIXED = ([1, 300, 2, 1, 0, 3, 1], [513, 900, 129, 1, 70, 260, 640])
+
+
+@pytest.mark.parametrize("cache8", [False, True])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D,page", [(128, 16), (64, 128)])
+def test_chunks_and_single_tokens_in_one_call(D, page, dtype, cache8):
+    route = "paged_tcgen05+paged_decode"
+    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route=route)
+    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route=route, causal=False, first=2, behind=4, order="pdh")
+    absent = [(0, 0), (1, 0), (1, 2), (3, 0), (6, 0), (6, 1)]
+    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route=route, absent=absent)
+
+
+@pytest.mark.parametrize("cache8", [False, True])
+def test_a_captured_mixed_call_follows_tokens_that_change_places(cache8):
+    c = Cache([600, 400, 500, 300], 2, 128, 16, BF, cache8)
+    T = 70
+    q = rand(T, 8, 128, dtype=BF, seed=1)
+    cu = cu_of([67, 1, 1, 1])
+    args = (q, *c.cache, c.table, c.kv_lens, cu, 67)
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        abi.paged_attention(*args, out=out, **c.kw)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        abi.paged_attention(*args, out=out, **c.kw)
+    assert abi.paged_attn_last_kernel() == "paged_tcgen05+paged_decode"
+    for q_lens in ([67, 1, 1, 1], [1, 4, 64, 1], [0, 5, 60, 5], [17, 18, 17, 18], [4, 4, 4, 4], [0, 0, 0, 0]):
+        cu.copy_(cu_of(q_lens))
+        out.fill_(5.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want, _, A, S = attend64(q[:sum(q_lens)], c, q_lens, [600, 400, 500, 300], 128 ** -0.5)
+        tol = attend_tolerance(want, A, S, BF, 128, 600)
+        assert ((out[:sum(q_lens)].cpu().double() - want).abs() <= tol).all()
+        assert bool((out[sum(q_lens):] == 5).all())
+
+
+@pytest.mark.parametrize("q_lens", [[1], [16], [40]], ids=["token", "draft", "chunk"])
+@pytest.mark.parametrize("cache8", [False, True])
+def test_one_item_cut_between_all_multiprocessors(q_lens, cache8):
+    # one kv head, more tiles than multiprocessors: every CTA leaves a part of the same rows
+    check_attention(q_lens, [40000], 1, 1, 64, 128, BF, cache8)
+
+
+def test_more_sequences_than_threads():
+    for cache8 in (False, True):
+        B = 700
+        kv = [1 + (37 * b) % 300 for b in range(B)]
+        check_attention([1] * B, kv, 2, 1, 64, 32, BF, cache8, route="paged_decode")
+        check_attention([(b * 7) % 3 for b in range(B - 1)] + [50], kv, 2, 1, 64, 32, BF, cache8, route="paged_tcgen05+paged_decode")
+        check_attention([24 if b % 50 == 0 else 18 for b in range(B)], [n + 24 for n in kv], 2, 1, 64, 32, BF, cache8, route="paged_tcgen05")
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1], [50, 40], [50, 1, 1]], ids=["token", "chunk", "mixed"])
+def test_workspaces(q_lens):
+    kv = [400 + 100 * i for i in range(len(q_lens))]
+    c = Cache(kv, 2, 128, 16, BF, False)
+    T = sum(q_lens)
+    q = rand(T, 8, 128, dtype=BF, seed=1)
+    cu = cu_of(q_lens)
+    args = lambda q: (q, *c.cache, c.table, c.kv_lens, cu, max(q_lens))      # noqa: E731
+    n = abi.paged_attn_workspace_bytes(*args(q))
+    want = abi.paged_attention(*args(q))
+    ws = torch.zeros(n + 16, dtype=torch.uint8, device=DEV)
+    with pytest.raises(RuntimeError, match="too small"):
+        abi.paged_attention(*args(q), workspace=ws[:n - 1])
+    with pytest.raises(RuntimeError, match="16-byte aligned"):
+        abi.paged_attention(*args(q), workspace=ws[8:8 + n])
+    # exactly as much as is asked for, nothing written behind it; rows with a stride on D are copied first
+    ws.fill_(7)
+    strided = torch.empty(T, 8, 128, 2, dtype=BF, device=DEV)[..., 0].copy_(q)
+    assert abi.paged_attn_workspace_bytes(*args(strided)) == n
+    for x in (q, strided):
+        assert torch.equal(abi.paged_attention(*args(x), workspace=ws[:n]), want)
+    assert bool((ws[n:] == 7).all())
+    # two captured graphs with one workspace, replayed in turn
+    q2 = -q
+    outs = [torch.empty_like(q) for _ in range(2)]
+    side = torch.cuda.Stream()
+    graphs = []
+    torch.cuda.synchronize()
+    for x, o in zip((q, q2), outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            abi.paged_attention(*args(x), workspace=ws[:n], out=o)
+        graphs.append(g)
+    want2 = abi.paged_attention(*args(q2))
+    for _ in range(3):
+        for g, o, w in zip(graphs, outs, (want, want2)):
+            o.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, w)
+
+
+def test_a_given_stream():
+    q_lens, kv = [1, 40], [300, 500]
+    c = Cache(kv, 2, 128, 16, BF, False)
+    q = rand(41, 8, 128, dtype=BF, seed=1)
+    args = (*c.cache, c.table, c.kv_lens, cu_of(q_lens), 40)
+    want = abi.paged_attention(q, *args)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    out = torch.empty_like(q)
+    got = abi.paged_attention(q, *args, out=out, stream=s.cuda_stream)
+    s.synchronize()
+    assert torch.equal(got, want)
+    strided = torch.empty(41, 8, 128, 2, dtype=BF, device=DEV)[..., 0].copy_(q)
+    assert torch.equal(abi.paged_attention(strided, *args), want)
+    with pytest.raises(RuntimeError, match="contiguous rows"):
+        abi.paged_attention(strided, *args, stream=s.cuda_stream)
+    with pytest.raises(RuntimeError, match="contiguous rows"):
+        abi.paged_kv_write(strided[:, :2], strided[:, :2], *c.cache, c.table, c.kv_lens, cu_of(q_lens), stream=s.cuda_stream)
+
+
+def test_rows_of_nothing_but_nan():
+    for dtype in (BF, HF, FP):
+        for T in (3, 4000):      # a warp per row, several heads a warp
+            c = Cache([T], 6, 64, 16, dtype, True)
+            k = rand(T, 6, 64, dtype=dtype, seed=1)
+            k[1, 2], k[2] = float("nan"), float("inf")
+            k[0, 1] = -0.0
+            abi.paged_kv_write(k, -k, *c.cache, c.table, c.kv_lens, cu_of([T]), **c.kw)
+            for got, x in zip(abi.paged_kv_read(*c.cache, c.table, cu_of([T]), T, dtype=FP, **c.kw), (k, -k)):
+                q, e = quantise64(x)
+                want = (q * torch.pow(2.0, e).unsqueeze(-1)).float()
+                assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want))
+                assert torch.equal(got.cpu().nan_to_num(), want.nan_to_num())
+
+
 # ---------------------------------------------------------------- writing and reading
 
 def rows_for(T, H, D, dtype, seed):

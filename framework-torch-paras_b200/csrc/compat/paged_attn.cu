@@ -98,7 +98,7 @@ int check(const paras_paged_attn_args* args, const char* what) {
     if (a.Hq < 1 || a.Hq % a.cache.Hkv)
         return fail(PARAS_E_INVALID, "%s: query heads (%d) must be a multiple of key/value heads (%d)", what, a.Hq, a.cache.Hkv);
     if (int64_t(a.T) * a.Hq > (int64_t(1) << 32)) return fail(PARAS_E_UNSUPPORTED, "%s: more than 2^32 query rows", what);
-    if (!std::isfinite(a.scale)) return fail(PARAS_E_INVALID, "%s: scale is not finite", what);
+    if (!std::isfinite(float(a.scale))) return fail(PARAS_E_INVALID, "%s: scale is not finite", what);
     return PARAS_OK;
 }
 

@@ -58,6 +58,12 @@ __device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& 
     return p.causal ? max(0, min(s.kv, s.pos0 + i + 1)) : s.kv;
 }
 
+// The streaming kernels move their reference by products with c2 = scale * log2(e) (times a row's power of two) and its
+// inverse, which have to stay finite: scales below 2^-100 go to the CUDA cores, a row's c2 stays above 2^-120 (rows of q
+// below 2^-126 of an ordinary one, whose scores are all the same to fp32).
+constexpr float kLeastC2 = 7.5231638452626401e-37f;      // 2^-120
+inline bool paged_scale_ok(const paras_paged_attn_args& a) { return a.scale >= 7.888609052210118e-31; }   // 2^-100
+
 int paged_simt_launch(const PagedParams& p, int dtype, bool cache8, cudaStream_t s);
 
 // ---- the streaming kernels' shared-out work ------------------------------------------------------

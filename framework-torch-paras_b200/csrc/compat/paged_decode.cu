@@ -445,7 +445,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             // largest magnitude to [1, 2)
                             const int ex = max(-120, min(120, int(__float_as_uint(amax) >> 23) - 127));
                             const float f = pow2f(-ex);
-                            c2[h] = p.scale_log2 * pow2f(ex);
+                            c2[h] = fmaxf(p.scale_log2 * pow2f(ex), kLeastC2);
                             lag[h] = 8.f / c2[h];
 #pragma unroll
                             for (int ks = 0; ks < HD / 16; ++ks) {
@@ -727,7 +727,7 @@ int paged_decode_rows() { return kRows; }
 
 bool paged_decode_supported(const Gpu* g, const paras_paged_attn_args& a) {
     return g->cc_major >= 9 && a.dtype != PARAS_F32 && paged_tma_ok(a.cache) && paged_q_tma_ok(a) &&
-           a.Hq / a.cache.Hkv <= kRows && a.scale > 0.0 && g->smem_optin >= 227 * 1024;
+           a.Hq / a.cache.Hkv <= kRows && paged_scale_ok(a) && g->smem_optin >= 227 * 1024;
 }
 
 int paged_decode_launch(Gpu* g, const paras_paged_attn_args& a, const PagedParams& p, const PagedWorkspace& ws, int G, cudaStream_t s) {

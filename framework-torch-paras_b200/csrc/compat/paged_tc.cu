@@ -638,7 +638,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 }
                 const int ex = max(-120, min(120, int(__float_as_uint(amax) >> 23) - 127));
                 const float f = pow2f(-ex);
-                c2 *= pow2f(ex);
+                c2 = fmaxf(c2 * pow2f(ex), kLeastC2);
 #pragma unroll
                 for (int u = 0; u < HD / 8; ++u) {
                     const uint32_t a = qrow + (u >> 3) * kChunkBytes + uint32_t(((u & 7) ^ (row & 7)) << 4);
@@ -868,7 +868,7 @@ int paged_tc_rows() { return 256; }
 
 bool paged_tc_supported(const Gpu* g, const paras_paged_attn_args& a) {
     if (g->cc_major != 10 || a.dtype == PARAS_F32 || !paged_tma_ok(a.cache) || !paged_q_tma_ok(a)) return false;
-    if (a.Hq / a.cache.Hkv > BM || !(a.scale > 0.0) || g->smem_optin < 227 * 1024) return false;
+    if (a.Hq / a.cache.Hkv > BM || !paged_scale_ok(a) || g->smem_optin < 227 * 1024) return false;
     // finished rows leave in 16-byte pieces
     return (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && a.o_strides[0] % 8 == 0 && a.o_strides[1] % 8 == 0;
 }

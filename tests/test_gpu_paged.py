@@ -157,6 +157,20 @@ def test_small_and_huge_queries_against_an_8_bit_cache():
         check_attention(q_lens, [200, 300], 4, 1, 128, 16, BF, True, q=q, scale=1e-3)
 
 
+@pytest.mark.parametrize("q_lens", [[1, 2], [1, 60]], ids=["token", "chunk"])
+@pytest.mark.parametrize("cache8", [False, True])
+def test_queries_of_zero_and_scales_down_to_nothing(q_lens, cache8):
+    T = sum(q_lens)
+    q = rand(T, 4, 128, dtype=BF, seed=4)
+    q[:, 1] = 0
+    q[:, 2] *= 2.0 ** -120
+    q[:, 3] *= 2.0 ** -133       # subnormal
+    for scale in (0.1, 1e-3, 1e-8, 2.0 ** -99, 1e-31, 1e-38, 1e-45, 1e-60):
+        check_attention(q_lens, [200, 300], 4, 1, 128, 16, BF, cache8, q=q, scale=scale)
+    with pytest.raises(RuntimeError, match="scale is not finite"):
+        check_attention(q_lens, [200, 300], 4, 1, 128, 16, BF, cache8, q=q, scale=1e39)
+
+
 def test_max_q_bounds_what_is_computed():
     c = Cache([50, 60], 1, 64, 16, BF, False)
     q = rand(30, 2, 64, dtype=BF, seed=2)

@@ -102,12 +102,17 @@ int check(const paras_paged_attn_args* args, const char* what) {
     return PARAS_OK;
 }
 
-// At most 16 query rows per kv head stream through mma.sync tiles, more go to the tensor-core tiles of 128 rows; fp32,
-// other head dims than 64 and 128, pages that no tile of 128 positions is made of, and unaligned tensors to CUDA cores.
+// At most 16 query rows per kv head stream through mma.sync tiles (64 single tokens over 512 .. 16384 positions: 340 us, in
+// 128-row tiles 441; 48 x 4 tokens: 146 and 199, from an 8-bit cache 126 and 320; one token over 1000: 12.0 and 14.3), more go
+// to the tensor-core tiles of 128 rows; fp32, other head dims than 64 and 128, pages that no tile of 128 positions is made of,
+// and unaligned tensors to CUDA cores.
 // A call for chunks whose sequences besides the longest average less than twice 16 rows is taken to mix both, and makes a
-// launch for each: single tokens in 128-row tiles cost their CTA a whole softmax tile per step (12 sequences, one of 700
-// tokens, 8-bit cache: 93 us in one launch).  The rule goes by counts the host knows; where it is wrong, one of the launches
-// finds nothing to do and costs about 3 us.
+// launch for each where the others may have enough tiles to make up for the second launch (about 12 us): 80 for each
+// multiprocessor, or 14 of an 8-bit cache, whose bytes the 128-row kernel converts at half the rate.  In one launch and in
+// two, one sequence of 700 tokens and n of one over up to L positions, 8 kv heads of 128: 16-bit n = 15, L = 4096: 97 and
+// 108 us; 47, 4096: 157 and 160; 95, 4096: 255 and 235; 31, 16384: 419 and 379; 8-bit n = 3, L = 4096: 105 and 109 us;
+// 7, 4096: 120 and 117; 31, 4096: 210 and 154; 15, 16384: 495 and 367.
+// The rule goes by counts the host knows, of lengths the page table's reach; where it is wrong, the second launch costs that.
 struct Routes {
     bool decode, tc;
     int small;      // tokens a sequence may have for the first of the two
@@ -122,7 +127,9 @@ Routes pick_routes(const Gpu* g, const paras_paged_attn_args& a) {
     } else if (paged_tc_supported(g, a)) {
         r.tc = true;
         const int64_t others = a.cache.B - 1, left = int64_t(a.T) - a.max_q;
-        r.decode = dec && others > 0 && left < others * 2 * r.small;
+        const int64_t tiles = others * a.cache.Hkv * ((int64_t(a.cache.max_pages) * a.cache.page + kTileKeys - 1) / kTileKeys);
+        const int64_t least = a.cache.cache_dtype == PARAS_E4M3 ? 14 : 80;
+        r.decode = dec && others > 0 && left < others * 2 * r.small && tiles >= least * g->sm_count;
     }
     return r;
 }

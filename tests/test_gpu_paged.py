@@ -18,9 +18,18 @@ def rand(*shape, dtype, seed, scale=1.0):
     return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).to(DEV)
 
 
+def widen(c):
+    """A page table with the reach that long sequences need, most of it absent: a call that mixes a chunk with single tokens
+    is then split (by the positions there may be)."""
+    P = -(-4_000_000 // (c.Hkv * (len(c.table) - 1) * c.page))
+    c.table = torch.cat([c.table, torch.full((len(c.table), P), -1, dtype=torch.int32, device=c.table.device)], 1)
+
+
 def check_attention(q_lens, kv_lens, Hq, Hkv, D, page, dtype, cache8, causal=True, order="phd", seed=1, q=None, qscale=1.0,
-                    absent=(), route=None, first=0, behind=0, scale=None, max_q=None):
+                    absent=(), route=None, first=0, behind=0, scale=None, max_q=None, wide=False):
     c = Cache(kv_lens, Hkv, D, page, dtype, cache8, seed=seed, order=order)
+    if wide:
+        widen(c)
     for b, p in absent:
         c.table[b, p] = [-1, c.pages, 2 ** 31 - 1, -2 ** 31][p % 4]
     T = first + sum(q_lens) + behind
@@ -299,8 +308,9 @@ def test_routes():
             assert route([4, 1], 8, 2, 64, 256, dtype, cache8) == "paged_decode"
             assert route([9, 9], 8, 2, 128, 16, dtype, cache8) == "paged_tcgen05"
             assert route([1, 1], 34, 2, 64, 8, dtype, cache8) == "paged_tcgen05"
-            assert route([60, 1, 1, 1], 8, 2, 128, 16, dtype, cache8) == "paged_tcgen05+paged_decode"
-            assert route([60, 30, 1, 1], 8, 2, 128, 16, dtype, cache8) == "paged_tcgen05"
+            assert route([60, 1, 1, 1], 8, 2, 128, 16, dtype, cache8) == "paged_tcgen05"
+            assert route([60, 1, 1, 1], 8, 2, 128, 16, dtype, cache8, wide=True) == "paged_tcgen05+paged_decode"
+            assert route([60, 30, 1, 1], 8, 2, 128, 16, dtype, cache8, wide=True) == "paged_tcgen05"
         assert route([3], 8, 2, 128, 16, FP, cache8) == "paged_simt"
         assert route([3], 8, 2, 96, 16, BF, cache8) == "paged_simt"
         assert route([3], 8, 2, 128, 24, BF, cache8) == "paged_simt"
@@ -316,15 +326,17 @@ MIXED = ([1, 300, 2, 1, 0, 3, 1], [513, 900, 129, 1, 70, 260, 640])
 @pytest.mark.parametrize("D,page", [(128, 16), (64, 128)])
 def test_chunks_and_single_tokens_in_one_call(D, page, dtype, cache8):
     route = "paged_tcgen05+paged_decode"
-    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route=route)
-    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route=route, causal=False, first=2, behind=4, order="pdh")
+    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route="paged_tcgen05")
+    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route=route, wide=True)
+    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route=route, wide=True, causal=False, first=2, behind=4, order="pdh")
     absent = [(0, 0), (1, 0), (1, 2), (3, 0), (6, 0), (6, 1)]
-    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route=route, absent=absent)
+    check_attention(*MIXED, 8, 2, D, page, dtype, cache8, route=route, wide=True, absent=absent)
 
 
 @pytest.mark.parametrize("cache8", [False, True])
 def test_a_captured_mixed_call_follows_tokens_that_change_places(cache8):
     c = Cache([600, 400, 500, 300], 2, 128, 16, BF, cache8)
+    widen(c)
     T = 70
     q = rand(T, 8, 128, dtype=BF, seed=1)
     cu = cu_of([67, 1, 1, 1])
@@ -361,14 +373,15 @@ def test_more_sequences_than_threads():
         B = 700
         kv = [1 + (37 * b) % 300 for b in range(B)]
         check_attention([1] * B, kv, 2, 1, 64, 32, BF, cache8, route="paged_decode")
-        check_attention([(b * 7) % 3 for b in range(B - 1)] + [50], kv, 2, 1, 64, 32, BF, cache8, route="paged_tcgen05+paged_decode")
-        check_attention([24 if b % 50 == 0 else 18 for b in range(B)], [n + 24 for n in kv], 2, 1, 64, 32, BF, cache8, route="paged_tcgen05")
+        check_attention([(b * 7) % 3 for b in range(B - 1)] + [50], kv, 2, 1, 64, 32, BF, cache8, route="paged_tcgen05+paged_decode", wide=True)
+        check_attention([24 if b % 50 == 0 else 18 for b in range(B)], [n + 24 for n in kv], 2, 1, 64, 32, BF, cache8, route="paged_tcgen05", wide=True)
 
 
 @pytest.mark.parametrize("q_lens", [[1, 1], [50, 40], [50, 1, 1]], ids=["token", "chunk", "mixed"])
 def test_workspaces(q_lens):
     kv = [400 + 100 * i for i in range(len(q_lens))]
     c = Cache(kv, 2, 128, 16, BF, False)
+    widen(c)
     T = sum(q_lens)
     q = rand(T, 8, 128, dtype=BF, seed=1)
     cu = cu_of(q_lens)

@@ -11,7 +11,7 @@
 //
 // Measured (8 kv heads of 128, pages of 64): write of 4 x 4096 tokens 21.1 us as bf16 (5.9 TB/s), 19.1 us into 8 bits
 // (4.9 TB/s; bound by instructions before the rows stayed in pairs of 16 bits: 25.3 us); one token for each of 64
-// sequences 2.6 us; read of 16 sequences of up to 8192 from 8 bits 61.4 us (5.8 TB/s), of one of 1500 as bf16 5.0 us.
+// sequences 2.6 us; read of 16 sequences of up to 8192 from 8 bits 61.4 us (5.8 TB/s), of one of 1500 as bf16 3.8 us.
 #include "paged_common.cuh"
 
 namespace pb {
@@ -363,12 +363,13 @@ void launch(const KvParams& p, bool vec, int sms, cudaStream_t s) {
     const int64_t rows = int64_t(p.T) * p.Hkv;
     auto go = [&](auto kernel, int64_t warps) { kernel<<<unsigned((warps + kWarps - 1) / kWarps), kWarps * 32, 0, s>>>(p); };
     if (!vec) return go(paged_kv_any_kernel<T, CACHE8, WRITE>, rows);
-    // Several heads a warp once there are rows enough for every warp slot of the GPU: the look-up of the token's place is
-    // shared and more loads are in flight; below that, a warp per row keeps the chain short.  4 x 4096 bf16 tokens of 8 heads
-    // into an 8-bit cache: 19.1 us with four heads a warp, 26.0 with two, 19.0 with eight (which costs short rows more:
-    // 4 x 2048 of 4 heads of 64 take 6.0, 8.0, 7.2 us).
+    // Several heads a warp: the look-up of the token's place is shared and more loads are in flight.  4 x 4096 bf16 tokens of
+    // 8 heads into an 8-bit cache: 19.1 us with four heads a warp, 26.0 with two, 19.0 with eight (which costs short rows
+    // more: 4 x 2048 of 4 heads of 64 take 6.0, 8.0, 7.2 us), 46.2 with one; 256 rows 2.6 us either way.  A reader waits for
+    // page numbers before its loads and is slower at few rows: 256 rows 2.4 us with one head a warp, 3.3 with eight; 2048
+    // rows 2.9 and 3.3; 8192 rows 4.8 and 3.8; 16000 rows 7.2 and 4.4 (16-bit: 2.4 / 2.9, 2.7 / 2.9, 3.9 / 3.4, 6.2 / 4.3).
     constexpr int kMany = WRITE ? 4 : 8;
-    const bool many = p.Hkv > 1 && rows >= int64_t(sms) * 64 * 2;
+    const bool many = p.Hkv > 1 && (WRITE || rows >= int64_t(sms) * 32);
     const int64_t warps = many ? int64_t(p.T) * ((p.Hkv + kMany - 1) / kMany) : rows;
     if constexpr (WRITE) many ? go(paged_kv_write_kernel<T, CACHE8, kMany>, warps) : go(paged_kv_write_kernel<T, CACHE8, 1>, warps);
     else many ? go(paged_kv_read_kernel<T, CACHE8, kMany>, warps) : go(paged_kv_read_kernel<T, CACHE8, 1>, warps);

@@ -235,3 +235,20 @@ def test_a_second_derivative_is_refused():
         g = torch.autograd.grad(y, x, grad_y, create_graph=True)[0]
         with pytest.raises(RuntimeError, match=text):
             g.backward(ones)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("width", [64, 256, 512, 1000, 2048])
+def test_backward_of_many_rows(width, dtype):
+    # every block walks several rows, and its ring of rows goes round
+    rows, u = 10_001, torch.finfo(dtype).eps / 2
+    h, w = data(rows, width, dtype, 1, 2.0), data(1, width, dtype, 3)[0]
+    gy, gh = data(rows, width, dtype, 4), data(rows, width, dtype, 5)
+    rstd = norm64(h, None, 1e-6)[1][:, 0].float().to(DEV)
+    gx, gw = abi.add_rmsnorm_bwd(gy, gh, h, w, rstd)
+    wx, ww, sx, sw = grads64(gy, gh, h, w, 1e-6)
+    close(gx, wx, u * wx.abs() + 96 * F32 * sx + torch.finfo(dtype).tiny)
+    # a column's products go through fp32 in runs of at most 32 rows (10001 / 592 and fewer), in 64 bits between the runs
+    close(gw, ww, u * ww.abs() + 64 * F32 * sw + torch.finfo(dtype).tiny)
+    again = abi.add_rmsnorm_bwd(gy, gh, h, w, rstd)
+    assert torch.equal(again[0], gx) and torch.equal(again[1], gw)

@@ -9,7 +9,7 @@
 //   warps 10-11     16-bit cache: zero what a page holds past the end of its sequence (0 * NaN must not reach O)
 //   warps 10-13     8-bit cache: bring e4m3 rows to fp16 (cp.async into a staging tile, exact conversion, 2^e of the row
 //                   multiplied in), a tile ahead of the MMAs; with two warps for this, 2 x 2048 tokens over 6000-8192
-//                   positions took 594 us, with four 553 (430 and 369 with heads of 64), and 330 from a 16-bit cache:
+//                   positions took 594 us, with four 553 (430 and 361 with heads of 64), and 330 (306) from a 16-bit cache:
 //                   the conversion shares the issue slots with the softmax.  (14 and 15 only fill their warpgroup.)
 // What differs: the query heads of a GQA group always share a tile (rows = (token, head), floor(128 / group) tokens of a
 // tile, by a 4-D box on q), so that K and V are read once per group whatever the lengths; tiles are shared out over the
@@ -40,21 +40,24 @@ using namespace tc;
 
 constexpr int BM = 128, BN = kTileKeys;
 constexpr int kChunkBytes = 64 * 2 * 128;    // 64 elements x 128 rows
-constexpr int kTileBytes = 2 * kChunkBytes;
-constexpr int kPairBytes = 2 * kTileBytes;   // V_j, then K_j+1
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kHelpWarp = 10;
 constexpr int kItems = 4;                     // descriptors in flight
 constexpr float kRescaleSum = 256.0f, kRedoSum = 32768.0f;
 constexpr int kColS = 0, kColO = 256;
 
 constexpr int kSmemQ = 0;
-constexpr int kSmemKV = 2 * kTileBytes;
-constexpr int kSmemO = kSmemKV + 2 * kPairBytes;       // per softmax warp: staging of finished rows, 32 x 64 or 128 B
-constexpr int kBarQFull = 0, kBarQEmpty = 2, kBarKVFull = 4, kBarKVEmpty = 6, kBarSFull = 8, kBarPFull = 10, kBarOFull = 12,
-              kBarQConv = 14, kBarVLand = 16, kBarItemFull = 18, kBarItemEmpty = kBarItemFull + kItems,
-              kNumBars = kBarItemEmpty + kItems;
+constexpr int kMaxPairs = 4;
+constexpr int kBarQFull = 0, kBarQEmpty = 2, kBarSFull = 4, kBarPFull = 6, kBarOFull = 8, kBarQConv = 10, kBarKVFull = 12,
+              kBarKVEmpty = kBarKVFull + kMaxPairs, kBarVLand = kBarKVEmpty + kMaxPairs, kBarItemFull = kBarVLand + kMaxPairs,
+              kBarItemEmpty = kBarItemFull + kItems, kNumBars = kBarItemEmpty + kItems;
 
-template <bool E8> struct Layout {
+template <bool E8, int HD> struct Layout {
+    static constexpr int kTileBytes = HD / 64 * kChunkBytes;           // of Q, K or V, fp16 or bf16
+    static constexpr int kPairBytes = 2 * kTileBytes;                  // V_j, then K_j+1
+    static constexpr int kPairLog = HD == 64 ? 2 : 1, kPairs = 1 << kPairLog;      // as many as there is room for
+    // (heads of 64 with two: 4 x 16 tokens over 16384 positions 66 us, with four 59)
+    static constexpr int kSmemKV = 2 * kTileBytes;
+    static constexpr int kSmemO = kSmemKV + kPairs * kPairBytes;       // per softmax warp: staging of finished rows
     static constexpr int kConv = E8 ? 4 : 0;                           // warps that convert, a quarter of a tile's rows each
     static constexpr int kThreads = E8 ? 512 : 384;
     static constexpr int kAtLaunch = E8 ? 128 : 168;                   // registers per thread
@@ -63,8 +66,8 @@ template <bool E8> struct Layout {
     static constexpr int kRaw = kSmemO + 8 * kOStage;                  // 8-bit: a tile of e4m3 rows
     static constexpr int kScale = kRaw + (E8 ? 16 * 1024 : 0);         // 8-bit: 2^e of the rows, fp16 twice
     static constexpr int kItem = kScale + (E8 ? 512 : 0);
-    static constexpr int kBits = kItem + kItems * 64;                  // pages that are there, of the last four tiles
-    static constexpr int kSums = kBits + 16;
+    static constexpr int kBits = kItem + kItems * 64;                  // pages that are there, of the last 2 * kPairs tiles
+    static constexpr int kSums = kBits + 2 * kPairs * 4;
     static constexpr int kBars = kSums + (kThreads / 32 + 3) * 8 + 8;
     static constexpr int kMisc = kBars + kNumBars * 8;
     static constexpr int kLaunch = kMisc + 16 + 1024;
@@ -115,16 +118,20 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 }
 
 template <bool BF16, bool E8, int HD>
-__global__ void __launch_bounds__(Layout<E8>::kThreads, 1)
+__global__ void __launch_bounds__(Layout<E8, HD>::kThreads, 1)
 paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const PagedParams p, const PagedWorkspace ws) {
-    using L = Layout<E8>;
+    using L = Layout<E8, HD>;
+    constexpr int kTileBytes = L::kTileBytes, kPairBytes = L::kPairBytes, kSmemKV = L::kSmemKV, kSmemO = L::kSmemO;
     constexpr bool kBfOps = BF16 && !E8;
     constexpr int kChunks = HD / 64;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     auto bar = [&](int i) { return base + L::kBars + 8u * i; };
+    auto slot_of = [](int g) { return g & (L::kPairs - 1); };               // of pair g, and the parity of its turn there
+    auto turn_of = [](int g) { return uint32_t(g >> L::kPairLog) & 1u; };
+    constexpr int kBitsMask = 2 * L::kPairs - 1;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::kMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::kMisc + 4);
     Item* items = reinterpret_cast<Item*>(gen + L::kItem);
@@ -135,7 +142,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNumBars; ++i) {
             int n = 1;                                                                   // a commit, a TMA, the loading warp
-            if (i >= kBarKVFull && i < kBarKVFull + 2) n = E8 ? 2 * L::kConv : 2;        // entries of a pair (by four warps)
+            if (i >= kBarKVFull && i < kBarKVFull + kMaxPairs) n = E8 ? 2 * L::kConv : 2;        // entries of a pair (by four warps)
             else if ((i >= kBarPFull && i < kBarPFull + 2) || i == kBarQConv || i == kBarQConv + 1) n = 4;   // softmax warps
             else if (i >= kBarItemEmpty) n = 1 + 8 + (E8 ? L::kConv : 2);                // MMA, softmax, converting or helping warps
             mbar_init(bar(i), n);
@@ -227,15 +234,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             };
             // entry: K (which = 0) or V of kv tile t, whose pages are pg
             auto load_entry = [&](const Item& it, int which, int t, int pg, bool edge) -> bool {
-                const int g = (r + 1) >> 1, slot = g & 1;
+                const int g = (r + 1) >> 1, slot = slot_of(g);
                 if ((r & 1) || r == 0) {      // the pair's first entry: its slot must have been released
-                    if (!__all_sync(0xffffffffu, mbar_wait(bar(kBarKVEmpty + slot), ((g >> 1) & 1) ^ 1u, abort_flag, 2))) return false;
+                    if (!__all_sync(0xffffffffu, mbar_wait(bar(kBarKVEmpty + slot), turn_of(g) ^ 1u, abort_flag, 2))) return false;
                     if (r == 0 && lane == 0) mbar_arrive(bar(kBarKVFull + slot));
                 }
                 const uint32_t full = bar(edge ? kBarVLand + slot : kBarKVFull + slot);
                 if (!which) {
                     const uint32_t there = __ballot_sync(0xffffffffu, pg >= 0);
-                    if (lane == 0) bits[g & 3] = there;
+                    if (lane == 0) bits[g & kBitsMask] = there;
                 }
                 if (lane == 0) mbar_arrive_expect_tx(full, kChunks * kChunkBytes);
                 __syncwarp();
@@ -336,7 +343,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 if (at < range.end) nt = item_tiles(p, sq, qi, pt);
             }
             if (ok) {
-                if (!E8 && r > 0 && lane == 0) mbar_arrive(bar(kBarKVFull + ((r >> 1) & 1)));   // the last pair has no K
+                if (!E8 && r > 0 && lane == 0) mbar_arrive(bar(kBarKVFull + slot_of(r >> 1)));   // the last pair has no K
                 Item end{};
                 put(end);
             }
@@ -347,7 +354,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             constexpr uint32_t idesc_pv = instr_desc_f16(kBfOps ? 1 : 0, BM, HD, false, true);
             auto issue_qk = [&](int t, int pair) {
                 const uint32_t qa = base + kSmemQ + t * kTileBytes;
-                const uint32_t ka = base + kSmemKV + (pair & 1) * kPairBytes + kTileBytes;
+                const uint32_t ka = base + kSmemKV + slot_of(pair) * kPairBytes + kTileBytes;
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -358,7 +365,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     }
             };
             auto issue_pv = [&](int t, int pair, bool acc) {
-                const uint32_t va = base + kSmemKV + (pair & 1) * kPairBytes;
+                const uint32_t va = base + kSmemKV + slot_of(pair) * kPairBytes;
 #pragma unroll
                 for (int ks = 0; ks < BN / 16; ++ks)
                     mma_ts(tmem + kColO + t * 128, tmem + kColS + t * 128 + ks * 8, smem_desc_sw128(va + ks * 16 * 128, kChunkBytes, 1024),
@@ -375,7 +382,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     const int nt[2] = {items[seq % kItems].ntile[0], items[seq % kItems].ntile[1]};
                     mbar_arrive(bar(kBarItemEmpty + seq % kItems));
                     if (n == 0) break;
-                    if (!have) ok = mbar_wait(bar(kBarKVFull + (G & 1)), (G >> 1) & 1, abort_flag, 3);
+                    if (!have) ok = mbar_wait(bar(kBarKVFull + slot_of(G)), turn_of(G), abort_flag, 3);
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         if (ok && nt[t] > 0) {
@@ -389,10 +396,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         }
                     }
                     if (!ok) break;
-                    tc_commit(bar(kBarKVEmpty + (G & 1)));
+                    tc_commit(bar(kBarKVEmpty + slot_of(G)));
                     for (int j = 0; ok && j < n; ++j) {
                         const int g = G + j + 1;          // (V_j, K_j+1)
-                        ok = mbar_wait(bar(kBarKVFull + (g & 1)), (g >> 1) & 1, abort_flag, 3);
+                        ok = mbar_wait(bar(kBarKVFull + slot_of(g)), turn_of(g), abort_flag, 3);
                         if (!ok) break;
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
@@ -412,7 +419,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                             }
                         }
                         if (!ok) break;
-                        if (j + 1 < n) tc_commit(bar(kBarKVEmpty + (g & 1)));   // the last one also holds the next item's K0
+                        if (j + 1 < n) tc_commit(bar(kBarKVEmpty + slot_of(g)));   // the last one also holds the next item's K0
                     }
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
@@ -426,15 +433,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             // ------------------------------ zeros past the end of a sequence (V) ------------------------------
             Item it;
             int G = 0;
-            uint32_t ecnt[2] = {0, 0};
+            uint32_t turns = 0;                 // bit per slot: parity of its next edge
             for (uint32_t seq = 0; get_item(seq, &it, 14); ++seq) {
                 G += it.n;                              // the last tile's V is in pair G (after this)
                 if (warp != kHelpWarp || !it.edge) continue;
-                const int slot = G & 1;
-                const uint32_t phase = slot ? ecnt[1] : ecnt[0];
-                if (!__all_sync(0xffffffffu, mbar_wait(bar(kBarVLand + slot), phase & 1u, abort_flag, 15))) break;
-                if (slot) ++ecnt[1];
-                else ++ecnt[0];
+                const int slot = slot_of(G);
+                if (!__all_sync(0xffffffffu, mbar_wait(bar(kBarVLand + slot), (turns >> slot) & 1u, abort_flag, 15))) break;
+                turns ^= 1u << slot;
                 const int r0 = it.kfin - (it.kv0 + it.n - 1) * BN, r1 = (r0 + (1 << p.box_shift) - 1) >> p.box_shift << p.box_shift;   // the page's rest
                 for (int i = lane; i < (r1 - r0) * kChunks * 8; i += 32) {
                     const int row = r0 + i / (kChunks * 8), u = i % (kChunks * 8);
@@ -529,9 +534,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         rows2 = rows_for(nx, nxx, pg2);
                         ex2 = exps_for(nx, nxx, pg2);
                     }
-                    const int g = (r + 1) >> 1, slot = g & 1;
+                    const int g = (r + 1) >> 1, slot = slot_of(g);
                     if ((r & 1) || r == 0) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarKVEmpty + slot), ((g >> 1) & 1) ^ 1u, abort_flag, 2));
+                        ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarKVEmpty + slot), turn_of(g) ^ 1u, abort_flag, 2));
                         if (!ok) break;
                         if (r == 0 && lane == 0) mbar_arrive(bar(kBarKVFull + slot));
                     }
@@ -539,7 +544,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         // bit i: page i of the tile is there, from the warp that has its first row
                         const int key = lane << p.box_shift, mine = __shfl_sync(0xffffffffu, pg, key & 31);
                         const uint32_t there = __ballot_sync(0xffffffffu, lane < npg && key >> 5 == w && mine >= 0);
-                        if (lane == 0) reinterpret_cast<volatile uint8_t*>(gen + L::kBits)[4 * (g & 3) + w] = uint8_t(there >> ((w * 32) >> p.box_shift));
+                        if (lane == 0) reinterpret_cast<volatile uint8_t*>(gen + L::kBits)[4 * (g & kBitsMask) + w] = uint8_t(there >> ((w * 32) >> p.box_shift));
                     }
                     // 2^e of this lane's row, fp16 twice
                     {
@@ -598,7 +603,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 more = next_more;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            if (ok && r > 0 && lane == 0) mbar_arrive(bar(kBarKVFull + ((r >> 1) & 1)));   // the last pair has no K
+            if (ok && r > 0 && lane == 0) mbar_arrive(bar(kBarKVFull + slot_of(r >> 1)));   // the last pair has no K
         }
     } else {
         // ------------------------------ softmax and results ------------------------------
@@ -689,7 +694,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     rescale_o(alpha);
                     m = m_next;
                 }
-                uint32_t there = bits[g & 3];
+                uint32_t there = bits[g & kBitsMask];
                 if constexpr (E8) {                              // (a byte per converting warp)
                     const uint32_t of = there;
                     there = 0u;
@@ -862,9 +867,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 template <bool BF16, bool E8, int HD>
 int launch(int gpu, int G, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
            const PagedWorkspace& ws) {
-    constexpr int bytes = Layout<E8>::kLaunch;
+    constexpr int bytes = Layout<E8, HD>::kLaunch;
     PB_CUDA((paged_allow_smem<paged_tc_kernel<BF16, E8, HD>>(gpu, bytes)));
-    PB_CUDA(paged_launch(paged_tc_kernel<BF16, E8, HD>, dim3(unsigned(G)), Layout<E8>::kThreads, bytes, s, mq, mk, mv, p, ws));
+    PB_CUDA(paged_launch(paged_tc_kernel<BF16, E8, HD>, dim3(unsigned(G)), Layout<E8, HD>::kThreads, bytes, s, mq, mk, mv, p, ws));
     return PARAS_OK;
 }
 

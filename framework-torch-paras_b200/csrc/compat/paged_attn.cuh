@@ -70,10 +70,9 @@ int paged_simt_launch(const PagedParams& p, int dtype, bool cache8, cudaStream_t
 // Their unit of work is a tile: 128 positions of the cache for one item (the query rows that share a pass over a kv
 // head's keys).  All W tiles of a call stand in one row, sequence by sequence, and CTA c of G takes those from c*W/G to
 // (c+1)*W/G (with fewer tiles than CTAs, G = W of them take one each): every CTA streams the same amount whatever the
-// lengths are, and the host need not know them.  An item cut by
-// such a border leaves partial results in the workspace, at most two per CTA (slot 2c for the item that the CTA starts
-// in the middle of or at its first tile, 2c+1 for a later one that goes on in the next CTA), and a second kernel, whose
-// block c looks after the item that starts in CTA c and goes on, joins them in the order of the CTAs.
+// lengths are, and the host need not know them.  An item cut by such a border leaves partial results in the workspace, at
+// most two per CTA (slot 2c for the item that the CTA starts in the middle of or at its first tile, 2c+1 for a later one
+// that goes on in the next CTA), and a second kernel joins the parts of each such item in the order of the CTAs.
 constexpr int kTileKeys = 128;
 
 struct PagedRange {
@@ -83,7 +82,7 @@ struct PagedRange {
     __device__ __forceinline__ int owner(int64_t x) const { return int(((x + 1) * ctas - 1) / total); }
 };
 
-// What block c of the joining kernel has to know; written by CTA c of the streaming kernel.
+// What the joining kernel has to know of the item that starts in CTA c and goes on; written by that CTA.
 struct PagedJoin {
     int first_slot;   // -1: nothing to join
     int last_cta;     // parts: first_slot, then slot 2*k for the CTAs up to this one
@@ -179,13 +178,19 @@ __device__ __forceinline__ PagedRange paged_range(int B, int64_t* sums, Tiles ti
     return r;
 }
 
-// Lets `Kernel` use `bytes` of dynamic shared memory on the current device `gpu`; asked of the driver once per device.
+// Lets `Kernel` use `bytes` of dynamic shared memory on the current device `gpu`; asked of the driver once per device.  A kernel
+// that moves registers between its warps counts on `regs` a thread at launch: with fewer it would wait for them for ever.
 template <auto Kernel>
-cudaError_t paged_allow_smem(int gpu, int bytes) {
+cudaError_t paged_allow_smem(int gpu, int bytes, int regs = 0) {
     static std::atomic<uint64_t> done{0};
     const uint64_t bit = uint64_t(1) << (gpu & 63);
     if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && regs > 0) {
+        cudaFuncAttributes at;
+        e = cudaFuncGetAttributes(&at, Kernel);
+        if (e == cudaSuccess && at.numRegs < regs) e = cudaErrorLaunchOutOfResources;
+    }
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return e;
 }

@@ -868,7 +868,7 @@ template <bool BF16, bool E8, int HD>
 int launch(int gpu, int G, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& p,
            const PagedWorkspace& ws) {
     constexpr int bytes = Layout<E8, HD>::kLaunch;
-    PB_CUDA((paged_allow_smem<paged_tc_kernel<BF16, E8, HD>>(gpu, bytes)));
+    PB_CUDA((paged_allow_smem<paged_tc_kernel<BF16, E8, HD>>(gpu, bytes, Layout<E8, HD>::kAtLaunch)));
     PB_CUDA(paged_launch(paged_tc_kernel<BF16, E8, HD>, dim3(unsigned(G)), Layout<E8, HD>::kThreads, bytes, s, mq, mk, mv, p, ws));
     return PARAS_OK;
 }

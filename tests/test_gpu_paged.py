@@ -420,6 +420,35 @@ def test_workspaces(q_lens):
             assert torch.equal(o, w)
 
 
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [90, 1, 5]], ids=["token", "chunk"])
+def test_captured_calls_that_run_at_the_same_time(q_lens):
+    # scratch from the pool: each graph has its own, on whatever stream it is replayed
+    kv = [3000, 700, 2000]
+    c = Cache(kv, 2, 128, 16, BF, False)
+    cu = cu_of(q_lens)
+    qs = [rand(sum(q_lens), 8, 128, dtype=BF, seed=i) for i in range(3)]
+    want = [abi.paged_attention(q, *c.cache, c.table, c.kv_lens, cu, max(q_lens)) for q in qs]
+    outs = [torch.empty_like(q) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    graphs = []
+    for q, o, s in zip(qs, outs, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            for _ in range(4):
+                abi.paged_attention(q, *c.cache, c.table, c.kv_lens, cu, max(q_lens), out=o)
+        graphs.append(g)
+    for turn in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for i in range(3):
+            with torch.cuda.stream(streams[(i + turn) % 3]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
 def test_a_given_stream():
     q_lens, kv = [1, 40], [300, 500]
     c = Cache(kv, 2, 128, 16, BF, False)

@@ -39,7 +39,7 @@ struct PagedParams {
 struct PagedSeq {
     int row0, nq;
     int kv;       // positions 0 .. kv-1, kv <= cap
-    int pos0;     // position of the first new token (may be negative or past kv)
+    int pos0;     // position of the first new token (may be negative or past kv); pos0 + count is kv_lens[b] or negative
 };
 __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
     PagedSeq s;
@@ -50,7 +50,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
     s.nq = min(count, p.max_q);
     if (s.nq < p.q_min || s.nq > p.q_max) s.nq = 0;
     s.kv = max(0, min(kv, p.cap));
-    s.pos0 = int(max(int64_t(-(1 << 30)), min(int64_t(kv) - count, int64_t(1 << 30))));
+    s.pos0 = int(max(int64_t(-(1 << 30)), int64_t(kv) - count));
     return s;
 }
 // Keys that new token i of the sequence attends: positions 0 .. n-1.

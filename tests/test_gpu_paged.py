@@ -484,6 +484,30 @@ def test_rows_of_nothing_but_nan():
                 assert torch.equal(got.cpu().nan_to_num(), want.nan_to_num())
 
 
+@pytest.mark.parametrize("q_lens", [[2], [40]], ids=["token", "chunk"])
+def test_positions_past_2_30(q_lens):
+    # one page of zeros again and again, then one whose keys outweigh them all: it has to be found at its place
+    page, n, D = 32768, q_lens[0], 64
+    k = torch.zeros(2, 1, page, D, dtype=torch.uint8, device=DEV).view(E4M3)
+    v = torch.zeros_like(k)
+    exps = [torch.full((2, 1, page), 127, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    last = 100
+    k[1, 0, :last] = torch.full((D,), 8.0, device=DEV).to(E4M3)
+    v[1, 0, :last] = torch.arange(1, last + 1, device=DEV).float()[:, None].expand(last, D).to(E4M3)
+    whole = (1 << 30) // page
+    table = torch.zeros(1, whole + 1, dtype=torch.int32, device=DEV)
+    table[0, whole] = 1
+    kv = torch.tensor([whole * page + last], dtype=torch.int32, device=DEV)
+    q = torch.ones(n, 1, D, dtype=BF, device=DEV)
+    out, lse = abi.paged_attention(q, k, v, table, kv, cu_of([n]), n, scale=1 / 8.0, k_exp=exps[0], v_exp=exps[1], return_lse=True)
+    seen = last - n + 1 + torch.arange(n)
+    vals = v[1, 0, :last, 0].cpu().double()
+    want = torch.stack([vals[:m].mean() for m in seen])          # (the zeros weigh 2^30 e^-64 of a key)
+    u = torch.finfo(BF).eps / 2
+    assert ((out[:, 0].cpu().double() - want[:, None]).abs() <= 2.0 * u * want[:, None]).all()
+    assert ((lse[:, 0].cpu().double() - (64 + seen.double().log())).abs() <= 1e-4).all()
+
+
 # ---------------------------------------------------------------- writing and reading
 
 def rows_for(T, H, D, dtype, seed):

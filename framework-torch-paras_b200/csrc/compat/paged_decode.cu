@@ -55,8 +55,8 @@ template <bool E8, int HD> struct Ring {
     static constexpr int kFit = (224 * 1024 - kMergeBytes) / kBytes;
     static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
     static constexpr int kMerge = kStages * kBytes;
-    static constexpr int kMl = kMerge + kMergeBytes;               // [8][16] maxima, [8][16] sums
-    static constexpr int kMeta = kMl + 2 * kConsumers * kRows * 4;
+    static constexpr int kMl = kMerge + kMergeBytes;               // [8][16] maxima, [8][16] sums, of this item and the last
+    static constexpr int kMeta = kMl + 4 * kConsumers * kRows * 4;
     static constexpr int kSums = kMeta + kMaxStages * kMetaBytes;
     static constexpr int kThreads = threads_of(E8);
     static constexpr int kBars = kSums + (kThreads / 32 + 3) * 8;
@@ -379,6 +379,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         float* merge = reinterpret_cast<float*>(gen + R::kMerge);
         float* m_sm = reinterpret_cast<float*>(gen + R::kMl);
         float* l_sm = m_sm + kConsumers * kRows;
+        int other = 2 * kConsumers * kRows;     // to the next item's maxima and sums
         uint32_t qf[HD / 16][4];
         float acc[HD / 8][4];
         float m_run[2], l_run[2];       // reference (in units of S) and sum of a row
@@ -629,7 +630,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
                     l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
                 }
-                merge_sync();       // the previous item's merge has been read
+                // (the previous item's maxima and sums lie elsewhere, so that only the barrier behind these is needed: who passes
+                // it has read all of the previous merge)
                 if (t == 0) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -657,6 +659,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     const float mw = m_sm[w * kRows + r];
                     if (mw != -INFINITY) l = fmaf(l_sm[w * kRows + r], ex2_approx(mw - M), l);
                 }
+                m_sm += other;
+                l_sm += other;
+                other = -other;
                 const float inv = M == -INFINITY ? 0.f : 1.0f / l;
                 const int tok = row_tok + r / p.group, hq = hk * p.group + r % p.group;
                 const size_t at = size_t(slot) * kRows + r;

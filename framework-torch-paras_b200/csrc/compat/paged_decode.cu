@@ -24,6 +24,7 @@
 // consumer warps do not fit (128 registers a thread: 173 us), e4m3 by shifts instead of conversions costs more instructions
 // than it saves (157 us; half and half 142), 32 keys a warp on every other tile brought nothing.
 #include <cmath>
+#include <type_traits>
 
 #include "paged_attn.cuh"
 #include "tc_prims.cuh"
@@ -648,71 +649,80 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, m_sm[w * kRows + r0 + 8 * h]);
                     f[h] = m_run[h] == -INFINITY ? 0.f : ex2_approx(m_run[h] * c2[h] - M);
                 }
-                // Sixteen threads finish a row; its maximum and sum are found once.
-                constexpr int kCols = R::kMergeCols, kMine = kCols / 16;
-                const int r = threadIdx.x >> 4, cp = threadIdx.x & 15;
-                float M = -INFINITY, l = 0.f;
+                // The outputs of R rows, COLS columns at a time, through [warp][R][COLS] fp32 in shared memory; 256 / R threads
+                // finish a row, whose maximum and sum they find once.
+                const float *m_in = m_sm, *l_in = l_sm;
+                auto finish = [&](auto rows_c, auto cols_c) {
+                    constexpr int RC = decltype(rows_c)::value, kCols = decltype(cols_c)::value;
+                    constexpr int kPerRow = kConsumers * 32 / RC, kMine = kCols / kPerRow;
+                    static_assert(kMine >= 2 && kConsumers * RC * kCols * 4 <= R::kMergeBytes, "");
+                    const int r = threadIdx.x / kPerRow, cp = threadIdx.x % kPerRow;
+                    float M = -INFINITY, l = 0.f;
 #pragma unroll
-                for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, m_sm[w * kRows + r]);
+                    for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, m_in[w * kRows + r]);
 #pragma unroll
-                for (int w = 0; w < kConsumers; ++w) {
-                    const float mw = m_sm[w * kRows + r];
-                    if (mw != -INFINITY) l = fmaf(l_sm[w * kRows + r], ex2_approx(mw - M), l);
-                }
+                    for (int w = 0; w < kConsumers; ++w) {
+                        const float mw = m_in[w * kRows + r];
+                        if (mw != -INFINITY) l = fmaf(l_in[w * kRows + r], ex2_approx(mw - M), l);
+                    }
+                    const float inv = M == -INFINITY ? 0.f : 1.0f / l;
+                    const int tok = row_tok + r / p.group, hq = hk * p.group + r % p.group;
+                    const size_t at = size_t(slot) * kRows + r;
+                    uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.os[0] + int64_t(hq) * p.os[1];
+                    if (r < rows && cp == 0) {
+                        if (flags & 4) ws.ml[at] = make_float2(M, l);
+                        else if (p.lse) p.lse[int64_t(tok) * p.Hq + hq] = M == -INFINITY ? -INFINITY : M * 0.6931471805599453f + logf(l);
+                    }
+                    // groups of 8 columns are exchanged by row so that the rows lie on different banks
+#pragma unroll
+                    for (int c = 0; c < HD / kCols; ++c) {
+                        if (c > 0) merge_sync();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int rr = r0 + 8 * h;
+                            if (rr < rows && rr < RC) {
+                                float* dst = merge + (warp * RC + rr) * kCols;
+#pragma unroll
+                                for (int x = 0; x < kCols / 8; ++x)
+                                    *reinterpret_cast<float2*>(dst + 8 * (x ^ (rr & (kCols / 8 - 1))) + 2 * t) =
+                                        make_float2(acc[c * (kCols / 8) + x][2 * h] * f[h], acc[c * (kCols / 8) + x][2 * h + 1] * f[h]);
+                            }
+                        }
+                        merge_sync();
+                        if (r < rows) {
+                            float o[kMine];
+#pragma unroll
+                            for (int e = 0; e < kMine; ++e) o[e] = 0.f;
+                            const int col = kMine * cp;
+                            const float* src = merge + r * kCols + 8 * ((col >> 3) ^ (r & (kCols / 8 - 1))) + (col & 7);
+#pragma unroll
+                            for (int w = 0; w < kConsumers; ++w)
+#pragma unroll
+                                for (int e = 0; e < kMine; e += 2) {
+                                    const float2 v = *reinterpret_cast<const float2*>(src + w * RC * kCols + e);
+                                    o[e] += v.x;
+                                    o[e + 1] += v.y;
+                                }
+#pragma unroll
+                            for (int e = 0; e < kMine; e += 2) {
+                                const int d = c * kCols + col + e;
+                                if (flags & 4) {
+                                    *reinterpret_cast<float2*>(ws.o + at * HD + d) = make_float2(o[e], o[e + 1]);
+                                } else {
+                                    const uint32_t w = pack16<BF16>(o[e] * inv, o[e + 1] * inv);
+                                    out[d] = uint16_t(w);
+                                    out[d + 1] = uint16_t(w >> 16);
+                                }
+                            }
+                        }
+                    }
+                };
                 m_sm += other;
                 l_sm += other;
                 other = -other;
-                const float inv = M == -INFINITY ? 0.f : 1.0f / l;
-                const int tok = row_tok + r / p.group, hq = hk * p.group + r % p.group;
-                const size_t at = size_t(slot) * kRows + r;
-                uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.os[0] + int64_t(hq) * p.os[1];
-                if (r < rows && cp == 0) {
-                    if (flags & 4) ws.ml[at] = make_float2(M, l);
-                    else if (p.lse) p.lse[int64_t(tok) * p.Hq + hq] = M == -INFINITY ? -INFINITY : M * 0.6931471805599453f + logf(l);
-                }
-                // [warp][row][kCols] fp32, groups of 8 columns exchanged by row so that the rows lie on different banks
-#pragma unroll
-                for (int c = 0; c < HD / kCols; ++c) {
-                    if (c > 0) merge_sync();
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int rr = r0 + 8 * h;
-                        if (rr < rows) {
-                            float* dst = merge + (warp * kRows + rr) * kCols;
-#pragma unroll
-                            for (int x = 0; x < kCols / 8; ++x)
-                                *reinterpret_cast<float2*>(dst + 8 * (x ^ (rr & (kCols / 8 - 1))) + 2 * t) =
-                                    make_float2(acc[c * (kCols / 8) + x][2 * h] * f[h], acc[c * (kCols / 8) + x][2 * h + 1] * f[h]);
-                        }
-                    }
-                    merge_sync();
-                    if (r < rows) {
-                        float o[kMine];
-#pragma unroll
-                        for (int e = 0; e < kMine; ++e) o[e] = 0.f;
-                        const int col = kMine * cp;
-                        const float* src = merge + r * kCols + 8 * ((col >> 3) ^ (r & (kCols / 8 - 1))) + (col & 7);
-#pragma unroll
-                        for (int w = 0; w < kConsumers; ++w)
-#pragma unroll
-                            for (int e = 0; e < kMine; e += 2) {
-                                const float2 v = *reinterpret_cast<const float2*>(src + w * kRows * kCols + e);
-                                o[e] += v.x;
-                                o[e + 1] += v.y;
-                            }
-#pragma unroll
-                        for (int e = 0; e < kMine; e += 2) {
-                            const int d = c * kCols + col + e;
-                            if (flags & 4) {
-                                *reinterpret_cast<float2*>(ws.o + at * HD + d) = make_float2(o[e], o[e + 1]);
-                            } else {
-                                const uint32_t w = pack16<BF16>(o[e] * inv, o[e + 1] * inv);
-                                out[d] = uint16_t(w);
-                                out[d + 1] = uint16_t(w >> 16);
-                            }
-                        }
-                    }
-                }
+                constexpr int kWhole = R::kMergeBytes / (kConsumers * HD * 4);     // rows that all columns are there for at once
+                if (kWhole < kRows && rows <= kWhole) finish(std::integral_constant<int, kWhole < kRows ? kWhole : kRows>(), std::integral_constant<int, HD>());
+                else finish(std::integral_constant<int, kRows>(), std::integral_constant<int, R::kMergeCols>());
             }
         }
     }

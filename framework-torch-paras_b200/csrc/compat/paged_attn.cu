@@ -103,7 +103,7 @@ int check(const paras_paged_attn_args* args, const char* what) {
 }
 
 // At most 16 query rows per kv head stream through mma.sync tiles (64 single tokens over 512 .. 16384 positions: 340 us, in
-// 128-row tiles 441; 48 x 4 tokens: 146 and 199, from an 8-bit cache 126 and 320; one token over 1000: 12.0 and 14.3), more go
+// 128-row tiles 441; 48 x 4 tokens: 144 and 199, from an 8-bit cache 122 and 320; one token over 1000: 12.0 and 14.3), more go
 // to the tensor-core tiles of 128 rows; fp32, other head dims than 64 and 128, pages that no tile of 128 positions is made of,
 // and unaligned tensors to CUDA cores.
 // A call for chunks whose sequences besides the longest average less than twice 16 rows is taken to mix both, and makes a

@@ -17,12 +17,13 @@
 // the 16-bit type that multiplies V, as in the dense kernels; maxima, sums and accumulators are fp32.
 //
 // Measured (32 query heads over 8 kv heads of 128).  64 single tokens over 512 .. 16384 positions, bf16: 340 to 346 us with
-// pages of 64 or 16, 6.5 TB/s, what a copy gets.  One token over 1000 positions: 12.1 us with the join, all latency.
-// 48 x 4 tokens over up to 8192 positions of an 8-bit cache: 126 us, 3.4 TB/s (a 16-bit one 146): there the consumers'
+// pages of 64 or 16, 6.5 TB/s, what a copy gets; 256 over 200 .. 1000 118 us (5.4 TB/s), 128 over 100 .. 300 44 us, where items'
+// starts and ends count.  One token over 1000 positions: 12 us with the join, all latency.
+// 48 x 4 tokens over up to 8192 positions of an 8-bit cache: 122 us, 3.5 TB/s (a 16-bit one 144): there the consumers'
 // instructions bound it, not the memory.  A warp's part of a tile takes 1440 cycles, at 442 instructions and two warps on a
-// scheduler, and about 330 go by around it, where the loads alone would allow 1350; an item's merge takes 3700.  Twelve
-// consumer warps do not fit (128 registers a thread: 173 us), e4m3 by shifts instead of conversions costs more instructions
-// than it saves (157 us; half and half 142), 32 keys a warp on every other tile brought nothing.
+// scheduler, and about 300 go by around it, where the loads alone would allow 1350.  Twelve consumer warps do not fit (128
+// registers a thread: 173 us), e4m3 by shifts instead of conversions costs more instructions than it saves (157 us; half and
+// half 142), 32 keys a warp on every other tile brought nothing.
 #include <cmath>
 #include <type_traits>
 
@@ -64,10 +65,10 @@ template <bool E8, int HD> struct Ring {
     static constexpr int kMisc = kBars + (2 * kMaxStages + 1) * 8 + 8;
     static constexpr int kLaunch = kMisc + 16 + 1024;
     static_assert(kLaunch <= 227 * 1024, "shared memory of a CTA");
-    static_assert(kBytes % 1024 == 0 && kSums % 8 == 0, "alignment");
+    static_assert(kBytes % 1024 == 0 && kMeta % 16 == 0 && kSums % 8 == 0, "alignment");
 };
 
-struct TileMeta {        // kMetaBytes, one per stage
+struct alignas(16) TileMeta {        // kMetaBytes, one per stage
     int key0;
     int flags;           // 1 first tile of the item here, 2 last, 4 the item is not whole here, 8 keys are to be masked
     uint32_t pages;      // bit i: page i of the tile is there
@@ -381,17 +382,22 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         float* m_sm = reinterpret_cast<float*>(gen + R::kMl);
         float* l_sm = m_sm + kConsumers * kRows;
         int other = 2 * kConsumers * kRows;     // to the next item's maxima and sums
+        // row / group without a division for every item (rows below 16, groups up to 16); kept for this thread's rows where
+        // registers are short
+        const int by_group = E8 ? (65536 + p.group - 1) / p.group : 0;
+        const int toks[2] = {E8 ? 0 : r0 / p.group, E8 ? 0 : (r0 + 8) / p.group};
         uint32_t qf[HD / 16][4];
         float acc[HD / 8][4];
         float m_run[2], l_run[2];       // reference (in units of S) and sum of a row
         float c2[2], lag[2];            // S * c2 is the exponent of 2; 2^8 in units of S
+        const float lag0 = 8.f / p.scale_log2;
         int lim[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             m_run[h] = -INFINITY;
             l_run[h] = 0.f;
             c2[h] = p.scale_log2;
-            lag[h] = 8.f / p.scale_log2;
+            lag[h] = lag0;
             lim[h] = 0;
         }
 #pragma unroll
@@ -416,16 +422,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (!__all_sync(0xffffffffu, mbar_wait(full(s), (i / R::kStages) & 1, abort_flag, 3))) break;
             const uint32_t kt = base + s * R::kBytes, vt = kt + R::kTile;
             const TileMeta& md = meta[s];
-            const int flags = md.flags, key0 = md.key0, kend = md.kend;
+            const int4 head = *reinterpret_cast<const int4*>(&md);       // key0, flags, pages, kend
+            const int flags = head.y, key0 = head.x, kend = head.w;
             if (flags & 1) {
                 // ---- a new item: query fragments, limits, empty state ----
                 const uint32_t qt = kt + R::kQ;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int r = r0 + 8 * h, tok = r / p.group;
+                    const int r = r0 + 8 * h;
                     m_run[h] = -INFINITY;
                     l_run[h] = 0.f;
-                    lim[h] = p.causal ? min(kend, md.pos0 + tok + 1) : kend;
+                    lim[h] = p.causal ? min(kend, md.pos0 + (E8 ? (r * by_group) >> 16 : toks[h]) + 1) : kend;
                     if constexpr (!E8) {
                         // a0/a1: d = 16 ks + 2t (+1); a2/a3: d + 8
 #pragma unroll
@@ -456,7 +463,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             const int ex = max(-120, min(120, int(__float_as_uint(amax) >> 23) - 127));
                             const float f = pow2f(-ex);
                             c2[h] = fmaxf(p.scale_log2 * pow2f(ex), kLeastC2);
-                            lag[h] = 8.f / c2[h];
+                            lag[h] = fminf(lag0 * f, 1e37f);       // (8 / c2)
 #pragma unroll
                             for (int ks = 0; ks < HD / 16; ++ks) {
                                 const float2 x = pair16_to_f32<true>(qf[ks][h]), y = pair16_to_f32<true>(qf[ks][2 + h]);
@@ -649,8 +656,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, m_sm[w * kRows + r0 + 8 * h]);
                     f[h] = m_run[h] == -INFINITY ? 0.f : ex2_approx(m_run[h] * c2[h] - M);
                 }
-                // The outputs of R rows, COLS columns at a time, through [warp][R][COLS] fp32 in shared memory; 256 / R threads
-                // finish a row, whose maximum and sum they find once.
+                // The outputs of RC rows, kCols columns at a time, through [warp][RC][kCols] fp32 in shared memory; 256 / RC threads
+                // finish a row, whose maximum and sum they find once.  All columns at once where the rows are few: 128 single
+                // tokens over 100 .. 300 positions 60 us with 32 columns a pass, 49 in one.
                 const float *m_in = m_sm, *l_in = l_sm;
                 auto finish = [&](auto rows_c, auto cols_c) {
                     constexpr int RC = decltype(rows_c)::value, kCols = decltype(cols_c)::value;
@@ -666,7 +674,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         if (mw != -INFINITY) l = fmaf(l_in[w * kRows + r], ex2_approx(mw - M), l);
                     }
                     const float inv = M == -INFINITY ? 0.f : 1.0f / l;
-                    const int tok = row_tok + r / p.group, hq = hk * p.group + r % p.group;
+                    const int rt = E8 ? (r * by_group) >> 16 : r / p.group, tok = row_tok + rt, hq = hk * p.group + (r - rt * p.group);
                     const size_t at = size_t(slot) * kRows + r;
                     uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(tok) * p.os[0] + int64_t(hq) * p.os[1];
                     if (r < rows && cp == 0) {

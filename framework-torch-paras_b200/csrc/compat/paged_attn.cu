@@ -42,6 +42,7 @@ paged_simt_kernel(const PagedParams p) {
     __syncwarp();
     const int n = paged_keys(p, sq, i);
     float m = -INFINITY, l = 0.f, acc[8];
+    bool nan = false;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
     for (int j0 = 0; j0 < n; j0 += 32) {
@@ -62,6 +63,7 @@ paged_simt_kernel(const PagedParams p) {
                 s = dot * p.scale;
             }
         }
+        nan = nan || __any_sync(0xffffffffu, s != s);      // (maxima skip it)
         const float m_new = fmaxf(m, warp_max(s));
         if (m_new == -INFINITY) continue;     // nothing attended so far
         const float alpha = expf(m - m_new);
@@ -82,11 +84,11 @@ paged_simt_kernel(const PagedParams p) {
         }
     }
     T* orow = static_cast<T*>(p.out) + int64_t(t) * p.os[0] + int64_t(h) * p.os[1];
-    const float inv = m == -INFINITY ? 0.f : 1.0f / l;
+    const float inv = nan ? NAN : m == -INFINITY ? 0.f : 1.0f / l;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         if (lane + 32 * e < p.D) orow[lane + 32 * e] = from_f32<T>(acc[e] * inv);
-    if (p.lse && lane == 0) p.lse[unit] = m == -INFINITY ? -INFINITY : m + logf(l);
+    if (p.lse && lane == 0) p.lse[unit] = nan ? NAN : m == -INFINITY ? -INFINITY : m + logf(l);
 }
 
 int check(const paras_paged_attn_args* args, const char* what) {

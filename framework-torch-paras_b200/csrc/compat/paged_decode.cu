@@ -643,7 +643,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (t == 0) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        m_sm[warp * kRows + r0 + 8 * h] = m_run[h] * c2[h];      // (exponents of 2 from here on)
+                        // (exponents of 2 from here on; scores of nothing but NaN leave no maximum, but their sum has to count)
+                        m_sm[warp * kRows + r0 + 8 * h] = m_run[h] == -INFINITY && l_run[h] != l_run[h] ? 0.f : m_run[h] * c2[h];
                         l_sm[warp * kRows + r0 + 8 * h] = l_run[h];
                     }
                 }

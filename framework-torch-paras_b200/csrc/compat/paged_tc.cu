@@ -773,7 +773,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (!ok) break;
             ++ocnt;
             tc_fence_after_sync();
-            const bool none = m == -INFINITY;
+            // (scores of nothing but NaN leave no maximum either, but a sum that is NaN: the row's results are)
+            const bool none = m == -INFINITY && l == l;
+            const float m2 = m == -INFINITY ? 0.f : m * c2;
             const int live = min(pt, it.nq - t * pt) * p.group;            // rows of this tile that are tokens
             const int crow = t * pt * p.group;                             // its first row in the item
             // Rows leave through the warp's staging buffer, so that a store writes whole pieces of kORow bytes of
@@ -808,7 +810,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                             *reinterpret_cast<uint4*>(ws.o + (size_t(it.slot) * 256 + crow + tr) * HD + kCols * c + 4 * u0) = v;
                     }
                 }
-                if (row < live) ws.ml[size_t(it.slot) * 256 + crow + row] = make_float2(none ? -INFINITY : m * c2, l);
+                if (row < live) ws.ml[size_t(it.slot) * 256 + crow + row] = make_float2(none ? -INFINITY : m2, l);
             } else {
                 constexpr int kCols = L::kORow / 2;
                 const float inv = none ? 0.f : 1.0f / l;
@@ -845,7 +847,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 }
                 if (p.lse && row < live) {
                     const int tok = it.row0 + t * pt + row / p.group, h = it.hk * p.group + row % p.group;
-                    p.lse[int64_t(tok) * p.Hq + h] = none ? -INFINITY : m * c2 * 0.6931471805599453f + logf(l);
+                    p.lse[int64_t(tok) * p.Hq + h] = none ? -INFINITY : m2 * 0.6931471805599453f + logf(l);
                 }
             }
             // (the next item's S_t, and with it the next write to O_t, waits for these warps' next P)

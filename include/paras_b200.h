@@ -437,7 +437,7 @@ int paras_b200_paged_kv_read(const paras_paged_kv_args* args);
  * of the new tokens themselves have to be in the cache already.  max_q bounds the new tokens of a sequence (queries
  * past it are not computed); the route is chosen by it.  A query that attends nothing (no position left, all
  * pages absent) gives zeros, with lse = -inf.  What lies in the cache past a sequence's last position is never used,
- * whatever it holds; K and V of the attended positions have to be finite.  `lse` (optional): fp32 [T, Hq] contiguous,
+ * whatever it holds; K and V of the attended positions have to be finite; a NaN in q makes its own row NaN.  `lse` (optional): fp32 [T, Hq] contiguous,
  * natural log of the sum of the exponentials of the scaled scores.  dtype F32, BF16 or F16; cache_dtype the same or
  * PARAS_E4M3.  D up to 256.  `workspace`: as for paras_b200_sdpa_fwd; size from paras_b200_paged_attn_workspace_bytes. */
 typedef struct paras_paged_attn_args {

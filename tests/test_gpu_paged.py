@@ -180,6 +180,26 @@ def test_queries_of_zero_and_scales_down_to_nothing(q_lens, cache8):
         check_attention(q_lens, [200, 300], 4, 1, 128, 16, BF, cache8, q=q, scale=1e39)
 
 
+@pytest.mark.parametrize("cache8", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("q_lens,kv", [([1, 1], [40, 30000]), ([3, 4], [40, 30000]), ([30, 25], [40, 30000])], ids=["token", "draft", "chunk"])
+def test_a_query_of_nan_stays_in_its_row(q_lens, kv, dtype, cache8):
+    # in an item that one block finishes, and in one that is cut between many
+    c = Cache(kv, 1, 64, 16, dtype, cache8)
+    T = sum(q_lens)
+    q = rand(T, 4, 64, dtype=dtype, seed=1)
+    args = (*c.cache, c.table, c.kv_lens, cu_of(q_lens), max(q_lens))
+    want, wlse = abi.paged_attention(q, *args, return_lse=True, **c.kw)
+    gone = torch.zeros(T, 4, dtype=torch.bool, device=DEV)
+    for row, head in ((0, 1), (T - 1, 2)):
+        q[row, head, 5] = float("nan")
+        gone[row, head] = True
+    out, lse = abi.paged_attention(q, *args, return_lse=True, **c.kw)
+    assert torch.isnan(out[gone]).all() and torch.isnan(lse[gone]).all()
+    tol = 4 * torch.finfo(dtype).eps      # (a row's neighbours may be summed against another reference: half a step of P and of the result, twice)
+    assert torch.allclose(out[~gone].float(), want[~gone].float(), rtol=tol, atol=tol) and torch.allclose(lse[~gone], wlse[~gone], atol=1e-4)
+
+
 def test_max_q_bounds_what_is_computed():
     c = Cache([50, 60], 1, 64, 16, BF, False)
     q = rand(30, 2, 64, dtype=BF, seed=2)

@@ -687,6 +687,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
                         tmem_st16(o_addr + 16 * c, o);
                     }
+                    tmem_wait_st();      // (a second rescaling in the same tile loads these columns again)
                 };
                 if (j > 0 && move_ref) {
                     const float alpha = m_next == m ? 1.f : ex2_approx((m - m_next) * c2);

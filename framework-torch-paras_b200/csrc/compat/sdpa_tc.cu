@@ -711,6 +711,7 @@ sdpa_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                         for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
                         tmem_st16(o_addr + 16 * c, o);
                     }
+                    tmem_wait_st();      // (a second rescaling in the same tile loads these columns again)
                 };
                 // Only the item's first tile looks for its row max before exponentiating: that pass
                 // heads the tile's dependency chain (S ready -> P ready -> next S ...).  Later tiles

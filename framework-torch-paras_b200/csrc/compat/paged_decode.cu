@@ -280,7 +280,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (mine >= 0 && exp4) {
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(k) : "memory");
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 128), "l"(v) : "memory");
-                } else {
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(s)) : "memory");
+                } else {      // (ordinary stores, which an ordinary arrival releases)
                     uint32_t ek = 0x7f7f7f7fu, ev = 0x7f7f7f7fu;
                     if (mine >= 0) {
                         ek = ev = 0;
@@ -292,8 +293,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(ek) : "memory");
                     asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + 128), "r"(ev) : "memory");
+                    mbar_arrive(full(s));
                 }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(s)) : "memory");
                 if (i + 1 < ntiles) advance();
             }
             asm volatile("cp.async.wait_all;" ::: "memory");

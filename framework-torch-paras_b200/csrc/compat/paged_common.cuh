@@ -57,6 +57,9 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
 }
 __device__ __forceinline__ float e4m3_to_f32(uint8_t b) { return e4m3x2_to_f32(b).x; }
 
+// Positions that a page table may reach: the kernels count them in 32 bits and step or round up by as many as 128 beyond.
+constexpr int64_t kMostPositions = (int64_t(1) << 31) - 256;
+
 // Checks shared by the entry points; `what` names the caller in the message.
 int check_paged_cache(const paras_paged_cache& c, int dtype, const char* what);
 

@@ -432,8 +432,8 @@ int check_paged_cache(const paras_paged_cache& c, int dtype, const char* what) {
     if (c.page < 1 || c.page > 65536) return fail(PARAS_E_INVALID, "%s: a page holds 1 to 65536 positions", what);
     if (c.D < 1 || c.D > 256) return fail(PARAS_E_UNSUPPORTED, "%s: head dim %d is not within 1..256", what, c.D);
     if (c.Hkv < 1) return fail(PARAS_E_INVALID, "%s: no kv heads", what);
-    if (int64_t(c.max_pages) * c.page > INT32_MAX)
-        return fail(PARAS_E_INVALID, "%s: max_pages * page exceeds 2^31 - 1 positions", what);
+    if (int64_t(c.max_pages) * c.page > kMostPositions)
+        return fail(PARAS_E_INVALID, "%s: max_pages * page exceeds 2^31 - 256 positions", what);
     if (c.B > 0 && c.max_pages > 0 && !c.page_table) return fail(PARAS_E_INVALID, "%s: null page table", what);
     if (c.pages > 0 && (!c.k || !c.v)) return fail(PARAS_E_INVALID, "%s: null cache", what);
     if (c.cache_dtype == PARAS_E4M3 && c.pages > 0 && (!c.k_exp || !c.v_exp))

@@ -389,7 +389,8 @@ int paras_b200_scale_columns(int gpu, const void* weight, const void* scale, voi
  * here leaves, give unspecified finite or infinite values.
  *
  * The sequences, all on the device, so that a captured launch follows them: page_table[b][i] (row stride
- * table_stride) is the page of positions i*page .. of sequence b, max_pages entries a row.  An entry outside
+ * table_stride) is the page of positions i*page .. of sequence b, max_pages entries a row (max_pages * page at most
+ * 2^31 - 256).  An entry outside
  * [0, pages) is an absent page: its positions are not written, read back as zeros and are not attended.
  * Sequence b owns the ragged rows cu[b] .. cu[b+1]-1 (cu is non-decreasing, B+1 entries) of the token tensors.  Rows
  * that belong to no sequence (below cu[0], from cu[B] on) are neither read nor written.

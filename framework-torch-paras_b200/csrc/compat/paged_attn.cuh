@@ -54,8 +54,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
     return s;
 }
 // Keys that new token i of the sequence attends: positions 0 .. n-1.
-__device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& s, int i) {
-    return p.causal ? max(0, min(s.kv, s.pos0 + i + 1)) : s.kv;
+__host__ __device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& s, int i) {
+    const int n = s.pos0 + i + 1;
+    return !p.causal ? s.kv : n < 0 ? 0 : n < s.kv ? n : s.kv;
 }
 
 // The streaming kernels move their reference by products with c2 = scale * log2(e) (times a row's power of two) and its
@@ -74,6 +75,21 @@ int paged_simt_launch(const PagedParams& p, int dtype, bool cache8, cudaStream_t
 // most two per CTA (slot 2c for the item that the CTA starts in the middle of or at its first tile, 2c+1 for a later one
 // that goes on in the next CTA), and a second kernel joins the parts of each such item in the order of the CTAs.
 constexpr int kTileKeys = 128;
+
+// Tiles of the kernel for chunks: an item is up to 2 * pt tokens of a sequence (two query tiles) and one kv head, and an item
+// with nothing to attend has one empty tile.  A head's tiles are counted in 64 bits: many items of long sequences pass 2^31.
+__host__ __device__ __forceinline__ int tiles_for(int keys) { return keys <= kTileKeys ? 1 : (keys + kTileKeys - 1) / kTileKeys; }
+__host__ __device__ __forceinline__ int item_tiles(const PagedParams& p, const PagedSeq& s, int i, int pt) {
+    const int end = (i + 1) * 2 * pt;
+    return tiles_for(paged_keys(p, s, (end < s.nq ? end : s.nq) - 1));
+}
+__host__ __device__ __forceinline__ int64_t head_tiles(const PagedParams& p, const PagedSeq& s, int pt) {
+    const int items = (s.nq + 2 * pt - 1) / (2 * pt);
+    if (!p.causal) return items > 0 ? int64_t(items) * tiles_for(s.kv) : 0;
+    int64_t n = 0;
+    for (int i = 0; i < items; ++i) n += item_tiles(p, s, i, pt);
+    return n;
+}
 
 struct PagedRange {
     int64_t total, ctas;    // W, G

@@ -98,18 +98,6 @@ struct Item {            // 64 bytes
 static_assert(sizeof(Item) == 64, "");
 
 __device__ __forceinline__ int keys_at(const PagedParams& p, int kv, int pos) { return p.causal ? max(0, min(kv, pos + 1)) : kv; }
-__device__ __forceinline__ int tiles_for(int keys) { return max(1, (keys + BN - 1) / BN); }
-// tiles of item i of a sequence (per kv head); items are 2 * pt tokens
-__device__ __forceinline__ int item_tiles(const PagedParams& p, const PagedSeq& s, int i, int pt) {
-    return tiles_for(paged_keys(p, s, min(s.nq, (i + 1) * 2 * pt) - 1));
-}
-__device__ __forceinline__ int head_tiles(const PagedParams& p, const PagedSeq& s, int pt) {
-    const int items = (s.nq + 2 * pt - 1) / (2 * pt);
-    if (!p.causal) return items > 0 ? items * tiles_for(s.kv) : 0;
-    int n = 0;
-    for (int i = 0; i < items; ++i) n += item_tiles(p, s, i, pt);
-    return n;
-}
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 x;
@@ -167,7 +155,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     int b0;
     int64_t base0;
     const PagedRange range = paged_range(p.B, reinterpret_cast<int64_t*>(gen + L::kSums),
-                                         [&](int b) { return int64_t(p.Hkv) * head_tiles(p, paged_seq(p, b), pt); }, &b0, &base0);
+                                         [&](int b) { return p.Hkv * head_tiles(p, paged_seq(p, b), pt); }, &b0, &base0);
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -212,7 +200,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             };
             if (at < range.end) {
                 enter();
-                const int per = head_tiles(p, sq, pt);
+                const int64_t per = head_tiles(p, sq, pt);
                 int64_t in = at - base0;
                 hk = int(in / per);
                 in -= int64_t(hk) * per;

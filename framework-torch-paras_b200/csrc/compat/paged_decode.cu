@@ -554,7 +554,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 for (int h = 0; h < 2; ++h) {
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                    const float m_new = fmaxf(m_run[h], mx[h]);
+                    // a row goes by its own scores: its bits depend neither on its neighbours nor on the rows of the tile of
+                    // queries that no token fills, which hold anything
+                    const float m_new = mx[h] > m_run[h] + lag[h] ? mx[h] : m_run[h];
                     alpha[h] = m_new == m_run[h] ? 1.f : ex2_approx((m_run[h] - m_new) * c2[h]);
                     l_run[h] *= alpha[h];
                     m_run[h] = m_new;

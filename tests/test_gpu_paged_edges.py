@@ -44,3 +44,32 @@ def test_exponent_bytes_wherever_they_lie(q_lens, dtype, D):
         for k_exp, v_exp in zip(*ways):
             out, l2 = abi.paged_attention(*args, return_lse=True, k_exp=k_exp, v_exp=v_exp)
             assert torch.equal(out, ref) and torch.equal(l2, lse)
+
+
+@pytest.mark.parametrize("cache8", [False, True])
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 64)])
+def test_bits_do_not_depend_on_what_ran_before(dtype, D, cache8):
+    # a call for single tokens after one whose query rows fill whole tiles with other values: what its own tiles of query rows
+    # do not cover in shared memory must not show, and neither must a neighbour's row
+    kv = [30000, 700, 9000, 4100]
+    c = Cache(kv, 2, D, 16, dtype, cache8, seed=2)
+    q = rand(4, 8, D, dtype=dtype, seed=3)
+    args = (*c.cache, c.table, c.kv_lens)
+    before = [torch.zeros(16, 8, D, dtype=dtype, device=DEV)] + [rand(16, 8, D, dtype=dtype, seed=5 + i, scale=s)
+                                                                 for i, s in enumerate((1.0, 30.0, 300.0))]
+    ref = None
+    for turn in range(3):
+        for other in before:
+            abi.paged_attention(other, *args, cu_of([4] * 4), 4, **c.kw)
+            out, lse = abi.paged_attention(q, *args, cu_of([1] * 4), 1, return_lse=True, **c.kw)
+            assert abi.paged_attn_last_kernel() == "paged_decode"
+            ref = ref or (out, lse)
+            assert torch.equal(out, ref[0]) and torch.equal(lse, ref[1])
+    # one head's query changes: the others keep their bits
+    for scale in (0.0, 30.0):
+        q2 = q.clone()
+        q2[:, 1] *= scale
+        q2[:, 6] = float("nan")
+        out, lse = abi.paged_attention(q2, *args, cu_of([1] * 4), 1, return_lse=True, **c.kw)
+        for h in (0, 2, 3, 4, 5, 7):
+            assert torch.equal(out[:, h], ref[0][:, h]) and torch.equal(lse[:, h], ref[1][:, h])

@@ -122,6 +122,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     constexpr int kBitsMask = 2 * L::kPairs - 1;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::kMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::kMisc + 4);
+    // kv tiles the MMA warp has issued: waits that last a whole item (for its end, or for the next one) take their limit by it
+    volatile uint32_t* progress = reinterpret_cast<volatile uint32_t*>(gen + L::kMisc + 8);
     Item* items = reinterpret_cast<Item*>(gen + L::kItem);
     volatile uint32_t* bits = reinterpret_cast<volatile uint32_t*>(gen + L::kBits);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -136,6 +138,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             mbar_init(bar(i), n);
         }
         *abort_flag = 0;
+        *progress = 0;
         mbar_fence_init();
     }
     // rows that no token fills (128 is not a multiple of the group) stay zero
@@ -163,7 +166,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int npg = p.npg;              // pages (or, of larger pages, pieces) in a tile
     // Item i of this CTA for the warps that wait for it, false at the end; its descriptor stays until they let it go.
     auto wait_item = [&](uint32_t i, int tag) -> bool {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kBarItemFull + i % kItems), (i / kItems) & 1, abort_flag, tag))) return false;
+        if (!__all_sync(0xffffffffu, mbar_wait_progress(bar(kBarItemFull + i % kItems), (i / kItems) & 1, abort_flag, tag, progress))) return false;
         if (items[i % kItems].n > 0) return true;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarItemEmpty + i % kItems));
@@ -245,7 +248,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             };
             uint32_t seq = 0;
             auto put = [&](const Item& it) -> bool {
-                if (!__all_sync(0xffffffffu, mbar_wait(bar(kBarItemEmpty + seq % kItems), ((seq / kItems) & 1) ^ 1u, abort_flag, 12))) return false;
+                if (!__all_sync(0xffffffffu, mbar_wait_progress(bar(kBarItemEmpty + seq % kItems), ((seq / kItems) & 1) ^ 1u, abort_flag, 12, progress)))
+                    return false;
                 if (lane == 0) {
                     items[seq % kItems] = it;
                     mbar_arrive(bar(kBarItemFull + seq % kItems));
@@ -295,7 +299,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         if (ok && it.ntile[t] > 0) {
-                            ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarQEmpty + t), (qcnt[t] & 1u) ^ 1u, abort_flag, 0 + t));
+                            ok = __all_sync(0xffffffffu, mbar_wait_progress(bar(kBarQEmpty + t), (qcnt[t] & 1u) ^ 1u, abort_flag, 0 + t, progress));
                             if (!ok) break;
                             ++qcnt[t];
                             if (lane == 0) {
@@ -387,6 +391,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     tc_commit(bar(kBarKVEmpty + slot_of(G)));
                     for (int j = 0; ok && j < n; ++j) {
                         const int g = G + j + 1;          // (V_j, K_j+1)
+                        *progress = uint32_t(g);
                         ok = mbar_wait(bar(kBarKVFull + slot_of(g)), turn_of(g), abort_flag, 3);
                         if (!ok) break;
 #pragma unroll
@@ -426,7 +431,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 G += it.n;                              // the last tile's V is in pair G (after this)
                 if (warp != kHelpWarp || !it.edge) continue;
                 const int slot = slot_of(G);
-                if (!__all_sync(0xffffffffu, mbar_wait(bar(kBarVLand + slot), (turns >> slot) & 1u, abort_flag, 15))) break;
+                if (!__all_sync(0xffffffffu, mbar_wait_progress(bar(kBarVLand + slot), (turns >> slot) & 1u, abort_flag, 15, progress))) break;
                 turns ^= 1u << slot;
                 const int r0 = it.kfin - (it.kv0 + it.n - 1) * BN, r1 = (r0 + (1 << p.box_shift) - 1) >> p.box_shift << p.box_shift;   // the page's rest
                 for (int i = lane; i < (r1 - r0) * kChunks * 8; i += 32) {

@@ -83,6 +83,31 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity,
     return true;
 }
 
+// The same for a wait that lasts as long as another warp's whole piece of work, whatever that takes: the limit begins anew
+// whenever `*progress` (a shared-memory word that the working warp counts up, and whose own waits are bounded) has moved.
+__device__ __forceinline__ bool mbar_wait_progress(uint32_t bar, uint32_t parity, volatile int* abort_flag, int tag,
+                                                   const volatile uint32_t* progress, uint64_t limit_ns = kWaitLimitNs) {
+#pragma unroll 1
+    for (int i = 0; i < 2048; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    uint64_t t0 = global_timer_ns();
+    uint32_t polls = 0, seen = *progress;
+    while (!mbar_try_wait(bar, parity)) {
+        if ((++polls & 0xffu) == 0) {
+            const uint32_t now = *progress;
+            if (now != seen) {
+                seen = now;
+                t0 = global_timer_ns();
+            }
+            if (*abort_flag || global_timer_ns() - t0 > limit_ns) {
+                atomicOr(const_cast<int*>(abort_flag), int(0x40000000u | (1u << tag)));
+                return false;
+            }
+        }
+    }
+    return true;
+}
+
 // ---- TMA: 4-D tiled load global -> shared, completion on an mbarrier -------------------
 __device__ __forceinline__ void tma_load_4d(uint32_t dst_smem, const CUtensorMap* map,
                                             uint32_t bar, int c0, int c1, int c2, int c3) {

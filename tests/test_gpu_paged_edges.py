@@ -73,3 +73,34 @@ def test_bits_do_not_depend_on_what_ran_before(dtype, D, cache8):
         out, lse = abi.paged_attention(q2, *args, cu_of([1] * 4), 1, return_lse=True, **c.kw)
         for h in (0, 2, 3, 4, 5, 7):
             assert torch.equal(out[:, h], ref[0][:, h]) and torch.equal(lse[:, h], ref[1][:, h])
+
+
+@pytest.mark.parametrize("cache8", [False, True])
+def test_an_item_that_lasts_longer_than_any_wait(cache8):
+    # a sequence of 2^26 positions for every multiprocessor (all of one page of zeros, then one whose keys outweigh them): a
+    # block's item takes more than half a second, for all of which its idle warps wait for the next one
+    page, D, H, last = 32768, 64, 128, 100
+    B = torch.cuda.get_device_properties(0).multi_processor_count
+    whole = (1 << 26) // page
+    k, v = torch.zeros(2, 1, page, D, device=DEV), torch.zeros(2, 1, page, D, device=DEV)
+    k[1, 0, :last] = 8.0
+    v[1, 0, :last] = torch.arange(1, last + 1, device=DEV).float()[:, None]
+    kind = torch.float8_e4m3fn if cache8 else BF
+    k, v = k.to(kind), v.to(kind)
+    exps = {n: torch.full((2, 1, page), 127, dtype=torch.uint8, device=DEV) for n in ("k_exp", "v_exp")} if cache8 else {}
+    table = torch.zeros(1, whole + 1, dtype=torch.int32, device=DEV)
+    table[0, whole] = 1
+    kv = torch.full((B,), whole * page + last, dtype=torch.int32, device=DEV)
+    q = torch.ones(B, H, D, dtype=BF, device=DEV)
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    out, lse = abi.paged_attention(q, k, v, table.expand(B, -1), kv, cu_of([1] * B), 1, scale=1 / 8.0, return_lse=True, **exps)
+    end.record()
+    torch.cuda.synchronize()
+    assert abi.paged_attn_last_kernel() == "paged_tcgen05"
+    abi.paged_attention(q, k, v, table.expand(B, -1), torch.ones_like(kv), cu_of([1] * B), 1, scale=1 / 8.0, **exps)      # (would report a wait that ran out)
+    want = v[1, 0, :last, 0].cpu().double().mean()          # (the zeros weigh 2^26 e^-64 of a key)
+    u = torch.finfo(BF).eps / 2
+    assert ((out.cpu().double() - want).abs() <= 2 * u * want).all()
+    assert ((lse.cpu().double() - (64 + torch.tensor(float(last)).double().log())).abs() <= 1e-4).all()
+    assert start.elapsed_time(end) > 400      # (twice the limit of a wait: the case is what it claims to be)

@@ -742,6 +742,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (p.wait_late) asm volatile("griddepcontrol.wait;" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) {
+        drain_after_abort();
         *p.status = *abort_flag;
         __threadfence_system();
     }

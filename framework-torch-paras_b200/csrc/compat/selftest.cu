@@ -26,6 +26,7 @@ __global__ void bounded_wait_selftest_kernel(int* status, uint64_t limit_ns) {
         ok = tc::mbar_wait(tc::smem_u32(&barrier_word), 0, &abort_flag, kSelftestTag, limit_ns);
     __syncthreads();
     if (threadIdx.x == 0 && !ok) {
+        tc::drain_after_abort();
         *status = abort_flag;
         __threadfence_system();
     }

@@ -108,6 +108,13 @@ __device__ __forceinline__ bool mbar_wait_progress(uint32_t bar, uint32_t parity
     return true;
 }
 
+// For the exit of a CTA whose wait ran out: loads and MMAs that it issued may still be on their way into its shared memory
+// and TMEM, which the next CTA of the SM would get.  Gives them a millisecond; they take microseconds.
+constexpr uint64_t kDrainNs = 1000000ull;
+__device__ __forceinline__ void drain_after_abort() {
+    for (const uint64_t t0 = global_timer_ns(); global_timer_ns() - t0 < kDrainNs;) __nanosleep(10000);
+}
+
 // ---- TMA: 4-D tiled load global -> shared, completion on an mbarrier -------------------
 __device__ __forceinline__ void tma_load_4d(uint32_t dst_smem, const CUtensorMap* map,
                                             uint32_t bar, int c0, int c1, int c2, int c3) {

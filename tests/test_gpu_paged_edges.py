@@ -104,3 +104,15 @@ def test_an_item_that_lasts_longer_than_any_wait(cache8):
     assert ((out.cpu().double() - want).abs() <= 2 * u * want).all()
     assert ((lse.cpu().double() - (64 + torch.tensor(float(last)).double().log())).abs() <= 1e-4).all()
     assert start.elapsed_time(end) > 400      # (twice the limit of a wait: the case is what it claims to be)
+
+
+def test_a_block_that_gives_up_leaves_its_copies_time_to_land():
+    # the exit of the chunk and streaming kernels and of the self-test kernel, whose wait runs out after 0.2 ms
+    import time
+    abi.selftest_bounded_wait(0, 200)
+    t0 = time.perf_counter()
+    status, word = abi.selftest_bounded_wait(0, 200)
+    assert status == -6 and word & (1 << 27)
+    assert time.perf_counter() - t0 >= 1.2e-3
+    check = torch.ones(4, device=DEV).sum()
+    assert check.item() == 4

@@ -4,12 +4,14 @@
 //
 //   h = T(x + r)      the sum every later layer sees, so the statistics are taken of the rounded value and the
 //                     backward pass needs h alone
-//   rstd = 1 / sqrt(mean(h^2) + eps)          sums in fp32 per thread (at most 32 squares each), in double across them
+//   rstd = 1 / sqrt(mean(h^2) + eps)          sums in fp32 per thread (at most 32 squares each), in double across them;
+//                                             a row too large or too small for fp32 squares again, in double
 //   y = h * rstd * w                          fp32, rounded once: to T, or to e4m3 of y / scale
 //   scale = max(max|y| / 448, 2^-126)         over a row or over 32 / 64 / 128 columns
 //
 // Backward, with n = h * rstd and a = grad_y * w:
 //   grad_x = rstd * (a - n * mean(a * n)) + grad_h          grad_w = sum over rows of grad_y * n
+// evaluated in this order, in which everything but the result is near grad_y's size whatever h's is.
 //
 // Measured, bf16: 16384 x 4096 forward 81 us (6.65 TB/s), with 8-bit output by 128 columns 71.6 us (6.6 TB/s), backward 87 us
 // (6.1 TB/s); 64 x 4096 with 8-bit output 2.9 us; 8192 x 5000 forward 51 us and backward 61 us with grad_w.
@@ -88,9 +90,32 @@ __device__ __forceinline__ void store_quad(void* p, int64_t i, const Quad& q) {
 constexpr float kScaleMin = 1.1754943508222875e-38f;   // 2^-126
 __device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax * (1.0f / 448.0f), kScaleMin); }
 
+// Squares are summed in fp32 first, which is right unless magnitudes reach 2^63 (infinite squares, rstd = 0) or the mean square
+// with eps lies below 2^-100 (a square is off by up to 2^-150).  Such a row is told by its rstd and summed again in double.
+__device__ __forceinline__ bool fp32_squares_fail(float rstd) { return !(rstd > 0.f && rstd <= 1125899906842624.f); }      // 2^50
+
+// The squares of a thread's pieces of `N` consecutive elements of a row; not inlined, so that the usual path keeps its registers.
+template <typename T, int N>
+__device__ __noinline__ double squares_in_double(const T* row, int H, int tid, int threads) {
+    double sum = 0.0;
+#pragma unroll 1
+    for (int j = tid * N; j < H; j += threads * N)
+#pragma unroll 1
+        for (int e = 0; e < N; ++e) {
+            const double f = to_f32<T>(row[j + e]);
+            sum += f * f;
+        }
+    return sum;
+}
+
 // TPR threads hold a row in registers, V vectors of 16 bytes each (rows whole and aligned in such vectors).
+// (blocks an SM: as many as the registers that a row of V vectors takes leave room for; with two registers more a thread rows of 200
+// bf16 columns take 33.7 us for 30.8)
+constexpr int rows_blocks(int tpr, int v, bool quant) {
+    return tpr > 128 ? 1024 / tpr : tpr == 32 && v == 1 ? (quant ? 10 : 12) : v <= 2 && !quant ? 10 : 8;
+}
 template <typename T, int TPR, int V, bool QUANT>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR <= 128 ? 8 : 1024 / TPR)
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, rows_blocks(TPR, V, QUANT))
 add_rmsnorm_rows_kernel(const NormParams p) {
     using W = Word<T>;
     constexpr int E = W::E, N = 4 * E;
@@ -142,15 +167,22 @@ add_rmsnorm_rows_kernel(const NormParams p) {
                 for (int e = 0; e < E; ++e) ss = fmaf(f[e], f[e], ss);
             }
         }
-    double total = warp_sum(double(ss));
-    if constexpr (kW > 1) {
-        if (lane == 0) red[warp] = total;
-        __syncthreads();
-        total = 0.0;
+    auto rstd_of = [&](double part) {
+        part = warp_sum(part);
+        if constexpr (kW > 1) {
+            if (lane == 0) red[warp] = part;
+            __syncthreads();
+            part = 0.0;
 #pragma unroll
-        for (int i = 0; i < kW; ++i) total += red[i];
+            for (int i = 0; i < kW; ++i) part += red[i];
+        }
+        return float(1.0 / sqrt(part / double(p.H) + p.eps));
+    };
+    float rstd = rstd_of(double(ss));
+    if (fp32_squares_fail(rstd)) {       // (the same for the whole row, which each thread reads as it wrote it)
+        if constexpr (kW > 1) __syncthreads();
+        rstd = rstd_of(squares_in_double<T, N>(static_cast<const T*>(p.r ? p.h : p.x) + row * p.H, int(p.H), tid, TPR));
     }
-    const float rstd = float(1.0 / sqrt(total / double(p.H) + p.eps));
     if (p.rstd && tid == 0) p.rstd[row] = rstd;
     // y of word k of vector i.  (The 8-bit form needs it twice, for the maxima and for the result: keeping it would cost 32
     // registers and with them loads in flight.)
@@ -243,8 +275,9 @@ add_rmsnorm_rows_kernel(const NormParams p) {
 // Rows that are not whole 16-byte vectors, or not aligned: TPR threads hold a row in registers as single columns, thread t
 // columns t, t + TPR, ...  Loads and stores of two bytes a lane, 64 a warp, are half as fast as vectors; rows need not
 // start anywhere in particular.
+// (48 registers for the rows of up to 256 columns, as without the second sum; 0: left to the compiler)
 template <typename T, int TPR, int V, bool QUANT>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 && V == 8 ? 10 : 0)
 add_rmsnorm_cols_kernel(const NormParams p) {
     constexpr int kW = TPR / 32, kRows = TPR < 128 ? 128 / TPR : 1;
     static_assert(kRows == 1 || kW == 1, "several rows a block: a warp each");
@@ -281,15 +314,29 @@ add_rmsnorm_cols_kernel(const NormParams p) {
         const float f = to_f32<T>(hv[i]);
         ss = fmaf(f, f, ss);
     }
-    double total = warp_sum(double(ss));
-    if constexpr (kW > 1) {
-        if (lane == 0) red[warp] = total;
-        __syncthreads();
-        total = 0.0;
+    auto rstd_of = [&](double part) {
+        part = warp_sum(part);
+        if constexpr (kW > 1) {
+            if (lane == 0) red[warp] = part;
+            __syncthreads();
+            part = 0.0;
 #pragma unroll
-        for (int i = 0; i < kW; ++i) total += red[i];
+            for (int i = 0; i < kW; ++i) part += red[i];
+        }
+        return float(1.0 / sqrt(part / double(p.H) + p.eps));
+    };
+    float rstd = rstd_of(double(ss));
+    if (fp32_squares_fail(rstd)) {
+        if constexpr (kW > 1) __syncthreads();
+        double sd = 0.0;
+        if constexpr (kW == 1) {      // (a call costs the narrowest rows a tenth; so does this code the others)
+#pragma unroll
+            for (int i = 0; i < V; ++i) sd += double(to_f32<T>(hv[i])) * double(to_f32<T>(hv[i]));
+        } else {
+            sd = squares_in_double<T, 1>(static_cast<const T*>(p.r ? p.h : p.x) + at, H, tid, TPR);
+        }
+        rstd = rstd_of(sd);
     }
-    const float rstd = float(1.0 / sqrt(total / double(p.H) + p.eps));
     if (p.rstd && tid == 0) p.rstd[row] = rstd;
     auto yv = [&](int i) { return to_f32<T>(hv[i]) * rstd * to_f32<T>(wv[i]); };
     if constexpr (!QUANT) {
@@ -468,6 +515,25 @@ template <int LEFT> __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 
+// mean(a * n) is summed as rstd times a sum of a * h, which stays in fp32's range while rstd is within 2^-40 .. 2^40; other rows are
+// summed as the definition has it, a product more an element (8192 x 5000 bf16: 62 us this way, 70 with that product for all).
+__device__ __forceinline__ bool far_from_one(float rstd) { return !(rstd >= 9.094947017729282e-13f && rstd <= 1099511627776.f); }
+
+// a * n over a thread's pieces of `N` consecutive elements of a row.
+template <typename T, int N>
+__device__ __forceinline__ float normed_dot(const T* gy, const T* h, const T* w, float rstd, int H, int tid, int threads) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int j = tid * N; j < H; j += threads * N)
+#pragma unroll 1
+        for (int e = j; e < j + N; ++e) sum = fmaf(to_f32<T>(gy[e]) * (w ? to_f32<T>(w[e]) : 1.0f), to_f32<T>(h[e]) * rstd, sum);
+    return sum;
+}
+template <typename T, int N>
+__device__ __noinline__ float normed_dot_call(const T* gy, const T* h, const T* w, float rstd, int H, int tid, int threads) {
+    return normed_dot<T, N>(gy, h, w, rstd, H, tid, threads);
+}
+
 struct BwdParams {
     const void *gy, *gh, *h, *w;
     const float* rstd;
@@ -546,13 +612,19 @@ add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
                 }
             }
         }
+        dot *= rr;
+        if (far_from_one(rr)) {
+            const T *g0 = reinterpret_cast<const T*>(buf), *x0 = reinterpret_cast<const T*>(buf + kOne / 16), *w0 = static_cast<const T*>(p.w);
+            // (4 vectors a thread: a call leaves them in registers, 8192 x 8192 bf16 97 us for 103; fewer are held up by it, 8192 x 5000 71 for 63)
+            dot = V == 4 ? normed_dot_call<T, N>(g0, x0, w0, rr, int(p.H), tid, THREADS) : normed_dot<T, N>(g0, x0, w0, rr, int(p.H), tid, THREADS);
+        }
         dot = warp_sum(dot);
         if (lane == 0) red[flip][warp] = dot;
         __syncthreads();      // (two buffers in turn: the next row's writes cannot overtake these reads)
         dot = 0.f;
 #pragma unroll
         for (int i = 0; i < THREADS / 32; ++i) dot += red[flip][i];
-        const float coef = rr * rr * (inv_h * dot) * rr;
+        const float mean = inv_h * dot;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = i * THREADS + tid;
@@ -568,8 +640,9 @@ add_rmsnorm_bwd_rows_kernel(const BwdParams p) {
                     W::get(a.w[k], ae);
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        oe[e] = fmaf(ge[e] * we[e], rr, fmaf(-coef, xe[e], ae[e]));
-                        dw[i * N + k * E + e] = fmaf(ge[e] * xe[e], rr, dw[i * N + k * E + e]);
+                        const float n = xe[e] * rr;
+                        oe[e] = fmaf(fmaf(-n, mean, ge[e] * we[e]), rr, ae[e]);
+                        dw[i * N + k * E + e] = fmaf(ge[e], n, dw[i * N + k * E + e]);
                     }
                     o.w[k] = W::put(oe);
                 }
@@ -632,6 +705,12 @@ add_rmsnorm_bwd_cols_kernel(const BwdParams p) {
         float dot = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) dot = fmaf(to_f32<T>(fg[i]) * to_f32<T>(wv[i]), to_f32<T>(fx[i]), dot);
+        dot *= rr;
+        if (far_from_one(rr)) {
+            dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) dot = fmaf(to_f32<T>(fg[i]) * to_f32<T>(wv[i]), to_f32<T>(fx[i]) * rr, dot);
+        }
         dot = warp_sum(dot);
         if constexpr (kSubs == 1) {
             if (lane == 0) red[flip][warp] = dot;
@@ -641,13 +720,13 @@ add_rmsnorm_bwd_cols_kernel(const BwdParams p) {
             for (int i = 0; i < THREADS / 32; ++i) dot += red[flip][i];
             flip ^= 1;
         }
-        const float coef = rr * rr * (inv_h * dot) * rr;
+        const float mean = inv_h * dot;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int j = i * THREADS + tid;
-            const float ge = to_f32<T>(fg[i]), xe = to_f32<T>(fx[i]);
-            if (j < H) static_cast<T*>(p.gx)[row * p.H + j] = from_f32<T>(fmaf(ge * to_f32<T>(wv[i]), rr, fmaf(-coef, xe, to_f32<T>(fa[i]))));
-            dw[i] = fmaf(ge * xe, rr, dw[i]);
+            const float ge = to_f32<T>(fg[i]), n = to_f32<T>(fx[i]) * rr;
+            if (j < H) static_cast<T*>(p.gx)[row * p.H + j] = from_f32<T>(fmaf(fmaf(-n, mean, ge * to_f32<T>(wv[i])), rr, to_f32<T>(fa[i])));
+            dw[i] = fmaf(ge, n, dw[i]);
         }
     };
     fetch(walker, g, x, a);
@@ -687,12 +766,11 @@ add_rmsnorm_bwd_dx_kernel(const BwdParams p) {
         __syncthreads();
         dot = 0.0;
         for (int i = 0; i < 8; ++i) dot += red[i];
-        const double rr = p.rstd[row];
-        const float coef = float(rr * rr * rr * dot / double(p.H)), r1 = float(rr);
+        const float rr = p.rstd[row], mean = float(dot * double(rr) / double(p.H));
         T* out = static_cast<T*>(p.gx) + row * p.H;
         for (int64_t j = tid; j < p.H; j += 256) {
             const float a = to_f32<T>(gy[j]) * (w ? to_f32<T>(w[j]) : 1.0f);
-            out[j] = from_f32<T>(fmaf(a, r1, -coef * to_f32<T>(h[j])) + (gh ? to_f32<T>(gh[j]) : 0.f));
+            out[j] = from_f32<T>(fmaf(fmaf(-(to_f32<T>(h[j]) * rr), mean, a), rr, gh ? to_f32<T>(gh[j]) : 0.f));
         }
         __syncthreads();
     }

@@ -469,7 +469,8 @@ const char* paras_b200_paged_attn_last_kernel(void);
  * (pointwise_ops.cpp:62-85, fused_ops.cpp:43-88).  All tensors [rows, H] contiguous.
  *   h = x + residual, rounded to `dtype` (residual NULL: h is x and is not written)
  *   y = h * rstd * weight,  rstd = 1 / sqrt(mean(h^2) + eps) of the rounded h        (weight NULL: ones)
- * _fwd writes y rounded once to `dtype`, h, and rstd (optional, fp32 [rows]).
+ * _fwd writes y rounded once to `dtype`, h, and rstd (optional, fp32 [rows]).  Any finite h is in range as long as rstd
+ * fits fp32 (mean(h^2) + eps of at least 2^-254).
  * _quant_fwd writes y in 8 bits instead, y ~ e4m3 * scale: one fp32 scale per row (group = 0) or per `group` = 32, 64
  * or 128 consecutive columns (the last group of a row may be shorter), scales [rows, ceil(H / group)] contiguous,
  * scale = max |y| / 448, at least 2^-126; y is not rounded to 16 bits in between.  The maximum skips NaN, which stays NaN.

@@ -96,7 +96,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     tdir = os.path.dirname(torch.__file__)
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    hdrs = _headers(os.path.join(CSRC, "core"), INCLUDE)
+    hdrs = _headers(os.path.join(CSRC, "core"), os.path.join(CSRC, "ops"), INCLUDE)
     out = os.path.join(PKG, "_C.so")
     flags = ["-std=c++17", "-O2", "-fPIC", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
              "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_C",

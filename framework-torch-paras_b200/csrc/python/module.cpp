@@ -50,7 +50,10 @@ PYBIND11_MODULE(_C, m) {
     m.def("paged_kv_read", [](const T& k_cache, const T& v_cache, const T& page_table, const T& cu_kv, int64_t total, const py::object& dtype,
                               const O& k_exp, const O& v_exp, const O& out_k, const O& out_v, int64_t stream) {
         std::optional<c10::ScalarType> to;
-        if (!dtype.is_none()) to = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+        if (!dtype.is_none()) {
+            if (!THPDtype_Check(dtype.ptr())) throw py::type_error("paras paged_kv_read: dtype must be a torch.dtype");
+            to = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+        }
         return paras::paged_kv_read(k_cache, v_cache, page_table, cu_kv, total, to, k_exp, v_exp, out_k, out_v, stream);
     });
     m.def("paged_attention", [](const T& q, const T& k_cache, const T& v_cache, const T& page_table, const T& kv_lens, const T& cu_q,

@@ -49,3 +49,11 @@ def test_the_widest_table_is_taken(page, max_pages):
         args.cache.page, args.cache.max_pages, args.cache.k = page, max_pages, None
         assert call() == -1
         assert "null cache" in abi.lib().paras_b200_last_error().decode()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", 15, float, object()])
+def test_a_dtype_that_is_none_is_refused(dtype):
+    import torch
+    pool, table = torch.zeros(2, 1, 16, 64), torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.raises(TypeError, match="torch.dtype"):
+        abi.paged_kv_read(pool, pool, table, torch.zeros(2, dtype=torch.int32), 4, dtype=dtype)

@@ -130,6 +130,7 @@ std::tuple<Tensor, Tensor> paged_kv_read(const Tensor& k_cache, const Tensor& v_
     const auto to = dtype.value_or(k_cache.scalar_type() == c10::kFloat8_e4m3fn ? c10::kBFloat16 : k_cache.scalar_type());
     TORCH_CHECK(dtype_code(to) >= 0, "paras paged_kv_read: unsupported dtype ", to);
     Tensor k, v;
+    TORCH_CHECK(out_k.has_value() == out_v.has_value(), "paras paged_kv_read: the outputs are given both or not at all");
     if (out_k && out_v) {
         k = *out_k;
         v = *out_v;
@@ -137,6 +138,7 @@ std::tuple<Tensor, Tensor> paged_kv_read(const Tensor& k_cache, const Tensor& v_
                         rows_of(v, k_cache.size(1), k_cache.size(3), what, "v").is_same(v) && k.size(0) == total && v.size(0) == total &&
                         v.scalar_type() == k.scalar_type() && k.device() == k_cache.device() && v.device() == k.device(),
                     "paras paged_kv_read: the two outputs must have one type, the cache's device, contiguous rows and `total` of them");
+        TORCH_CHECK(!dtype || *dtype == k.scalar_type(), "paras paged_kv_read: the outputs have type ", k.scalar_type(), ", not the dtype asked for");
     } else {
         k = at::empty({total, k_cache.size(1), k_cache.size(3)}, k_cache.options().dtype(to));
         v = at::empty_like(k);

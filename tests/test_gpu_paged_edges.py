@@ -116,3 +116,20 @@ def test_a_block_that_gives_up_leaves_its_copies_time_to_land():
     assert time.perf_counter() - t0 >= 1.2e-3
     check = torch.ones(4, device=DEV).sum()
     assert check.item() == 4
+
+
+def test_outputs_that_are_given_to_the_reader():
+    c = Cache([40, 20], 2, 64, 16, BF, True)
+    k, v = (torch.full((60, 2, 64), 5.0, dtype=HF, device=DEV) for _ in range(2))
+    args = (*c.cache, c.table, cu_of([40, 20]), 60)
+    with pytest.raises(RuntimeError, match="not the dtype asked for"):
+        abi.paged_kv_read(*args, dtype=BF, out=(k, v), **c.kw)
+    for out in ((k, None), (None, v)):
+        with pytest.raises(RuntimeError, match="both or not at all"):
+            abi.paged_kv_read(*args, out=out, **c.kw)
+    assert bool((k == 5).all()) and bool((v == 5).all())
+    want = abi.paged_kv_read(*args, dtype=HF, **c.kw)
+    for dtype in (None, HF):
+        got = abi.paged_kv_read(*args, dtype=dtype, out=(k, v), **c.kw)
+        assert got[0].data_ptr() == k.data_ptr() and torch.equal(k, want[0]) and torch.equal(v, want[1])
+        k.zero_()

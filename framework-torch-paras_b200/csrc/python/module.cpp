@@ -46,6 +46,7 @@ PYBIND11_MODULE(_C, m) {
     // The calls of torch_paras.abi on torch.cuda tensors (`stream`: raw handle) that are short enough for Python's checks to show.
     using T = at::Tensor;
     using O = paras::OptTensor;
+    m.def("paged_attn_last_kernel", [] { return std::string(paras_b200_paged_attn_last_kernel()); });
     m.def("paged_kv_write", &paras::paged_kv_write);
     m.def("paged_kv_read", [](const T& k_cache, const T& v_cache, const T& page_table, const T& cu_kv, int64_t total, const py::object& dtype,
                               const O& k_exp, const O& v_exp, const O& out_k, const O& out_v, int64_t stream) {

@@ -12,7 +12,8 @@ import os
 
 import torch
 
-# PARAS_B200_LIB points the bindings at another build of the library (e.g. a tuning variant).
+# PARAS_B200_LIB points the ctypes bindings at another build of the library (e.g. a tuning variant); the paged cache's and the
+# residual norm's calls below, which go through `_C`, always run the one that `_C` is linked to.
 _LIB_PATH = os.environ.get("PARAS_B200_LIB") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), "libparas_b200.so")
 
@@ -626,7 +627,7 @@ def paged_attn_workspace_bytes(q, k_cache, v_cache, page_table, kv_lens, cu_q, m
 
 
 def paged_attn_last_kernel() -> str:
-    return lib().paras_b200_paged_attn_last_kernel().decode()
+    return (_C or _c()).paged_attn_last_kernel()
 
 
 def add_rmsnorm_fwd(x, residual, weight, eps=1e-6, *, return_rstd=False, stream=None):

@@ -133,3 +133,22 @@ def test_outputs_that_are_given_to_the_reader():
         got = abi.paged_kv_read(*args, dtype=dtype, out=(k, v), **c.kw)
         assert got[0].data_ptr() == k.data_ptr() and torch.equal(k, want[0]) and torch.equal(v, want[1])
         k.zero_()
+
+
+def test_the_last_kernel_is_that_of_the_library_that_ran(tmp_path):
+    # with the ctypes bindings pointed at another build, the paged calls still run, and report on, the one `_C` is linked to
+    import os
+    import shutil
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    package = os.path.dirname(os.path.dirname(abi.__file__))
+    other = shutil.copy(os.path.join(package, "torch_paras", "libparas_b200.so"), tmp_path / "libother.so")
+    code = ("import torch, torch_paras\nfrom torch_paras import abi\nfrom paged_cases import Cache, cu_of\n"
+            "c = Cache([300], 2, 64, 16, torch.bfloat16, False)\nq = torch.ones(1, 4, 64, dtype=torch.bfloat16, device='cuda:0')\n"
+            "abi.paged_attention(q, *c.cache, c.table, c.kv_lens, cu_of([1]), 1)\ntorch.cuda.synchronize()\n"
+            "print(abi._LIB_PATH, abi.paged_attn_last_kernel())\n")
+    env = dict(os.environ, PARAS_B200_LIB=str(other), PYTHONPATH=os.pathsep.join([package, here]))
+    out = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr
+    assert out.stdout.split() == [str(other), "paged_decode"]

@@ -39,19 +39,24 @@ struct PagedParams {
 struct PagedSeq {
     int row0, nq;
     int kv;       // positions 0 .. kv-1, kv <= cap
-    int pos0;     // position of the first new token (may be negative or past kv); pos0 + count is kv_lens[b] or negative
+    int pos0;     // position of the first new token (may be negative or past kv); pos0 + nq is at most kv_lens[b]
 };
-__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
+// From cu[b], cu[b+1] and kv_lens[b].  A row's position is kv_lens[b] - cu[b+1] + row, also of a sequence that goes on past the last
+// row there is; below -2^31 any negative position is as good.
+__host__ __device__ __forceinline__ PagedSeq paged_place(const PagedParams& p, int c0, int c1, int kv) {
     PagedSeq s;
-    const int c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1), kv = __ldg(p.kv_lens + b);
-    s.row0 = max(0, min(c0, p.T));
-    const int end = max(s.row0, min(c1, p.T));
+    s.row0 = c0 < 0 ? 0 : c0 < p.T ? c0 : p.T;
+    const int end = c1 < s.row0 ? s.row0 : c1 < p.T ? c1 : p.T;
     const int count = end - s.row0;
-    s.nq = min(count, p.max_q);
+    s.nq = count < p.max_q ? count : p.max_q;
     if (s.nq < p.q_min || s.nq > p.q_max) s.nq = 0;
-    s.kv = max(0, min(kv, p.cap));
-    s.pos0 = int(max(int64_t(-(1 << 30)), int64_t(kv) - count));
+    s.kv = kv < 0 ? 0 : kv < p.cap ? kv : p.cap;
+    const int64_t pos0 = int64_t(kv) - c1 + s.row0, least = -(int64_t(1) << 31);
+    s.pos0 = int(pos0 < least ? least : pos0);
     return s;
+}
+__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
+    return paged_place(p, __ldg(p.cu + b), __ldg(p.cu + b + 1), __ldg(p.kv_lens + b));
 }
 // Keys that new token i of the sequence attends: positions 0 .. n-1.
 __host__ __device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& s, int i) {

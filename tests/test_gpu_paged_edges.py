@@ -152,3 +152,19 @@ def test_the_last_kernel_is_that_of_the_library_that_ran(tmp_path):
     out = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0, out.stderr
     assert out.stdout.split() == [str(other), "paged_decode"]
+
+
+@pytest.mark.parametrize("cache8", [False, True])
+@pytest.mark.parametrize("dtype,q_lens,max_q", [(BF, [4, 4], 4), (BF, [40, 60], 60), (torch.float32, [4, 7], 7)], ids=["token", "chunk", "simt"])
+def test_a_sequence_that_goes_on_past_the_rows_there_are(dtype, q_lens, max_q, cache8):
+    # the rows of a longer batch that are there stand where they stood
+    kv = [n + 1 for n in q_lens]
+    c = Cache(kv, 2, 64, 16, dtype, cache8)
+    T = sum(q_lens)
+    q = rand(T, 4, 64, dtype=dtype, seed=1)
+    args = (*c.cache, c.table, c.kv_lens, cu_of(q_lens), max_q)
+    full = abi.paged_attention(q, *args, **c.kw)
+    for there in (T - 1, T - 3):
+        out = abi.paged_attention(q[:there], *args, **c.kw)
+        tol = 2 * torch.finfo(dtype).eps      # (shared out between other blocks: half a step of P and of the result, twice)
+        assert torch.allclose(out.float(), full[:there].float(), rtol=tol, atol=tol)

@@ -548,15 +548,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             float mx[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) mx[h] = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-            if (__any_sync(0xffffffffu, mx[0] > m_run[0] + lag[0] || mx[1] > m_run[1] + lag[1])) {
+            const bool over[2] = {mx[0] > m_run[0] + lag[0], mx[1] > m_run[1] + lag[1]};
+            if (__any_sync(0xffffffffu, over[0] || over[1])) {
                 float alpha[2];
+                uint32_t up = (over[0] ? 1u : 0u) | (over[1] ? 2u : 0u);
+                up |= __shfl_xor_sync(0xffffffffu, up, 1);
+                up |= __shfl_xor_sync(0xffffffffu, up, 2);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
                     // a row goes by its own scores: its bits depend neither on its neighbours nor on the rows of the tile of
                     // queries that no token fills, which hold anything
-                    const float m_new = mx[h] > m_run[h] + lag[h] ? mx[h] : m_run[h];
+                    const float m_new = (up >> h) & 1u ? mx[h] : m_run[h];
                     alpha[h] = m_new == m_run[h] ? 1.f : ex2_approx((m_run[h] - m_new) * c2[h]);
                     l_run[h] *= alpha[h];
                     m_run[h] = m_new;

@@ -853,8 +853,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    if (*abort_flag) drain_after_abort();
-    if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+    if (warp == kMmaWarp) {
+        if (*abort_flag) drain_after_abort();
+        tmem_dealloc(tmem, 512);
+    }
     if (threadIdx.x == 0 && *abort_flag) {
         *p.status = *abort_flag;
         __threadfence_system();

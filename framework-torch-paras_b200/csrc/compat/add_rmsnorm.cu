@@ -13,8 +13,9 @@
 //   grad_x = rstd * (a - n * mean(a * n)) + grad_h          grad_w = sum over rows of grad_y * n
 // evaluated in this order, in which everything but the result is near grad_y's size whatever h's is.
 //
-// Measured, bf16: 16384 x 4096 forward 81 us (6.65 TB/s), with 8-bit output by 128 columns 71.6 us (6.6 TB/s), backward 87 us
-// (6.1 TB/s); 64 x 4096 with 8-bit output 2.9 us; 8192 x 5000 forward 51 us and backward 61 us with grad_w.
+// Measured, bf16: 16384 x 4096 forward 81 us (6.65 TB/s), with 8-bit output by 128 columns 72 us (6.6 TB/s), backward 88 us
+// (6.1 TB/s); 64 x 4096 with 8-bit output 2.9 us; 8192 x 5000 forward 51 us and backward 63 us with grad_w; rows that are summed again
+// in double only where they occur.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -87,6 +88,8 @@ __device__ __forceinline__ void store_quad(void* p, int64_t i, const Quad& q) {
     __stcs(static_cast<uint4*>(p) + i, *reinterpret_cast<const uint4*>(&q));
 }
 
+// The 8-bit form multiplies by reciprocals, each rounded once: a y within 2^-23 of the border between two e4m3 steps may fall on the
+// other one.
 constexpr float kScaleMin = 1.1754943508222875e-38f;   // 2^-126
 __device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax * (1.0f / 448.0f), kScaleMin); }
 

@@ -17,9 +17,9 @@
 // the 16-bit type that multiplies V, as in the dense kernels; maxima, sums and accumulators are fp32.
 //
 // Measured (32 query heads over 8 kv heads of 128).  64 single tokens over 512 .. 16384 positions, bf16: 340 to 346 us with
-// pages of 64 or 16, 6.5 TB/s, what a copy gets; 256 over 200 .. 1000 118 us (5.4 TB/s), 128 over 100 .. 300 44 us, where items'
+// pages of 64 or 16, 6.5 TB/s, what a copy gets; 256 over 200 .. 1000 120 us (5.3 TB/s), 128 over 100 .. 300 45 to 47 us, where items'
 // starts and ends count.  One token over 1000 positions: 12 us with the join, all latency.
-// 48 x 4 tokens over up to 8192 positions of an 8-bit cache: 122 us, 3.5 TB/s (a 16-bit one 144): there the consumers'
+// 48 x 4 tokens over up to 8192 positions of an 8-bit cache: 124 us, 3.5 TB/s (a 16-bit one 149): there the consumers'
 // instructions bound it, not the memory.  A warp's part of a tile takes 1440 cycles, at 442 instructions and two warps on a
 // scheduler, and about 300 go by around it, where the loads alone would allow 1350.  Twelve consumer warps do not fit (128
 // registers a thread: 173 us), e4m3 by shifts instead of conversions costs more instructions than it saves (157 us; half and
@@ -543,7 +543,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         for (int e = 0; e < 2; ++e)
                             if (kb + nt * kStep + e >= lim[h] || !(nt ? here1 : here0)) sc[nt][2 * h + e] = -INFINITY;
             }
-            // The reference m of a row lags behind its maximum: it moves when a score has outgrown it by 2^8 (P stays far
+            // The reference m of a row lags behind its maximum: it moves when a score of the row has outgrown it by 2^8 (P stays far
             // inside 16 bits), which after an item's first tiles is rare, so that a tile usually needs no exchange between lanes.
             float mx[2];
 #pragma unroll

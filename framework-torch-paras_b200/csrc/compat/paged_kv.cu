@@ -10,7 +10,7 @@
 // found by the warp (warp_count_le) while the row's loads are in flight.
 //
 // Measured (8 kv heads of 128, pages of 64): write of 4 x 4096 tokens 21.1 us as bf16 (5.9 TB/s), 19.1 us into 8 bits
-// (4.9 TB/s; bound by instructions before the rows stayed in pairs of 16 bits: 25.3 us); one token for each of 64
+// (4.9 TB/s; bound by instruction issue, DRAM at 42 % and SM at 64 %; 25.3 us before the rows stayed in pairs of 16 bits); one token for each of 64
 // sequences 2.6 us; read of 16 sequences of up to 8192 from 8 bits 61.4 us (5.8 TB/s), of one of 1500 as bf16 3.8 us.
 #include "paged_common.cuh"
 

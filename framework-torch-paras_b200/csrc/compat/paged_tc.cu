@@ -23,7 +23,7 @@
 // brought to fp16 in shared memory, scaled by a power of two per row (see paged_decode.cu).
 //
 // Measured (32 query heads over 8 kv heads of 128, causal, bf16): 2 x 2048 tokens at the end of 6000 .. 8192 positions 330 us
-// (1100 TFLOP/s; 380 when run back to back for long, under the power cap), 2 x 128 over 16384 91 us, 64 over 1024 19 us.
+// (1100 TFLOP/s; 380 when run back to back for long, under the power cap), 2 x 128 over 16384 84 us, 64 over 1024 19 us.
 // As in the dense kernel the chain S -> softmax -> P -> O of the two query tiles bounds it.  Ranges in several rounds, so
 // that all CTAs read the same few kv heads at a time, cost more in cut items than the L2 gave back up to 134 MB of keys and
 // values (64 heads, 2 x 1024 over 8192: 466 for 435 us) and won 10 % at 268 MB: not kept.

@@ -438,7 +438,8 @@ int paras_b200_paged_kv_read(const paras_paged_kv_args* args);
  * of the new tokens themselves have to be in the cache already.  max_q bounds the new tokens of a sequence (queries
  * past it are not computed); the route is chosen by it.  A query that attends nothing (no position left, all
  * pages absent) gives zeros, with lse = -inf.  What lies in the cache past a sequence's last position is never used,
- * whatever it holds; K and V of the attended positions have to be finite; a NaN in q makes its own row NaN.  `lse` (optional): fp32 [T, Hq] contiguous,
+ * whatever it holds; K and V of the attended positions have to be finite, and scores within fp32's range, before and after the scale; a NaN
+ * in q makes its own row NaN.  `lse` (optional): fp32 [T, Hq] contiguous,
  * natural log of the sum of the exponentials of the scaled scores.  dtype F32, BF16 or F16; cache_dtype the same or
  * PARAS_E4M3.  D up to 256.  `workspace`: as for paras_b200_sdpa_fwd; size from paras_b200_paged_attn_workspace_bytes. */
 typedef struct paras_paged_attn_args {
@@ -473,7 +474,8 @@ const char* paras_b200_paged_attn_last_kernel(void);
  * fits fp32 (mean(h^2) + eps of at least 2^-254).
  * _quant_fwd writes y in 8 bits instead, y ~ e4m3 * scale: one fp32 scale per row (group = 0) or per `group` = 32, 64
  * or 128 consecutive columns (the last group of a row may be shorter), scales [rows, ceil(H / group)] contiguous,
- * scale = max |y| / 448, at least 2^-126; y is not rounded to 16 bits in between.  The maximum skips NaN, which stays NaN.
+ * scale = max |y| / 448, at least 2^-126; y is not rounded to 16 bits in between (scale and y / scale by fp32 reciprocals).  The maximum
+ * skips NaN, which stays NaN.
  * h may be the memory of x or of residual; no other two tensors may overlap.
  * _bwd: the gradients of _fwd from grad_y and grad_h (the gradient that arrives at h, NULL: none): grad_x is the
  * gradient of x and of residual alike, grad_weight [H] in `dtype` (NULL with weight NULL). */

@@ -439,7 +439,8 @@ int paras_b200_paged_kv_read(const paras_paged_kv_args* args);
  * past it are not computed); the route is chosen by it.  A query that attends nothing (no position left, all
  * pages absent) gives zeros, with lse = -inf.  What lies in the cache past a sequence's last position is never used,
  * whatever it holds; K and V of the attended positions have to be finite, and scores within fp32's range, before and after the scale; a NaN
- * in q makes its own row NaN.  `lse` (optional): fp32 [T, Hq] contiguous,
+ * in q makes its own row NaN.  16-bit routes round the weights, relative to the row's reference, to the type that multiplies V before that
+ * product: `dtype`, or fp16 over an 8-bit cache, where a weight is off by up to 2^-25 however small it is.  `lse` (optional): fp32 [T, Hq] contiguous,
  * natural log of the sum of the exponentials of the scaled scores.  dtype F32, BF16 or F16; cache_dtype the same or
  * PARAS_E4M3.  D up to 256.  `workspace`: as for paras_b200_sdpa_fwd; size from paras_b200_paged_attn_workspace_bytes. */
 typedef struct paras_paged_attn_args {

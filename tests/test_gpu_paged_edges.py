@@ -168,3 +168,26 @@ def test_a_sequence_that_goes_on_past_the_rows_there_are(dtype, q_lens, max_q, c
         out = abi.paged_attention(q[:there], *args, **c.kw)
         tol = 2 * torch.finfo(dtype).eps      # (shared out between other blocks: half a step of P and of the result, twice)
         assert torch.allclose(out.float(), full[:there].float(), rtol=tol, atol=tol)
+
+
+@pytest.mark.parametrize("q_lens", [[1, 2], [1, 60]], ids=["token", "chunk"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_what_the_heaviest_key_adds_nothing_to(dtype, q_lens):
+    # scores so far apart that a row is nearly one key's, whose value is zero in every fourth column: what is left there are weights
+    # down to nothing, which fp16 holds to 2^-25 of the reference, each times its value
+    kv = [300, 200]
+    c = Cache(kv, 1, 128, 16, dtype, True, seed=4)
+    for b in range(2):
+        c.dense[1][b][:, :, ::4] *= (torch.arange(kv[b]) % 2)[:, None, None]
+        pos = torch.arange(kv[b])
+        where, off = c.table[b].long().cpu()[pos // 16], pos % 16
+        raw = c.cache[1].view(torch.uint8)
+        row = raw[where, :, off]
+        row[::2, :, ::4] = 0
+        raw[where, :, off] = row
+    q = rand(sum(q_lens), 4, 128, dtype=dtype, seed=5, scale=20.0)
+    out = abi.paged_attention(q, *c.cache, c.table, c.kv_lens, cu_of(q_lens), max(q_lens), **c.kw)
+    want, _, A, S = attend64(q, c, q_lens, kv, 128 ** -0.5)
+    small = torch.cat([c.dense[1][b].abs().sum(0).expand(n, 4, 128) for b, n in enumerate(q_lens)])
+    tol = attend_tolerance(want, A, S, dtype, 128, max(kv)) + 2.0 ** -25 * small
+    assert ((out.cpu().double() - want).abs() <= tol).all()
